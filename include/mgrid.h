@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define MG_ABI_VERSION 8
+#define MG_ABI_VERSION 9
 
 /* error codes */
 #define MG_OK 0
@@ -295,6 +295,132 @@ int mg_launch_census(char *buf, int32_t size);
 int mg_episode_stats(int32_t num_envs, int32_t num_agents, const float *reward_dev, const uint8_t *terminated_dev,
                      const uint8_t *truncated_dev, double *return_acc_dev, int64_t *length_acc_dev, uint8_t *done_dev,
                      double *episode_return_dev, int64_t *episode_length_dev, void *stream);
+
+/* ---- between the simulator and a policy network -----------------------------------------------------------------
+ *
+ * What follows needs no handle: the embedding of what an environment shows (cells of an image, tokens of a mission
+ * text), and what a policy's logits go through until they are an answer (an action, a word).  The reference leaves
+ * these to its training libraries (multigrid/rllib/models.py:45); they
+ * stand here because their inputs and outputs are this simulator's.  All `_dev` pointers are device pointers on the
+ * stream's device, which has to be the calling thread's current one when `stream` is NULL; nothing is allocated, and
+ * nothing is kept from one call for the next, so every call may be captured into a HIP graph, and calls may overlap
+ * as long as they do not share a workspace or an output. */
+
+/* element types */
+#define MG_F32 0
+#define MG_BF16 1
+#define MG_F16 2
+#define MG_F64 3 /* uniform numbers only */
+#define MG_U8 0
+#define MG_I32 1
+#define MG_I64 2
+
+/* Embedding.  Every token has `fields` ids, field f's between 0 and sizes[f] - 1; the table holds sizes[0] rows for
+ * field 0, then sizes[1] for field 1, ... of `dim` elements each.
+ *     out[n] = scale * sum over f of table[sizes[0] + ... + sizes[f - 1] + id[n][f]]
+ * An id outside its field's range reads nothing (a token with none left gives zeros: padding).  A cell of an image is
+ * a token of three fields (type, colour, state: 11, 6, 7), for which this is the one-hot cell (onehot_dev) times the
+ * table; a word is a token of one field.  Sums are held in 32 bits and rounded once. */
+#define MG_MAX_FIELDS 8
+typedef struct MgEmbed {
+    int64_t n;                    /* tokens, 0 .. 2^31 - 1 */
+    int32_t fields;               /* 1 .. MG_MAX_FIELDS */
+    int32_t dim;                  /* 1 .. 2^24 */
+    int32_t ids_type;             /* MG_U8, MG_I32, MG_I64 */
+    int32_t dtype;                /* of table, output and gradients: MG_F32, MG_BF16, MG_F16 */
+    int64_t ids_stride;           /* elements from one token's ids to the next one's; 0 allowed */
+    int64_t field_stride;         /* elements from one id of a token to the next one */
+    int64_t row_stride;           /* elements from one row of the table (mg_embed), or of the incoming gradient
+                                     (mg_embed_grad), to the next; inside a row elements are adjacent */
+    int32_t sizes[MG_MAX_FIELDS]; /* every one positive, their sum at most 2^30 */
+    float scale;
+    int32_t reserved0;            /* must be 0 */
+} MgEmbed;
+
+/* out [n][dim], contiguous. */
+int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void *out_dev, void *stream);
+
+/* The table's gradient: table_grad [sum of sizes][dim], contiguous, every element written,
+ *     table_grad[r] = scale * sum of grad[n] over the tokens n that read row r.
+ * Sums are held in 32 bits in an order that depends on the arguments alone: the same call gives the same bits.
+ * `workspace_dev`: mg_embed_grad_workspace(e) bytes, 16-byte aligned (NULL where that is 0); it returns a negative
+ * MG_E* code for arguments that mg_embed_grad refuses. */
+int64_t mg_embed_grad_workspace(const MgEmbed *e);
+int mg_embed_grad(const MgEmbed *e, const void *ids_dev, const void *grad_dev, void *table_grad_dev,
+                  void *workspace_dev, int64_t workspace_bytes, void *stream);
+
+/* Adjustment of logits [n][k] before an answer is drawn.  With c = how often token j stands among the first
+ * lengths[i] entries of history[i] (entries outside 0 .. k - 1 count for nothing):
+ *     x = logit;  c > 0: x = (x > 0 ? x / repetition : x * repetition) - presence;
+ *     x = x - frequency * c + bias[j];  x = -inf where the mask bars j.
+ * Worked out in 32 bits, each operation rounded, and rounded to `dtype` once.  A row whose mask bars everything becomes
+ * -inf throughout.  What a barred place held (NaN, infinities) does not matter. */
+#define MG_MASK_NONE 0
+#define MG_MASK_BYTES 1 /* uint8 [n][k], non-zero = allowed */
+#define MG_MASK_BITS 2  /* uint32 [n][ceil(k / 32)], token j in bit j % 32 of word j / 32, set = allowed */
+typedef struct MgAdjust {
+    int64_t n;                   /* rows, 0 .. 2^31 - 1 */
+    int32_t k;                   /* tokens, 1 .. 2^24 */
+    int32_t dtype;               /* MG_F32, MG_BF16, MG_F16 */
+    int64_t logits_stride;       /* elements between rows of the logits */
+    int64_t out_stride;          /* ... of the output */
+    int64_t grad_stride;         /* ... of the incoming gradient (mg_adjust_logits_grad) */
+    const void *history_dev;     /* [n][t], NULL: none */
+    const int32_t *lengths_dev;  /* [n], NULL: t everywhere; below 0 counts as 0, above t as t */
+    int64_t history_stride;      /* elements between rows of the history; 0: one history for all */
+    int32_t history_type;        /* MG_U8, MG_I32, MG_I64 */
+    int32_t t;                   /* 0 .. 2^24 */
+    const float *repetition_dev; /* [n], NULL: the number below; positive */
+    const float *presence_dev, *frequency_dev; /* likewise */
+    float repetition, presence, frequency;
+    int32_t mask_kind;           /* MG_MASK_* */
+    const float *bias_dev;       /* NULL: none */
+    int64_t bias_stride;         /* elements between rows of the bias; 0: one row for all */
+    const void *mask_dev;
+    int64_t mask_stride;         /* elements (bytes or words) between rows of the mask; 0: one row for all */
+} MgAdjust;
+
+/* out may be the logits themselves (same stride). */
+int mg_adjust_logits(const MgAdjust *a, const void *logits_dev, void *out_dev, void *stream);
+
+/* The gradient of the logits: out = grad * (c > 0 ? (logit > 0 ? 1 / repetition : repetition) : 1), 0 where barred.
+ * `logits_dev` are the logits that mg_adjust_logits was given; out may be grad itself (same stride). */
+int mg_adjust_logits_grad(const MgAdjust *a, const void *logits_dev, const void *grad_dev, void *out_dev, void *stream);
+
+/* Rows of logits as a distribution, p_j = exp((x_j - max) / temperature) / total. */
+typedef struct MgLogits {
+    int64_t n;                     /* rows, 0 .. 2^31 - 1 */
+    int32_t k;                     /* tokens, 1 .. 2^24 */
+    int32_t dtype;                 /* MG_F32, MG_BF16, MG_F16 */
+    int64_t stride;                /* elements between rows */
+    const float *temperature_dev;  /* [n], NULL: the number below; positive and finite */
+    float temperature;
+    int32_t tokens_type;           /* MG_U8 (k at most 255), MG_I32, MG_I64 */
+} MgLogits;
+
+/* Draws one token of every row: the lowest j whose p_0 + ... + p_j exceeds uniforms[i] (in [0, 1), `uniforms_type`
+ * MG_F32 or MG_F64), worked out in 64 bits; uniforms_dev NULL: the lowest j of the largest logit.  logprob[i] (float32,
+ * may be NULL) = log p of that token.  A row that is no distribution (all -inf, or a NaN or +inf in it) gives token -1
+ * (255 as MG_U8, which mg_step takes for no action at all) and log-probability -inf (all -inf) or NaN.
+ * `workspace_dev`: mg_draw_workspace(l) bytes, 16-byte aligned (NULL where that is 0). */
+int64_t mg_draw_workspace(const MgLogits *l);
+int mg_draw(const MgLogits *l, const void *logits_dev, const void *uniforms_dev, int32_t uniforms_type, void *tokens_dev,
+            float *logprob_dev, void *workspace_dev, int64_t workspace_bytes, void *stream);
+
+/* Log-probability of a given token of every row and the row's entropy (either output may be NULL), and what the
+ * gradient needs of the row: stats [n][4] floats, 16-byte aligned (may be NULL).  A token outside 0 .. k - 1 is ignored:
+ * log-probability 0, and none of its gradient.  Rows that are all -inf: log-probability -inf, entropy 0, no gradient. */
+int64_t mg_token_logprobs_workspace(const MgLogits *l);
+int mg_token_logprobs(const MgLogits *l, const void *logits_dev, const void *tokens_dev, float *logprob_dev,
+                      float *entropy_dev, float *stats_dev, void *workspace_dev, int64_t workspace_bytes, void *stream);
+
+/* The gradient of the logits [n][k], contiguous, in the logits' type:
+ *     (g_i * ((j == token) - p_j) - h_i * p_j * (log p_j + entropy_i)) / temperature,  0 where the logit is -inf,
+ * for the gradients g of the log-probabilities and h of the entropies (float32 [n] with the strides given, in elements,
+ * 0 = one number for all; either pointer may be NULL). */
+int mg_token_logprobs_grad(const MgLogits *l, const void *logits_dev, const void *tokens_dev, const float *stats_dev,
+                           const float *grad_logprob_dev, int64_t grad_logprob_stride, const float *grad_entropy_dev,
+                           int64_t grad_entropy_stride, void *out_dev, void *stream);
 
 #ifdef __cplusplus
 }

@@ -13,19 +13,27 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 LIB_PATH = os.environ.get("MGRID_LIB", os.path.join(PKG_DIR, "libmgrid_hip.so"))
 SRC_PATH = os.path.join(PKG_DIR, "csrc", "mgrid.hip")
+POLICY_PATH = os.path.join(PKG_DIR, "csrc", "policy.hip")
 INCLUDE_DIR = os.path.join(ROOT, "include")
 
 MG_OK = 0
 KIND_EMPTY, KIND_REDBLUEDOORS, KIND_BLOCKEDUNLOCKPICKUP, KIND_LOCKEDHALLWAY, KIND_COMPETITIVE = range(5)
 AUTORESET_NONE, AUTORESET_SAME_STEP, AUTORESET_NEXT_STEP = range(3)
 NUM_STATS = 8
-ABI_VERSION = 8
+ABI_VERSION = 9
 ONE_HOT_DIM = 24  # 11 types + 6 colours + 7 states, multigrid/wrappers.py:95
 
 EXPORTS = ("mg_abi_version", "mg_create", "mg_destroy", "mg_last_error", "mg_upload_layouts", "mg_generate_layouts",
            "mg_set_reward_schemes",
            "mg_reset", "mg_step", "mg_step_shards", "mg_step_n", "mg_gen_obs", "mg_gen_obs_of_state", "mg_get_state", "mg_set_state",
-           "mg_stats", "mg_episode_stats", "mg_agents_mask", "mg_launch_census")
+           "mg_stats", "mg_episode_stats", "mg_agents_mask", "mg_launch_census",
+           "mg_embed", "mg_embed_grad_workspace", "mg_embed_grad", "mg_adjust_logits", "mg_adjust_logits_grad",
+           "mg_draw_workspace", "mg_draw", "mg_token_logprobs_workspace", "mg_token_logprobs", "mg_token_logprobs_grad")
+# element types, types of ids and tokens, kinds of masks (include/mgrid.h)
+F32, BF16, F16, F64 = range(4)
+U8, I32, I64 = range(3)
+MASK_NONE, MASK_BYTES, MASK_BITS = range(3)
+MAX_FIELDS = 8
 
 
 class MgConfig(ctypes.Structure):
@@ -46,6 +54,28 @@ class MgLayoutSpec(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in (
         "size", "random_start", "start_x", "start_y", "start_dir", "max_hallway_keys",
         "max_keys_per_room")] + [("agent_color", ctypes.c_uint8 * 64)]
+
+
+class MgEmbed(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("fields", "dim", "ids_type", "dtype")] + [
+        (n, ctypes.c_int64) for n in ("ids_stride", "field_stride", "row_stride")] + [
+        ("sizes", ctypes.c_int32 * MAX_FIELDS), ("scale", ctypes.c_float), ("reserved0", ctypes.c_int32)]
+
+
+class MgAdjust(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int64), ("k", ctypes.c_int32), ("dtype", ctypes.c_int32)] + [
+        (n, ctypes.c_int64) for n in ("logits_stride", "out_stride", "grad_stride")] + [
+        ("history_dev", ctypes.c_void_p), ("lengths_dev", ctypes.c_void_p), ("history_stride", ctypes.c_int64),
+        ("history_type", ctypes.c_int32), ("t", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("repetition_dev", "presence_dev", "frequency_dev")] + [
+        (n, ctypes.c_float) for n in ("repetition", "presence", "frequency")] + [
+        ("mask_kind", ctypes.c_int32), ("bias_dev", ctypes.c_void_p), ("bias_stride", ctypes.c_int64),
+        ("mask_dev", ctypes.c_void_p), ("mask_stride", ctypes.c_int64)]
+
+
+class MgLogits(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int64), ("k", ctypes.c_int32), ("dtype", ctypes.c_int32), ("stride", ctypes.c_int64),
+                ("temperature_dev", ctypes.c_void_p), ("temperature", ctypes.c_float), ("tokens_type", ctypes.c_int32)]
 
 
 def kernel_resources(listing: str):
@@ -92,25 +122,36 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
     the library; printed with ``verbose``), a step kernel that spills vector registers to scratch memory fails the
     build, and so does a code pattern this compiler was seen to get wrong (see _isa_lint.py)."""
     target = out_path or LIB_PATH
-    sources = [SRC_PATH, os.path.join(PKG_DIR, "csrc", "mgrid_experiment.h"), os.path.join(INCLUDE_DIR, "mgrid.h")]
+    sources = [SRC_PATH, POLICY_PATH, os.path.join(PKG_DIR, "csrc", "mgrid_experiment.h"),
+               os.path.join(PKG_DIR, "csrc", "mgrid_error.h"), os.path.join(INCLUDE_DIR, "mgrid.h")]
     if not force and os.path.exists(target) and os.path.getmtime(target) >= max(os.path.getmtime(f) for f in sources):
         return target
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    # -Os, measured: the step kernel is 7 % faster than at -O3 (smaller code, and 126 instead of 129 vector
-    # registers, which lets a fourth wavefront onto every SIMD)
+    # mgrid.hip at -Os, measured: the step kernel is 7 % faster than at -O3 (smaller code, and 126 instead of 129
+    # vector registers, which lets a fourth wavefront onto every SIMD).  The streaming kernels of policy.hip are unrolled
+    # where it pays: -O2.  Packed float32 instructions stay off: some of their forms have given wrong results.
     import glob
     import json
     import shutil
     import tempfile
     from ._isa_lint import find_masked_copies
     tmp = tempfile.mkdtemp(prefix="mgrid_build_")
+    running = []
     try:
         out = os.path.join(tmp, "libmgrid_hip.so")
-        cmd = [hipcc, "-Os", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-shared", "-save-temps",
-               "-I", INCLUDE_DIR, *extra_flags, SRC_PATH, "-o", out]
-        if verbose:
-            print(" ".join(cmd))
-        subprocess.check_call(cmd, cwd=tmp)
+        objects = []
+        for path, level in ((SRC_PATH, "-Os"), (POLICY_PATH, "-O2")):  # side by side
+            objects.append(os.path.join(tmp, os.path.basename(path) + ".o"))
+            cmd = [hipcc, level, "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-c", "-save-temps",
+                   "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", INCLUDE_DIR, *extra_flags, path,
+                   "-o", objects[-1]]
+            if verbose:
+                print(" ".join(cmd))
+            running.append((cmd, subprocess.Popen(cmd, cwd=tmp)))
+        for cmd, process in running:
+            if process.wait() != 0:
+                raise subprocess.CalledProcessError(process.returncode, cmd)
+        subprocess.check_call([hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", *objects, "-o", out], cwd=tmp)
         listings = glob.glob(os.path.join(tmp, "*gfx950*.s"))
         if not listings:
             raise RuntimeError("the build left no device assembly to check")
@@ -146,6 +187,10 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
                 json.dump(report, f, indent=1, sort_keys=True)
                 f.write("\n")
     finally:
+        for _, process in running:
+            if process.poll() is None:
+                process.kill()
+            process.wait()
         shutil.rmtree(tmp, ignore_errors=True)
     return target
 
@@ -187,8 +232,21 @@ def lib() -> ctypes.CDLL:
             L.mg_episode_stats.argtypes = [i32, i32] + [vp] * 9
         if hasattr(L, "mg_launch_census"):
             L.mg_launch_census.argtypes = [ctypes.c_char_p, i32]
+        if hasattr(L, "mg_embed"):
+            i64, emb, adj, lgt = ctypes.c_int64, ctypes.POINTER(MgEmbed), ctypes.POINTER(MgAdjust), ctypes.POINTER(MgLogits)
+            L.mg_embed.argtypes = [emb] + [vp] * 4
+            L.mg_embed_grad.argtypes = [emb] + [vp] * 4 + [i64, vp]
+            L.mg_adjust_logits.argtypes = [adj] + [vp] * 3
+            L.mg_adjust_logits_grad.argtypes = [adj] + [vp] * 4
+            L.mg_draw.argtypes = [lgt, vp, vp, i32] + [vp] * 3 + [i64, vp]
+            L.mg_token_logprobs.argtypes = [lgt] + [vp] * 6 + [i64, vp]
+            L.mg_token_logprobs_grad.argtypes = [lgt] + [vp] * 4 + [i64, vp, i64, vp, vp]
+            for name, arg in (("mg_embed_grad_workspace", emb), ("mg_draw_workspace", lgt), ("mg_token_logprobs_workspace", lgt)):
+                getattr(L, name).argtypes = [arg]
         for name in EXPORTS:
-            if name not in ("mg_last_error",) and hasattr(L, name):
+            if name.endswith("_workspace") and hasattr(L, name):
+                getattr(L, name).restype = ctypes.c_int64
+            elif name not in ("mg_last_error",) and hasattr(L, name):
                 getattr(L, name).restype = ctypes.c_int
         _lib = L
     return _lib

@@ -47,6 +47,7 @@
 #include <mutex>
 
 #include "mgrid.h"
+#include "mgrid_error.h"
 // Rewards are doubles worked out in the reference's order of operations (multigrid/base.py:655-659 and the hooks'
 // `+=`), every operation rounded on its own as Python rounds it: no fused multiply-add anywhere in this file.
 #pragma clang fp contract(off)
@@ -2770,6 +2771,27 @@ int fail(MgEnv *h, int code, const char *fmt, ...) {
         g_create_error = buf;
     return code;
 }
+
+}  // namespace
+
+namespace mgrid {
+
+int refuse(int code, const char *fmt, ...) noexcept {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    try {
+        g_create_error = buf;
+    } catch (...) {
+    }
+    return code;
+}
+
+}  // namespace mgrid
+
+namespace {
 
 #define MG_HIP(h, call)                                                                         \
     do {                                                                                        \

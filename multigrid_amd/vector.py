@@ -36,7 +36,7 @@ from typing import Optional
 import numpy as np
 import torch
 
-from . import _lib, envs, layouts
+from . import _lib, envs, layouts, policy
 from .batched import BatchedMultiGrid
 
 
@@ -157,6 +157,24 @@ class MultiGridVectorEnv:
         # (the flags are bytes of 0 / 1: reinterpreted as booleans, not converted)
         return (self._obs(out), self._view(out.reward), self._view(out.terminated.view(torch.bool)),
                 self._view(out.truncated.view(torch.bool)), infos)
+
+    def step_logits(self, logits, uniforms=None, *, temperature=1.0, **adjust):
+        """``step`` with the actions drawn here from a policy's ``logits`` ``[N, A, 7]`` (``[N, 7]`` with ``single_agent``) on
+        the GPU: adjusted as ``policy.adjust_logits`` does it (``history``, ``repetition``, ``bias``, ``mask``, ...; not at all
+        without such arguments), then drawn with ``uniforms`` ``[N, A]`` (the likeliest action without them) as
+        ``policy.draw`` does it.  An agent whose mask bars every action takes none.  ``infos["actions"]`` (uint8, 255 for
+        none) and ``infos["action_logprobs"]`` say what was drawn."""
+        lead = (self.num_envs,) if self.single_agent else (self.num_envs, self.num_agents)
+        if tuple(logits.shape) != lead + (self.num_actions,):
+            raise ValueError(f"expected logits of shape {lead + (self.num_actions,)}, got {tuple(logits.shape)}")
+        with torch.no_grad():
+            if adjust:
+                logits = policy.adjust_logits(logits, **adjust)
+            actions, logprobs = policy.draw(logits, uniforms, temperature=temperature, dtype=torch.uint8)
+        obs, reward, terminated, truncated, infos = self.step(actions)
+        infos["actions"] = actions.cpu().numpy() if self.numpy else actions
+        infos["action_logprobs"] = logprobs.cpu().numpy() if self.numpy else logprobs
+        return obs, reward, terminated, truncated, infos
 
     def _view_mask(self, done):
         return done.cpu().numpy() if self.numpy else done

@@ -21,7 +21,15 @@ from typing import Dict, Optional
 
 import torch
 
+from . import policy
 from .batched import BatchedMultiGrid
+
+
+def cell_embedding(image: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """The first layer of a policy on the image, by lookup: ``image`` uint8 ``[..., V, V, 3]``, ``table`` ``[24, dim]`` ->
+    ``[..., V, V, dim]`` in the table's type.  It is the one-hot image of ``OneHotObsWrapper`` (multigrid/wrappers.py:95,114-146)
+    times the table, without the one-hot image (24 bytes a cell); differentiable with respect to the table."""
+    return policy.embed(image, table, fields=policy.CELL_FIELDS, scale=scale)
 
 
 def competitive_v2_observation(image: torch.Tensor, direction: torch.Tensor) -> torch.Tensor:
