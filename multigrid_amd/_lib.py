@@ -129,9 +129,14 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     # mgrid.hip at -Os, measured: the step kernel is 7 % faster than at -O3 (smaller code, and 126 instead of 129
     # vector registers, which lets a fourth wavefront onto every SIMD).  The streaming kernels of policy.hip are unrolled
-    # where it pays: -O2.  Packed float32 instructions stay off: some of their forms have given wrong results.
+    # where it pays: -O2.  Packed float32 instructions (v_pk_add_f32 and its like) are to stay out of the device code,
+    # some of their forms have given wrong results: policy.hip is compiled without them; in mgrid.hip the compiler finds
+    # no use for them, while the switch itself costs nine of its kernels two spilled registers each.  The listings of
+    # both are searched for them below.
+    no_packed = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
     import glob
     import json
+    import re
     import shutil
     import tempfile
     from ._isa_lint import find_masked_copies
@@ -140,11 +145,10 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
     try:
         out = os.path.join(tmp, "libmgrid_hip.so")
         objects = []
-        for path, level in ((SRC_PATH, "-Os"), (POLICY_PATH, "-O2")):  # side by side
+        for path, level in ((SRC_PATH, ("-Os",)), (POLICY_PATH, ("-O2", *no_packed))):  # side by side
             objects.append(os.path.join(tmp, os.path.basename(path) + ".o"))
-            cmd = [hipcc, level, "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-c", "-save-temps",
-                   "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", INCLUDE_DIR, *extra_flags, path,
-                   "-o", objects[-1]]
+            cmd = [hipcc, *level, "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-c", "-save-temps", "-I", INCLUDE_DIR,
+                   *extra_flags, path, "-o", objects[-1]]
             if verbose:
                 print(" ".join(cmd))
             running.append((cmd, subprocess.Popen(cmd, cwd=tmp)))
@@ -163,6 +167,9 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
                 raise RuntimeError(f"device code writes vector registers before a divergent region's lanes are "
                                    f"switched back on ({len(hits)} place(s): {what}); change the source around the "
                                    "named kernel until the compiler stops doing that")
+            packed = re.search(r"\bv_pk_(add|mul|fma)_f32\b", open(path).read())
+            if packed:
+                raise RuntimeError(f"{os.path.basename(path)} holds {packed.group(0)}")
             res = kernel_resources(path)
             for mangled, plain in zip(res, _demangle(list(res))):
                 report[plain.replace("(anonymous namespace)::", "")] = res[mangled]
