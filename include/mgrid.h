@@ -323,7 +323,7 @@ int mg_episode_stats(int32_t num_envs, int32_t num_agents, const float *reward_d
  * table; a word is a token of one field.  Sums are held in 32 bits and rounded once. */
 #define MG_MAX_FIELDS 8
 typedef struct MgEmbed {
-    int64_t n;                    /* tokens, 0 .. 2^31 - 1 */
+    int64_t n;                    /* tokens; n * fields 0 .. 2^31 - 1 */
     int32_t fields;               /* 1 .. MG_MAX_FIELDS */
     int32_t dim;                  /* 1 .. 2^24 */
     int32_t ids_type;             /* MG_U8, MG_I32, MG_I64 */

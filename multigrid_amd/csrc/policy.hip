@@ -20,6 +20,8 @@ namespace {
 
 using bf16 = __bf16;
 using f16 = _Float16;
+using float4_t = __attribute__((__vector_size__(16))) float;
+using ushort2_t = unsigned short __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 256;
 constexpr float NEG_INF = -__builtin_inff();
@@ -104,60 +106,561 @@ __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *id
     }
 }
 
-// A block owns ROW_TILE rows and SLAB columns of the gradient, looks through all ids for those rows, in order, and adds up the
-// tokens it finds in 32 bits; one thread per column and group of rows, so that no two threads share a sum.
-constexpr int ROW_TILE = 16, SLAB = 256, SCAN = 1024;
+// ---- gradient of the embedding -------------------------------------------------------------------------------------
 
-template <class T, class I>
-__global__ __launch_bounds__(THREADS) void embed_grad_scan_kernel(EmbedArgs a, const I *ids, const T *grad, T *out) {
-    __shared__ float acc[ROW_TILE][SLAB];
-    __shared__ uint32_t found[4][SCAN / 4];  // token of the segment in the low 16 bits, row of the tile above
-    __shared__ int count[4];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-    const int d0 = blockIdx.y * SLAB, width = min(SLAB, a.dim - d0);
-    const int groups = THREADS / width, group = threadIdx.x / width, col = threadIdx.x - group * width;
-    const int tiles = (a.rows + ROW_TILE - 1) / ROW_TILE;
-    const int64_t entries = a.n * a.fields;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int row0 = tile * ROW_TILE;
-        for (int i = threadIdx.x; i < ROW_TILE * SLAB; i += THREADS) (&acc[0][0])[i] = 0.f;
-        for (int64_t e0 = 0; e0 < entries; e0 += SCAN) {
-            __syncthreads();  // the last round's list is read, the sums are cleared
-            int n_found = 0;
-            for (int j = 0; j < SCAN / 4; j += 64) {
-                const int64_t e = e0 + wave * (SCAN / 4) + j + lane;
-                int row = -1;
-                if (e < entries) {
-                    const int64_t n = a.fields == 1 ? e : e / a.fields;
-                    const int f = static_cast<int>(e - n * a.fields);
-                    const int64_t id = static_cast<int64_t>(ids[n * a.ids_stride + f * a.field_stride]);
-                    int base = 0;
-                    for (int k = 0; k < f; ++k) base += a.sizes[k];
-                    if (id >= 0 && id < a.sizes[f]) row = base + static_cast<int>(id) - row0;
-                }
-                const bool hit = row >= 0 && row < ROW_TILE;
-                const uint64_t hits = __ballot(hit);
-                if (hit) found[wave][n_found + __popcll(hits & ((1ull << lane) - 1))] = static_cast<uint32_t>(wave * (SCAN / 4) + j + lane) | static_cast<uint32_t>(row) << 16;
-                n_found += __popcll(hits);
+// id f of token n as a row of the table, or -1 if it reads none
+__device__ __forceinline__ int row_of(const EmbedArgs &a, const void *ids, int ids_type, int64_t n, int f, int base) {
+    const int64_t at = n * a.ids_stride + f * a.field_stride;
+    const int64_t id = ids_type == MG_U8 ? static_cast<const uint8_t *>(ids)[at]
+                                         : (ids_type == MG_I32 ? static_cast<const int32_t *>(ids)[at] : static_cast<const int64_t *>(ids)[at]);
+    return id >= 0 && id < a.sizes[f] ? base + static_cast<int>(id) : -1;
+}
+
+// Few rows (up to FEW): the gradient is the product of the rows' indicator [rows][n] (1 where token n reads the row) and the
+// incoming gradient [n][dim], which is what matrix instructions are for: 1 is exact in every type, so every product is, and
+// the sums are held in float32.  16-bit gradients go in as they are, float32 ones as three bfloat16 parts of eight bits each.
+//
+// A wave takes 64 tokens at a time: lane n puts its token's rows into LDS, then two 16 x 16 x 32 products per 16 rows and 16
+// columns.  The indicator's fragment (row l % 16, tokens 8 (l / 16) ...) is made from eight row numbers by three packed 16-bit
+// instructions per pair; the gradient's fragment (column l % 16, the same tokens) comes straight from memory, W adjacent
+// columns of a token to a lane, so that product i of W covers columns W * (0 .. 15) + i and pairs of tokens meet by one byte
+// permutation each.  Waves and blocks stride over the tokens, a block adds its four waves, embed_join_kernel the blocks, all
+// in a fixed order.
+//
+// 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
+// again, one after the other, each added to its own rows only.
+constexpr int FEW = 64, FEW_BLOCKS = 1024;
+
+template <class T>
+struct Operand {
+    using type = __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16;
+    static constexpr uint32_t ONE = 0x3F80;
+    static __device__ __forceinline__ float4_t multiply(type a, type b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Operand<f16> {
+    using type = __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16;
+    static constexpr uint32_t ONE = 0x3C00;
+    static __device__ __forceinline__ float4_t multiply(type a, type b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+union Fragment {
+    uint32_t w[4];
+    Operand<float>::type b;
+    Operand<f16>::type h;
+    template <class T>
+    __device__ __forceinline__ typename Operand<T>::type get() const {
+        if constexpr (sizeof(typename Operand<T>::type) && __is_same(T, f16))
+            return h;
+        else
+            return b;
+    }
+};
+
+// Words of W adjacent elements; elements from `left` on are 0.
+template <class T, int W>
+__device__ __forceinline__ void load_words(const T *p, int left, uint32_t (&w)[(W * sizeof(T) + 3) / 4]) {
+    constexpr int WORDS = (W * sizeof(T) + 3) / 4;
+    if (left >= W) {
+        if constexpr (W * sizeof(T) >= 4) {
+            const Vec<T, W> r = *reinterpret_cast<const Vec<T, W> *>(p);
+            __builtin_memcpy(w, &r, sizeof r);
+        } else {
+            w[0] = __builtin_bit_cast(uint16_t, p[0]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (i < left) {
+                if constexpr (sizeof(T) == 4)
+                    w[i] = __builtin_bit_cast(uint32_t, p[i]);
+                else
+                    w[i / 2] |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, p[i])) << (16 * (i & 1));
             }
-            if (lane == 0) count[wave] = n_found;
-            __syncthreads();
-            if (group < groups)
-                for (int w = 0; w < 4; ++w)
-                    for (int i = 0; i < count[w]; ++i) {
-                        const uint32_t what = found[w][i];
-                        const int row = what >> 16;
-                        if (row % groups != group) continue;
-                        const int64_t e = e0 + (what & 0xFFFF);
-                        const int64_t n = a.fields == 1 ? e : e / a.fields;
-                        acc[row][col] += static_cast<float>(grad[n * a.row_stride + d0 + col]);
+    }
+}
+
+template <class T, int W, int TILES>
+__global__ __launch_bounds__(THREADS) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
+    constexpr int COLS = 16 * W, WORDS = (W * sizeof(T) + 3) / 4;
+    __shared__ __align__(16) uint16_t rows_s[THREADS / 64][MG_MAX_FIELDS][64];  // 0xFFFF: none
+    __shared__ float sum_s[TILES * 16][COLS];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, quad = lane / 16;
+    const int d0 = blockIdx.y * COLS, col = l16 * W, left = a.dim - d0 - col;
+    // the field that this lane's row of each tile belongs to, and the row twice in a word (a row that is none never matches)
+    int field[TILES];
+    uint32_t twice[TILES];
+#pragma unroll
+    for (int m = 0; m < TILES; ++m) {
+        const int row = m * 16 + l16;
+        int f = 0, base = 0;
+        while (f + 1 < a.fields && row >= base + a.sizes[f]) base += a.sizes[f++];
+        field[m] = f;
+        twice[m] = row < a.rows ? static_cast<uint32_t>(row) * 0x10001u : 0xFFFEFFFEu;
+    }
+    float4_t acc[TILES][W];
+#pragma unroll
+    for (int m = 0; m < TILES; ++m)
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[m][i] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+    const int64_t step = static_cast<int64_t>(gridDim.x) * THREADS;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64; t0 < a.n; t0 += step) {
+        uint32_t x[2][8][WORDS];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t t = t0 + s * 32 + quad * 8 + j;
+                load_words<T, W>(grad + t * a.row_stride + d0 + col, t < a.n ? left : 0, x[s][j]);
+            }
+        int base = 0;
+        for (int f = 0; f < a.fields; ++f) {
+            const int64_t t = t0 + lane;
+            rows_s[wave][f][lane] = static_cast<uint16_t>(t < a.n ? row_of(a, ids, ids_type, t, f, base) : -1);
+            base += a.sizes[f];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            Fragment hot[TILES];
+#pragma unroll
+            for (int m = 0; m < TILES; ++m) {
+                const uint4 r = *reinterpret_cast<const uint4 *>(&rows_s[wave][field[m]][s * 32 + quad * 8]);
+                const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {  // ONE where the halves are equal: ONE - min(xor, 1) * ONE
+                    ushort2_t d = __builtin_bit_cast(ushort2_t, rr[p] ^ twice[m]);
+                    d = __builtin_elementwise_min(d, ushort2_t{1, 1});
+                    constexpr uint16_t ONE = Operand<T>::ONE;
+                    hot[m].w[p] = __builtin_bit_cast(uint32_t, static_cast<ushort2_t>(ushort2_t{ONE, ONE} - d * ushort2_t{ONE, ONE}));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                Fragment g;
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int p = 0; p < 4; ++p)
+                        g.w[p] = __builtin_amdgcn_perm(x[s][2 * p + 1][i / 2], x[s][2 * p][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int m = 0; m < TILES; ++m) acc[m][i] = Operand<T>::multiply(hot[m].template get<T>(), g.template get<T>(), acc[m][i]);
+                } else {
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) {
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            g.w[p] = __builtin_amdgcn_perm(x[s][2 * p + 1][i], x[s][2 * p][i], 0x07060302u);
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {  // what the upper half leaves
+                                uint32_t &v = x[s][2 * p + o][i];
+                                v = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, v) - __builtin_bit_cast(float, v & 0xFFFF0000u));
+                            }
+                        }
+#pragma unroll
+                        for (int m = 0; m < TILES; ++m) acc[m][i] = Operand<T>::multiply(hot[m].template get<T>(), g.template get<T>(), acc[m][i]);
                     }
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();  // the next tokens' rows come after these reads
+    }
+
+    bool fine = true;
+#pragma unroll
+    for (int m = 0; m < TILES; ++m)
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) fine &= fabsf(acc[m][i][q]) < -NEG_INF;
+    if (__syncthreads_and(fine)) {
+        for (int w = 0; w < THREADS / 64; ++w) {
+            if (wave == w) {
+#pragma unroll
+                for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            float &s = sum_s[m * 16 + quad * 4 + q][col + i];
+                            s = w ? s + acc[m][i][q] : acc[m][i][q];
+                        }
+            }
+            __syncthreads();
+        }
+    } else {  // one thread for a column and every (THREADS / COLS)th row
+        const int c = threadIdx.x % COLS, share = threadIdx.x / COLS;
+        for (int r = share; r < TILES * 16; r += THREADS / COLS) sum_s[r][c] = 0.f;
+        for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * THREADS; t0 < a.n; t0 += step)
+            for (int64_t t = t0; t < t0 + THREADS && t < a.n; ++t) {
+                int base = 0;
+                for (int f = 0; f < a.fields; ++f) {
+                    const int r = row_of(a, ids, ids_type, t, f, base);
+                    if (r >= 0 && r % (THREADS / COLS) == share && d0 + c < a.dim) sum_s[r][c] += static_cast<float>(grad[t * a.row_stride + d0 + c]);
+                    base += a.sizes[f];
+                }
+            }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < a.rows * COLS; i += THREADS) {
+        const int r = i / COLS, c = i % COLS;
+        if (d0 + c >= a.dim) continue;
+        if (parts)
+            parts[(static_cast<int64_t>(blockIdx.x) * a.rows + r) * a.dim + d0 + c] = sum_s[r][c];
+        else
+            out[static_cast<int64_t>(r) * a.dim + d0 + c] = static_cast<T>(sum_s[r][c] * a.scale);
+    }
+}
+
+// The blocks' sums of one table gradient added up: 16 adjacent elements and 64 shares of the blocks to a workgroup.
+constexpr int JOIN_COLS = 16, JOIN_SHARES = 64;
+
+template <class T>
+__global__ __launch_bounds__(JOIN_COLS *JOIN_SHARES) void embed_join_kernel(const float *parts, int blocks, int64_t elements, float scale, T *out) {
+    __shared__ float sum_s[JOIN_SHARES][JOIN_COLS];
+    const int c = threadIdx.x % JOIN_COLS, share = threadIdx.x / JOIN_COLS;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * JOIN_COLS + c;
+    float s = 0.f;
+    if (at < elements)
+#pragma unroll 8
+        for (int b = share; b < blocks; b += JOIN_SHARES) s += parts[b * elements + at];
+    sum_s[share][c] = s;
+    __syncthreads();
+    for (int half = JOIN_SHARES / 2; half > 0; half /= 2) {
+        if (share < half) sum_s[share][c] += sum_s[share + half][c];
+        __syncthreads();
+    }
+    if (share == 0 && at < elements) out[at] = static_cast<T>(sum_s[0][c] * scale);
+}
+
+// More rows: the entries (token n, field f) are sorted by row, order kept (a radix sort of up to 9 bits a pass), and the sorted
+// list is cut into chunks of equal length whatever the rows' frequencies are.  A chunk adds up its runs of equal rows; a run
+// that lies inside one chunk is finished there, one that passes a border leaves float32 parts for embed_span_kernel.
+constexpr int MOST_BINS = 512, DIGIT = 9;
+
+// Lanes with the same digit as this one.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool live) {
+    uint64_t same = __ballot(live);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t ones = __ballot((digit >> b) & 1);
+        same &= (digit >> b) & 1 ? ones : ~ones;
+    }
+    return same;
+}
+
+// Place among the wave's earlier entries of the same digit, counted in `count`.
+__device__ __forceinline__ uint32_t place(uint32_t *count, uint32_t digit, int bits, bool live, int lane) {
+    const uint64_t same = same_digit(digit, bits, live);
+    const int leader = same ? __builtin_ctzll(same) : 0;
+    uint32_t before = 0;
+    if (live && lane == leader) before = atomicAdd(&count[digit], static_cast<uint32_t>(__popcll(same)));
+    before = __shfl(before, leader, 64);
+    return before + __popcll(same & ((1ull << lane) - 1));
+}
+
+// exclusive sums of v over the threads of a block
+template <int N>
+__device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t *wave_sums, uint32_t *total) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    uint32_t s = v;
+#pragma unroll
+    for (int by = 1; by < 64; by *= 2) {
+        const uint32_t o = __shfl_up(s, by, 64);
+        if (lane >= by) s += o;
+    }
+    if (lane == 63) wave_sums[wave] = s;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int w = 0; w < N / 64; ++w) {
+        if (w < wave) before += wave_sums[w];
+        all += wave_sums[w];
+    }
+    if (total) *total = all;
+    __syncthreads();
+    return before + s - v;
+}
+
+// Up to SORT_ONE entries and 2^18 - 1 rows: one workgroup sorts words of row << 14 | entry in LDS.
+constexpr int SORT_THREADS = 1024, SORT_ONE = 1 << 14, SORT_ROWS = (1 << 18) - 1;
+
+__global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, const void *ids, int ids_type, int entries, int passes, int bits,
+                                                                  uint32_t *rows_out, uint32_t *tokens_out, uint8_t *touched) {
+    constexpr int WAVES = SORT_THREADS / 64, ROUNDS = SORT_ONE / SORT_THREADS;
+    __shared__ uint32_t word_s[SORT_ONE];
+    __shared__ uint32_t count_s[WAVES][MOST_BINS];
+    __shared__ uint32_t wave_sums[WAVES];
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
+    for (int r = tid; r < a.rows; r += SORT_THREADS) touched[r] = 0;
+    const int rounds = (entries + SORT_THREADS - 1) / SORT_THREADS, first = wave * rounds * 64 + lane;
+    for (int e = tid; e < entries; e += SORT_THREADS) {
+        const int n = a.fields == 1 ? e : e / a.fields, f = e - n * a.fields;
+        int base = 0;
+        for (int k = 0; k < f; ++k) base += a.sizes[k];
+        const int row = row_of(a, ids, ids_type, n, f, base);
+        word_s[e] = static_cast<uint32_t>(row < 0 ? a.rows : row) << 14 | e;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = 14 + pass * bits, bins = 1 << bits;
+        for (int i = tid; i < WAVES * MOST_BINS; i += SORT_THREADS) (&count_s[0][0])[i] = 0;
+        __syncthreads();
+        uint32_t word[ROUNDS], at[ROUNDS];
+#pragma unroll
+        for (int j = 0; j < ROUNDS; ++j) {
+            if (j >= rounds) break;
+            const int e = first + j * 64;
+            const bool live = e < entries;
+            word[j] = live ? word_s[e] : 0;
+            at[j] = place(count_s[wave], (word[j] >> shift) & (bins - 1), bits, live, lane);
         }
         __syncthreads();
-        if (group < groups)
-            for (int r = group; r < ROW_TILE && row0 + r < a.rows; r += groups)
-                out[static_cast<int64_t>(row0 + r) * a.dim + d0 + col] = static_cast<T>(acc[r][col] * a.scale);
+        uint32_t mine = 0;
+        if (tid < bins)
+            for (int w = 0; w < WAVES; ++w) {
+                const uint32_t c = count_s[w][tid];
+                count_s[w][tid] = mine;
+                mine += c;
+            }
+        const uint32_t before = sum_before<SORT_THREADS>(mine, wave_sums, nullptr);
+        if (tid < bins)
+            for (int w = 0; w < WAVES; ++w) count_s[w][tid] += before;
         __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ROUNDS; ++j)
+            if (j < rounds && first + j * 64 < entries) word_s[count_s[wave][(word[j] >> shift) & (bins - 1)] + at[j]] = word[j];
+        __syncthreads();
+    }
+    for (int i = tid; i < entries; i += SORT_THREADS) {
+        const uint32_t w = word_s[i], row = w >> 14;
+        rows_out[i] = row;
+        tokens_out[i] = a.fields == 1 ? (w & (SORT_ONE - 1)) : (w & (SORT_ONE - 1)) / a.fields;
+        if (row < static_cast<uint32_t>(a.rows)) touched[row] = 1;
+    }
+}
+
+// More entries: a pass is a count of every block's digits, one block's sums over all counts, and the placing.  A block owns
+// `span` adjacent entries (a multiple of SORT_TILE, so that there are at most SORT_BLOCKS blocks).
+constexpr int SORT_TILE = 4096, SORT_BLOCKS = 1024;
+
+__device__ __forceinline__ uint2 entry_at(const EmbedArgs &a, const void *ids, int ids_type, const uint2 *from, int64_t e) {
+    if (from) return from[e];
+    const int64_t n = a.fields == 1 ? e : e / a.fields;
+    const int f = static_cast<int>(e - n * a.fields);
+    int base = 0;
+    for (int k = 0; k < f; ++k) base += a.sizes[k];
+    const int row = row_of(a, ids, ids_type, n, f, base);
+    return make_uint2(static_cast<uint32_t>(row < 0 ? a.rows : row), static_cast<uint32_t>(n));
+}
+
+__global__ __launch_bounds__(THREADS) void embed_count_kernel(EmbedArgs a, const void *ids, int ids_type, const uint2 *from, int64_t entries, int span,
+                                                              int shift, int bits, uint32_t *counts, uint8_t *touched) {
+    __shared__ uint32_t count_s[MOST_BINS];
+    const int bins = 1 << bits;
+    for (int i = threadIdx.x; i < bins; i += THREADS) count_s[i] = 0;
+    if (touched)
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; r < a.rows; r += static_cast<int64_t>(gridDim.x) * THREADS) touched[r] = 0;
+    __syncthreads();
+    const int64_t lo = static_cast<int64_t>(blockIdx.x) * span, hi = min(lo + span, entries);
+    for (int64_t e = lo + threadIdx.x; e < hi; e += THREADS) atomicAdd(&count_s[(entry_at(a, ids, ids_type, from, e).x >> shift) & (bins - 1)], 1u);
+    __syncthreads();
+    for (int i = threadIdx.x; i < bins; i += THREADS) counts[static_cast<int64_t>(i) * gridDim.x + blockIdx.x] = count_s[i];
+}
+
+__global__ __launch_bounds__(SORT_THREADS) void embed_scan_kernel(uint32_t *counts, int n) {
+    __shared__ uint32_t wave_sums[SORT_THREADS / 64];
+    uint32_t done = 0;
+    for (int i0 = 0; i0 < n; i0 += SORT_THREADS * 8) {  // eight adjacent numbers to a thread
+        uint32_t v[8], mine = 0;
+        const int at = i0 + threadIdx.x * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = at + j < n ? counts[at + j] : 0;
+            mine += v[j];
+        }
+        uint32_t total;
+        uint32_t before = done + sum_before<SORT_THREADS>(mine, wave_sums, &total);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (at + j < n) counts[at + j] = before;
+            before += v[j];
+        }
+        done += total;
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const void *ids, int ids_type, const uint2 *from, int64_t entries, int span,
+                                                              int shift, int bits, const uint32_t *counts, uint2 *to, uint32_t *rows_out,
+                                                              uint32_t *tokens_out, uint8_t *touched) {
+    constexpr int WAVES = THREADS / 64, ROUNDS = SORT_TILE / THREADS;
+    __shared__ uint32_t count_s[WAVES][MOST_BINS], base_s[MOST_BINS];
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, bins = 1 << bits;
+    for (int i = tid; i < bins; i += THREADS) base_s[i] = counts[static_cast<int64_t>(i) * gridDim.x + blockIdx.x];
+    const int64_t lo = static_cast<int64_t>(blockIdx.x) * span, hi = min(lo + span, entries);
+    for (int64_t e0 = lo; e0 < hi; e0 += SORT_TILE) {
+        for (int i = tid; i < WAVES * MOST_BINS; i += THREADS) (&count_s[0][0])[i] = 0;
+        __syncthreads();
+        const int64_t first = e0 + wave * (SORT_TILE / WAVES) + lane;
+        uint2 entry[ROUNDS];
+        uint32_t at[ROUNDS];
+#pragma unroll
+        for (int j = 0; j < ROUNDS; ++j) entry[j] = first + j * 64 < hi ? entry_at(a, ids, ids_type, from, first + j * 64) : make_uint2(0, 0);
+#pragma unroll
+        for (int j = 0; j < ROUNDS; ++j) at[j] = place(count_s[wave], (entry[j].x >> shift) & (bins - 1), bits, first + j * 64 < hi, lane);
+        __syncthreads();
+        for (int i = tid; i < bins; i += THREADS) {
+            uint32_t s = base_s[i];
+            for (int w = 0; w < WAVES; ++w) {
+                const uint32_t c = count_s[w][i];
+                count_s[w][i] = s;
+                s += c;
+            }
+            base_s[i] = s;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ROUNDS; ++j)
+            if (first + j * 64 < hi) {
+                const uint32_t p = count_s[wave][(entry[j].x >> shift) & (bins - 1)] + at[j];
+                if (to) {
+                    to[p] = entry[j];
+                } else {
+                    rows_out[p] = entry[j].x;
+                    tokens_out[p] = entry[j].y;
+                    if (entry[j].x < static_cast<uint32_t>(a.rows)) touched[entry[j].x] = 1;
+                }
+            }
+        __syncthreads();
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void load_part(const T *p, int left, float (&x)[V]) {
+    if (left >= V) {
+        load<T, V>(p, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = i < left ? static_cast<float>(p[i]) : 0.f;
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void store_part(T *p, int left, const float (&x)[V]) {
+    if (left >= V) {
+        store<T, V>(p, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = static_cast<T>(x[i]);
+    }
+}
+
+struct Sorted {
+    const uint32_t *rows, *tokens;  // [entries], by row; a.rows behind the last row
+    const uint8_t *touched;         // [a.rows]
+    float *head, *tail;             // [chunks][dim]: what a chunk has of a run that an earlier chunk began / that goes on behind it
+    int64_t entries;
+    int32_t chunk, chunks;          // entries of a chunk, number of chunks
+    int32_t lanes;                  // threads per chunk: a power of two, up to 64
+    int32_t sum_blocks;             // blocks that add up; those behind clear the rows that no token reads
+};
+
+template <class T>
+__global__ __launch_bounds__(THREADS) void embed_runs_kernel(EmbedArgs a, Sorted s, const T *grad, T *out) {
+    constexpr int V = WIDE<T>, AHEAD = 8;
+    const int lane = threadIdx.x % s.lanes, group = threadIdx.x / s.lanes, groups = THREADS / s.lanes;
+    const int d0 = (blockIdx.y * s.lanes + lane) * V, left = a.dim - d0;
+    if (left <= 0) return;
+    if (static_cast<int>(blockIdx.x) >= s.sum_blocks) {
+        const float zero[V] = {};
+        const int64_t step = static_cast<int64_t>(gridDim.x - s.sum_blocks) * groups;
+        for (int64_t r = static_cast<int64_t>(blockIdx.x - s.sum_blocks) * groups + group; r < a.rows; r += step)
+            if (!s.touched[r]) store_part<T, V>(out + r * a.dim + d0, left, zero);
+        return;
+    }
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * groups + group;
+    if (c >= s.chunks) return;
+    const int64_t e0 = c * s.chunk, e1 = min(e0 + s.chunk, s.entries);
+    const uint32_t none = a.rows;
+    uint32_t row = s.rows[e0];
+    bool begun = c > 0 && s.rows[e0 - 1] == row;
+    float acc[V] = {};
+    auto finish = [&](bool goes_on) {
+        if (row == none) return;
+        if (begun || goes_on) {
+            store_part<float, V>((begun ? s.head : s.tail) + c * a.dim + d0, left, acc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] *= a.scale;
+            store_part<T, V>(out + static_cast<int64_t>(row) * a.dim + d0, left, acc);
+        }
+    };
+    for (int64_t e = e0; e < e1; e += AHEAD) {
+        uint32_t r[AHEAD], t[AHEAD];
+        float x[AHEAD][V];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            r[j] = e + j < e1 ? s.rows[e + j] : none;
+            t[j] = e + j < e1 ? s.tokens[e + j] : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) load_part<T, V>(grad + static_cast<int64_t>(t[j]) * a.row_stride + d0, r[j] == none ? 0 : left, x[j]);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (e + j >= e1) break;
+            if (r[j] != row) {
+                finish(false);
+                row = r[j];
+                begun = false;
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] += x[j][i];
+        }
+    }
+    finish(e1 < s.entries && s.rows[e1] == row);
+}
+
+// Runs that pass chunk borders: the block of the chunk where one begins adds up its parts, the waves' shares of them in order.
+template <class T>
+__global__ __launch_bounds__(THREADS) void embed_span_kernel(EmbedArgs a, Sorted s, T *out) {
+    constexpr int SPAN = 64;  // columns of a block
+    __shared__ float sum_s[THREADS / SPAN][SPAN];
+    const int64_t c = blockIdx.x, e0 = c * s.chunk, e1 = min(e0 + s.chunk, s.entries);
+    if (e1 >= s.entries) return;
+    const uint32_t row = s.rows[e1 - 1];
+    if (row == static_cast<uint32_t>(a.rows) || s.rows[e1] != row) return;  // nothing goes on here
+    if (c > 0 && s.rows[e0] == row && s.rows[e0 - 1] == row) return;        // an earlier chunk began it
+    int64_t lo = c + 1, hi = s.chunks;  // chunks lo .. hi - 1 start with this row: rows are sorted, so the end is found by halving
+    {
+        int64_t a0 = lo, b0 = hi;
+        while (a0 < b0) {
+            const int64_t mid = (a0 + b0) / 2;
+            if (s.rows[mid * s.chunk] == row)
+                a0 = mid + 1;
+            else
+                b0 = mid;
+        }
+        hi = a0;
+    }
+    const int col = threadIdx.x % SPAN, share = threadIdx.x / SPAN;
+    const int d = blockIdx.y * SPAN + col;
+    const int64_t per = (hi - lo + THREADS / SPAN - 1) / (THREADS / SPAN);
+    float sum = 0.f;
+    if (d < a.dim) {
+        if (share == 0) sum = s.tail[c * a.dim + d];
+        const int64_t from = lo + share * per, to = min(from + per, hi);
+#pragma unroll 8
+        for (int64_t i = from; i < to; ++i) sum += s.head[i * a.dim + d];
+    }
+    sum_s[share][col] = sum;
+    __syncthreads();
+    if (share == 0 && d < a.dim) {
+        for (int w = 1; w < THREADS / SPAN; ++w) sum += sum_s[w][col];
+        out[static_cast<int64_t>(row) * a.dim + d] = static_cast<T>(sum * a.scale);
     }
 }
 
@@ -451,6 +954,12 @@ unsigned blocks_for(int64_t items, int64_t most = 1 << 20) { return static_cast<
 constexpr int64_t MOST_ROWS = (1ll << 31) - 1;
 constexpr int32_t MOST_TOKENS = 1 << 24;
 
+bool workspace_ok(const char *who, const void *workspace, int64_t bytes, int64_t need) {
+    if (need == 0 || (workspace && bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0)) return true;
+    refuse(MG_EINVAL, "%s: needs a workspace of %lld bytes, 16-byte aligned", who, static_cast<long long>(need));
+    return false;
+}
+
 bool dtype_ok(int32_t t) { return t == MG_F32 || t == MG_BF16 || t == MG_F16; }
 bool int_ok(int32_t t) { return t == MG_U8 || t == MG_I32 || t == MG_I64; }
 
@@ -470,6 +979,7 @@ int embed_args(const char *who, const MgEmbed *e, EmbedArgs *a) {
         a->sizes[f] = e->sizes[f];
         rows += e->sizes[f];
     }
+    if (e->n * e->fields > MOST_ROWS) return refuse(MG_EINVAL, "%s: n %lld times %d fields not supported (at most 2^31 - 1)", who, static_cast<long long>(e->n), e->fields);
     if (rows > 1ll << 30) return refuse(MG_EINVAL, "%s: %lld rows not supported (at most 2^30)", who, static_cast<long long>(rows));
     a->rows = static_cast<int32_t>(rows);
     return MG_OK;
@@ -492,6 +1002,130 @@ void with_types(int32_t dtype, int32_t ints, F f) {
         inner(bf16{});
     else
         inner(f16{});
+}
+
+// How a table gradient is taken: what it needs of the workspace, in order, each part 16-byte aligned.
+struct GradPlan {
+    bool few;
+    // few rows
+    int width, tiles, blocks;  // columns of a lane, tiles of 16 rows, blocks over the tokens
+    // sorted
+    bool one;                   // sorted by one workgroup
+    int64_t entries;
+    int bits, passes, sort_blocks, span;
+    Sorted s;
+    int64_t at_rows, at_tokens, at_touched, at_head, at_tail, at_pairs, at_counts;
+    int64_t bytes;
+};
+
+GradPlan plan_grad(const EmbedArgs &a, int wide) {
+    GradPlan p{};
+    auto take = [&](int64_t bytes) {
+        const int64_t at = p.bytes;
+        p.bytes += (bytes + 15) / 16 * 16;
+        return at;
+    };
+    p.few = a.rows <= FEW;
+    if (p.few) {
+        p.width = wide;  // the narrowest that holds a token's columns at once, or 16 bytes
+        while (p.width > 1 && 16 * (p.width / 2) >= a.dim) p.width /= 2;
+        p.tiles = a.rows <= 16 ? 1 : (a.rows <= 32 ? 2 : 4);
+        const int64_t blocks = (a.n + THREADS - 1) / THREADS;
+        p.blocks = static_cast<int>(blocks < 1 ? 1 : (blocks < FEW_BLOCKS ? blocks : FEW_BLOCKS));
+        if (p.blocks > 1) take(static_cast<int64_t>(p.blocks) * a.rows * a.dim * 4);
+        return p;
+    }
+    p.entries = a.n * a.fields;
+    int bits = 1;
+    while ((a.rows >> bits) > 0) ++bits;  // the row numbers 0 .. rows
+    p.passes = (bits + DIGIT - 1) / DIGIT;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    p.one = p.entries <= SORT_ONE && a.rows <= SORT_ROWS;
+    p.at_rows = take(p.entries * 4);
+    p.at_tokens = take(p.entries * 4);
+    p.at_touched = take(a.rows);
+    // chunks of 16 entries until there are 4096 of them, longer ones then
+    int64_t chunk = (p.entries + 4095) / 4096;
+    chunk = chunk < 16 ? 16 : (chunk + 7) / 8 * 8;
+    p.s.entries = p.entries;
+    p.s.chunk = static_cast<int32_t>(chunk);
+    p.s.chunks = static_cast<int32_t>((p.entries + chunk - 1) / chunk);
+    p.at_head = take(static_cast<int64_t>(p.s.chunks) * a.dim * 4);
+    p.at_tail = take(static_cast<int64_t>(p.s.chunks) * a.dim * 4);
+    p.s.lanes = 1;
+    while (p.s.lanes < 64 && p.s.lanes * wide < a.dim) p.s.lanes *= 2;
+    const int groups = THREADS / p.s.lanes;
+    p.s.sum_blocks = (p.s.chunks + groups - 1) / groups;
+    if (!p.one) {
+        int64_t span = (p.entries + SORT_BLOCKS - 1) / SORT_BLOCKS;
+        span = (span + SORT_TILE - 1) / SORT_TILE * SORT_TILE;
+        p.span = static_cast<int>(span);
+        p.sort_blocks = static_cast<int>((p.entries + span - 1) / span);
+        p.at_pairs = take(p.entries * 8 * (p.passes > 2 ? 2 : 1));
+        p.at_counts = take(static_cast<int64_t>(p.sort_blocks) * (4 << p.bits));
+    }
+    return p;
+}
+
+template <class T, int W>
+void launch_few(const EmbedArgs &a, const GradPlan &p, const void *ids, int ids_type, const T *grad, T *out, float *parts, hipStream_t stream) {
+    const dim3 grid(p.blocks, (a.dim + 16 * W - 1) / (16 * W));
+    if (p.tiles == 1)
+        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, 1>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
+    else if (p.tiles == 2)
+        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, 2>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
+    else
+        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, 4>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
+}
+
+template <class T>
+void launch_grad(const EmbedArgs &a, GradPlan p, const void *ids, int ids_type, const T *grad, T *out, char *ws, hipStream_t stream) {
+    if (p.few) {
+        float *parts = p.blocks > 1 ? reinterpret_cast<float *>(ws) : nullptr;
+        if (p.width == 1)
+            launch_few<T, 1>(a, p, ids, ids_type, grad, out, parts, stream);
+        else if (p.width == 2)
+            launch_few<T, 2>(a, p, ids, ids_type, grad, out, parts, stream);
+        else if (p.width == 4)
+            launch_few<T, 4>(a, p, ids, ids_type, grad, out, parts, stream);
+        else if constexpr (sizeof(T) == 2)
+            launch_few<T, 8>(a, p, ids, ids_type, grad, out, parts, stream);
+        if (parts) {
+            const int64_t elements = static_cast<int64_t>(a.rows) * a.dim;
+            hipLaunchKernelGGL((embed_join_kernel<T>), dim3((elements + JOIN_COLS - 1) / JOIN_COLS), dim3(JOIN_COLS * JOIN_SHARES), 0, stream, parts, p.blocks,
+                               elements, a.scale, out);
+        }
+        return;
+    }
+    uint32_t *rows = reinterpret_cast<uint32_t *>(ws + p.at_rows), *tokens = reinterpret_cast<uint32_t *>(ws + p.at_tokens);
+    uint8_t *touched = reinterpret_cast<uint8_t *>(ws + p.at_touched);
+    if (p.one) {
+        hipLaunchKernelGGL(embed_sort_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, a, ids, ids_type, static_cast<int>(p.entries), p.passes, p.bits, rows, tokens,
+                           touched);
+    } else {
+        uint2 *pairs = reinterpret_cast<uint2 *>(ws + p.at_pairs);
+        uint32_t *counts = reinterpret_cast<uint32_t *>(ws + p.at_counts);
+        const uint2 *from = nullptr;
+        for (int pass = 0; pass < p.passes; ++pass) {
+            uint2 *to = pass + 1 < p.passes ? pairs + (pass & 1) * p.entries : nullptr;
+            hipLaunchKernelGGL(embed_count_kernel, dim3(p.sort_blocks), dim3(THREADS), 0, stream, a, ids, ids_type, from, p.entries, p.span, pass * p.bits, p.bits,
+                               counts, pass == 0 ? touched : nullptr);
+            hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, counts, p.sort_blocks << p.bits);
+            hipLaunchKernelGGL(embed_place_kernel, dim3(p.sort_blocks), dim3(THREADS), 0, stream, a, ids, ids_type, from, p.entries, p.span, pass * p.bits, p.bits,
+                               counts, to, rows, tokens, touched);
+            from = to;
+        }
+    }
+    p.s.rows = rows;
+    p.s.tokens = tokens;
+    p.s.touched = touched;
+    p.s.head = reinterpret_cast<float *>(ws + p.at_head);
+    p.s.tail = reinterpret_cast<float *>(ws + p.at_tail);
+    const int groups = THREADS / p.s.lanes;
+    const int64_t clear = (a.rows + groups - 1) / groups;
+    const dim3 grid(p.s.sum_blocks + static_cast<unsigned>(clear < 2048 ? clear : 2048), (a.dim + p.s.lanes * WIDE<T> - 1) / (p.s.lanes * WIDE<T>));
+    hipLaunchKernelGGL((embed_runs_kernel<T>), grid, dim3(THREADS), 0, stream, a, p.s, grad, out);
+    if (p.s.chunks > 1) hipLaunchKernelGGL((embed_span_kernel<T>), dim3(p.s.chunks, (a.dim + 63) / 64), dim3(THREADS), 0, stream, a, p.s, out);
 }
 
 int adjust_args(const char *who, const MgAdjust *a) {
@@ -546,7 +1180,8 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
 
 int64_t mg_embed_grad_workspace(const MgEmbed *e) {
     EmbedArgs a;
-    return embed_args("mg_embed_grad_workspace", e, &a);
+    const int rc = embed_args("mg_embed_grad_workspace", e, &a);
+    return rc != MG_OK ? rc : plan_grad(a, e->dtype == MG_F32 ? WIDE<float> : WIDE<bf16>).bytes;
 }
 
 int mg_embed_grad(const MgEmbed *e, const void *ids_dev, const void *grad_dev, void *table_grad_dev, void *workspace_dev,
@@ -555,15 +1190,12 @@ int mg_embed_grad(const MgEmbed *e, const void *ids_dev, const void *grad_dev, v
     const int rc = embed_args("mg_embed_grad", e, &a);
     if (rc != MG_OK) return rc;
     if (((!ids_dev || !grad_dev) && a.n > 0) || !table_grad_dev) return refuse(MG_EINVAL, "mg_embed_grad: null argument");
-    (void)workspace_dev;
-    (void)workspace_bytes;
-    with_types(e->dtype, e->ids_type, [&](auto t, auto i) {
+    const GradPlan p = plan_grad(a, e->dtype == MG_F32 ? WIDE<float> : WIDE<bf16>);
+    if (!workspace_ok("mg_embed_grad", workspace_dev, workspace_bytes, p.bytes)) return MG_EINVAL;
+    with_types(e->dtype, MG_U8, [&](auto t, auto) {
         using T = decltype(t);
-        using I = decltype(i);
-        const int64_t tiles = (static_cast<int64_t>(a.rows) + ROW_TILE - 1) / ROW_TILE;
-        hipLaunchKernelGGL((embed_grad_scan_kernel<T, I>), dim3(blocks_for(tiles, 1 << 16), (a.dim + SLAB - 1) / SLAB), dim3(THREADS), 0,
-                           static_cast<hipStream_t>(stream), a, static_cast<const I *>(ids_dev), static_cast<const T *>(grad_dev),
-                           static_cast<T *>(table_grad_dev));
+        launch_grad<T>(a, p, ids_dev, e->ids_type, static_cast<const T *>(grad_dev), static_cast<T *>(table_grad_dev), static_cast<char *>(workspace_dev),
+                       static_cast<hipStream_t>(stream));
     });
     return launched("mg_embed_grad");
 }
