@@ -664,6 +664,48 @@ __global__ __launch_bounds__(THREADS) void embed_span_kernel(EmbedArgs a, Sorted
     }
 }
 
+// ---- rows of few tokens --------------------------------------------------------------------------------------------
+
+// Up to SHORT tokens (actions, not words) a thread has a row to itself, in registers: a wave's rows are adjacent in memory, so
+// its unaligned 16-byte loads use every line they touch, and no lane waits for another.  K is 8, 16 or SHORT; the tests
+// against the real number of tokens are the same for all lanes.
+constexpr int SHORT = 32;
+
+template <class T, int K>
+__device__ __forceinline__ void load_row(const T *p, int k, float (&x)[K], float fill) {
+    constexpr int V = WIDE<T>;
+#pragma unroll
+    for (int i = 0; i < K; i += V) {
+        if (i + V <= k) {
+            float v[V];
+            load<T, V>(p + i, v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[i + j] = v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[i + j] = i + j < k ? static_cast<float>(p[i + j]) : fill;
+        }
+    }
+}
+
+template <class T, int K>
+__device__ __forceinline__ void store_row(T *p, int k, const float (&x)[K]) {
+    constexpr int V = WIDE<T>;
+#pragma unroll
+    for (int i = 0; i < K; i += V) {
+        if (i + V <= k) {
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = x[i + j];
+            store<T, V>(p + i, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (i + j < k) p[i + j] = static_cast<T>(x[i + j]);
+        }
+    }
+}
+
 // ---- adjustment of logits ------------------------------------------------------------------------------------------
 
 // How often each token of a chunk stands in a row's history is counted in LDS (a chunk is what LDS holds counters for), then
@@ -722,6 +764,69 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, const T *lo
             }
         }
     }
+}
+
+// Rows of few tokens: every thread counts its own row's history in its own LDS counters (an odd number of words apart, so that
+// lanes fall on different banks), which needs no barrier.
+template <class T, class H, bool GRAD, int K>
+__global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(MgAdjust a, const T *logits, const T *grad, T *out) {
+#pragma clang fp contract(off)
+    constexpr int ROWS = K <= 16 ? THREADS : 64;
+    __shared__ uint32_t counts_s[ROWS][K + 1];
+    uint32_t *counts = counts_s[threadIdx.x];
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x;
+    if (row >= a.n) return;
+    const bool history = a.history_dev != nullptr && a.t > 0;
+    float x[K], g[K];
+    load_row<T, K>(logits + row * a.logits_stride, a.k, x, 0.f);
+    if (GRAD) load_row<T, K>(grad + row * a.grad_stride, a.k, g, 0.f);
+    uint32_t allow = ~0u;
+    if (a.mask_kind == MG_MASK_BYTES) {
+        const uint8_t *m = static_cast<const uint8_t *>(a.mask_dev) + row * a.mask_stride;
+        allow = 0;
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+            if (j < a.k && m[j]) allow |= 1u << j;
+    } else if (a.mask_kind == MG_MASK_BITS) {
+        allow = static_cast<const uint32_t *>(a.mask_dev)[row * a.mask_stride];
+    }
+    if (history) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) counts[j] = 0;
+        constexpr int V = 16 / static_cast<int>(sizeof(H));
+        const int len = a.lengths_dev ? min(max(a.lengths_dev[row], 0), a.t) : a.t;
+        const H *h = static_cast<const H *>(a.history_dev) + row * a.history_stride;
+        int i = 0;
+        for (; i + V <= a.t && i < len; i += V) {
+            const Vec<H, V> v = *reinterpret_cast<const Vec<H, V> *>(h + i);
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (i + j < len && v.v[j] >= 0 && v.v[j] < static_cast<H>(a.k)) atomicAdd(&counts[v.v[j]], 1u);
+        }
+        for (; i < len; ++i)
+            if (h[i] >= 0 && h[i] < static_cast<H>(a.k)) atomicAdd(&counts[h[i]], 1u);
+    }
+    const float rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
+    const float presence = a.presence_dev ? a.presence_dev[row] : a.presence;
+    const float frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        if (j >= a.k) continue;
+        const uint32_t c = history ? counts[j] : 0;
+        const bool ok = (allow >> j) & 1;
+        if (GRAD) {
+            float v = g[j];
+            if (c > 0) v = x[j] > 0.f ? v / rep : v * rep;
+            x[j] = ok ? v : 0.f;
+        } else {
+            float v = x[j];
+            if (c > 0) v = (v > 0.f ? v / rep : v * rep) - presence;
+            v = v - frequency * static_cast<float>(c);
+            if (a.bias_dev) v = v + a.bias_dev[row * a.bias_stride + j];
+            x[j] = ok ? v : NEG_INF;
+        }
+    }
+    store_row<T, K>(out + row * a.out_stride, a.k, x);
 }
 
 // ---- draw ----------------------------------------------------------------------------------------------------------
@@ -826,6 +931,66 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(MgLogits l, const T *logi
     }
 }
 
+// Rows of few tokens: one thread each.
+template <class T, int K>
+__global__ __launch_bounds__(THREADS) void draw_short_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type,
+                                                             void *tokens, float *logprob) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (row >= l.n) return;
+    float x[K];
+    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF);
+    const double inv_t = 1.0 / static_cast<double>(l.temperature_dev ? l.temperature_dev[row] : l.temperature);
+    float best = x[0];
+    int arg = 0;
+    bool nan = x[0] != x[0];
+#pragma unroll
+    for (int j = 1; j < K; ++j) {
+        nan |= x[j] != x[j];
+        if (x[j] > best) {
+            best = x[j];
+            arg = j;
+        }
+    }
+    int64_t token = -1;
+    double lp = nan || best != NEG_INF ? __builtin_nan("") : -__builtin_inf();
+    if (!nan && fabsf(best) < -NEG_INF) {
+        // p of a token; what is filled up behind the last one is -inf, so 0
+        auto p = [&](int j) { return exp((static_cast<double>(x[j]) - best) * inv_t); };
+        constexpr bool KEEP = K <= 16;
+        double e[KEEP ? K : 1], total = 0.0;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            if (j >= l.k) break;
+            const double v = p(j);
+            if (KEEP) e[j] = v;
+            total += v;
+        }
+        if (uniforms) {
+            const double u = uniforms_type == MG_F64 ? static_cast<const double *>(uniforms)[row] : static_cast<double>(static_cast<const float *>(uniforms)[row]);
+            const double border = u * total;
+            double upto = 0.0;
+            int last = arg;
+            bool done = false;
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                if (j >= l.k) break;
+                const double v = KEEP ? e[KEEP ? j : 0] : p(j);
+                upto += v;
+                if (!done && v > 0.0) last = j;
+                done |= upto > border;
+            }
+            arg = last;
+        }
+        token = arg;
+        float at = x[0];
+#pragma unroll
+        for (int j = 1; j < K; ++j) at = arg == j ? x[j] : at;
+        lp = (static_cast<double>(at) - best) * inv_t - log(total);
+    }
+    put_token(tokens, l.tokens_type, row, token);
+    if (logprob) logprob[row] = static_cast<float>(lp);
+}
+
 // ---- log-probabilities and entropies -------------------------------------------------------------------------------
 
 // A part of a row: its maximum m, the sum of e = exp((x - m) / T) over its tokens LESS the one of the maximum itself (r), and
@@ -880,20 +1045,26 @@ __device__ __forceinline__ Soft merge_wave(Soft s, float inv_t) {
     return s;
 }
 
+// What the slope of a finished row needs: its maximum, the logarithm of its total, its entropy.
+__device__ __forceinline__ float4 row_stats(const Soft &s) {
+    const bool empty = s.m == NEG_INF && s.r == -1.f;
+    const float log_total = s.m == -NEG_INF ? __builtin_nanf("") : log1pf(s.r);
+    return make_float4(empty ? NEG_INF : (s.r == s.r ? s.m : s.r), log_total, empty ? 0.f : log_total - s.t / (1.f + s.r), 0.f);
+}
+
 // What a finished row gives.
 template <class T>
 __device__ __forceinline__ void row_result(const MgLogits &l, const T *x, int64_t row, const Soft &s, float inv_t, const void *tokens,
                                            float *logprob, float *entropy, float *stats) {
-    const bool empty = s.m == NEG_INF && s.r == -1.f;
-    const float log_total = s.m == -NEG_INF ? __builtin_nanf("") : log1pf(s.r), h = empty ? 0.f : log_total - s.t / (1.f + s.r);
+    const float4 st = row_stats(s);
     if (logprob) {
         const int64_t token = get_token(tokens, l.tokens_type, row);
         float lp = 0.f;
-        if (token >= 0 && token < l.k) lp = empty ? NEG_INF : (static_cast<float>(x[token]) - s.m) * inv_t - log_total;
+        if (token >= 0 && token < l.k) lp = st.x == NEG_INF ? NEG_INF : (static_cast<float>(x[token]) - s.m) * inv_t - st.y;
         logprob[row] = lp;
     }
-    if (entropy) entropy[row] = h;
-    if (stats) reinterpret_cast<float4 *>(stats)[row] = make_float4(empty ? NEG_INF : s.m, log_total, h, 0.f);
+    if (entropy) entropy[row] = st.z;
+    if (stats) reinterpret_cast<float4 *>(stats)[row] = st;
 }
 
 template <class T>
@@ -938,6 +1109,58 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, const
         for (int j = threadIdx.x; j < l.k; j += THREADS)
             out[row * l.k + j] = static_cast<T>(logprob_slope(static_cast<float>(x[j]), j == token, st, inv_t, g, h));
     }
+}
+
+// Rows of few tokens: one thread each, the row in registers, its maximum known before the first exponential.  The backward pass
+// works the row out again rather than reading what the forward pass could have kept (16 bytes, more than half of seven logits).
+template <int K>
+__device__ __forceinline__ Soft soft_short(const float (&x)[K], int k, float inv_t) {
+    float m = x[0];
+#pragma unroll
+    for (int j = 1; j < K; ++j) m = __builtin_elementwise_maximum(m, x[j]);  // NaN if one is there
+    Soft s{m, m == NEG_INF ? -1.f : 0.f, 0.f};
+    bool passed = m == NEG_INF;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        if (j >= k) break;
+        const float z = (x[j] - m) * inv_t, e = expf(z);
+        if (!passed && x[j] == m) {
+            passed = true;
+        } else if (m != NEG_INF) {
+            s.r += e;
+            if (e > 0.f) s.t += e * z;
+        }
+    }
+    return s;
+}
+
+template <class T, int K>
+__global__ __launch_bounds__(THREADS) void logprob_short_kernel(MgLogits l, const T *logits, const void *tokens, float *logprob,
+                                                                float *entropy, float *stats) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (row >= l.n) return;
+    float x[K];
+    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF);
+    const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
+    row_result(l, logits + row * l.stride, row, soft_short<K>(x, l.k, inv_t), inv_t, tokens, logprob, entropy, stats);
+}
+
+template <class T, int K>
+__global__ __launch_bounds__(THREADS) void logprob_grad_short_kernel(MgLogits l, const T *logits, const void *tokens, const float *grad_lp,
+                                                                     int64_t lp_stride, const float *grad_h, int64_t h_stride, T *out) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+    if (row >= l.n) return;
+    float x[K];
+    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF);
+    const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
+    const float4 st = row_stats(soft_short<K>(x, l.k, inv_t));
+    const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
+    const float g = token >= 0 && token < l.k ? grad_lp[row * lp_stride] * inv_t : 0.f;
+    const float h = grad_h ? grad_h[row * h_stride] * inv_t : 0.f;
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+        if (j < l.k) x[j] = logprob_slope(x[j], j == token, st, inv_t, g, h);
+    store_row<T, K>(out + row * l.k, l.k, x);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
@@ -1128,6 +1351,21 @@ void launch_grad(const EmbedArgs &a, GradPlan p, const void *ids, int ids_type, 
     if (p.s.chunks > 1) hipLaunchKernelGGL((embed_span_kernel<T>), dim3(p.s.chunks, (a.dim + 63) / 64), dim3(THREADS), 0, stream, a, p.s, out);
 }
 
+// f(the smallest of 8, 16, SHORT that holds k tokens), as a type with a constant `value`
+template <int K>
+struct Size {
+    static constexpr int value = K;
+};
+template <class F>
+void with_size(int k, F f) {
+    if (k <= 8)
+        f(Size<8>{});
+    else if (k <= 16)
+        f(Size<16>{});
+    else
+        f(Size<SHORT>{});
+}
+
 int adjust_args(const char *who, const MgAdjust *a) {
     if (!a) return refuse(MG_EINVAL, "%s: null argument", who);
     if (a->n < 0 || a->n > MOST_ROWS) return refuse(MG_EINVAL, "%s: n %lld not supported (0..2^31 - 1)", who, static_cast<long long>(a->n));
@@ -1143,6 +1381,25 @@ int adjust_args(const char *who, const MgAdjust *a) {
     if (!a->repetition_dev && !(a->repetition > 0.f && a->repetition < __builtin_inff()))
         return refuse(MG_EINVAL, "%s: repetition must be positive and finite", who);
     return MG_OK;
+}
+
+template <bool GRAD>
+void launch_adjust(const MgAdjust &a, const void *logits, const void *grad, void *out, hipStream_t stream) {
+    with_types(a.dtype, a.history_dev ? a.history_type : MG_U8, [&](auto t, auto h) {
+        using T = decltype(t);
+        using H = decltype(h);
+        const T *x = static_cast<const T *>(logits), *g = static_cast<const T *>(grad);
+        T *y = static_cast<T *>(out);
+        if (a.k <= SHORT) {
+            with_size(a.k, [&](auto size) {
+                constexpr int K = decltype(size)::value, ROWS = K <= 16 ? THREADS : 64;
+                hipLaunchKernelGGL((adjust_short_kernel<T, H, GRAD, K>), dim3((a.n + ROWS - 1) / ROWS), dim3(ROWS), 0, stream, a, x, g, y);
+            });
+        } else {
+            const int64_t chunks = (a.k + CHUNK - 1) / CHUNK;
+            hipLaunchKernelGGL((adjust_kernel<T, H, GRAD>), dim3(blocks_for(a.n * chunks)), dim3(THREADS), 0, stream, a, x, g, y);
+        }
+    });
 }
 
 int logits_args(const char *who, const MgLogits *l) {
@@ -1204,12 +1461,7 @@ int mg_adjust_logits(const MgAdjust *a, const void *logits_dev, void *out_dev, v
     const int rc = adjust_args("mg_adjust_logits", a);
     if (rc != MG_OK || a->n == 0) return rc;
     if (!logits_dev || !out_dev) return refuse(MG_EINVAL, "mg_adjust_logits: null argument");
-    with_types(a->dtype, a->history_type, [&](auto t, auto h) {
-        using T = decltype(t);
-        const int64_t chunks = (a->k + CHUNK - 1) / CHUNK;
-        hipLaunchKernelGGL((adjust_kernel<T, decltype(h), false>), dim3(blocks_for(a->n * chunks)), dim3(THREADS), 0,
-                           static_cast<hipStream_t>(stream), *a, static_cast<const T *>(logits_dev), static_cast<const T *>(nullptr), static_cast<T *>(out_dev));
-    });
+    launch_adjust<false>(*a, logits_dev, nullptr, out_dev, static_cast<hipStream_t>(stream));
     return launched("mg_adjust_logits");
 }
 
@@ -1217,12 +1469,7 @@ int mg_adjust_logits_grad(const MgAdjust *a, const void *logits_dev, const void 
     const int rc = adjust_args("mg_adjust_logits_grad", a);
     if (rc != MG_OK || a->n == 0) return rc;
     if (!logits_dev || !grad_dev || !out_dev) return refuse(MG_EINVAL, "mg_adjust_logits_grad: null argument");
-    with_types(a->dtype, a->history_type, [&](auto t, auto h) {
-        using T = decltype(t);
-        const int64_t chunks = (a->k + CHUNK - 1) / CHUNK;
-        hipLaunchKernelGGL((adjust_kernel<T, decltype(h), true>), dim3(blocks_for(a->n * chunks)), dim3(THREADS), 0,
-                           static_cast<hipStream_t>(stream), *a, static_cast<const T *>(logits_dev), static_cast<const T *>(grad_dev), static_cast<T *>(out_dev));
-    });
+    launch_adjust<true>(*a, logits_dev, grad_dev, out_dev, static_cast<hipStream_t>(stream));
     return launched("mg_adjust_logits_grad");
 }
 
@@ -1238,6 +1485,11 @@ int mg_draw(const MgLogits *l, const void *logits_dev, const void *uniforms_dev,
     (void)workspace_bytes;
     with_types(l->dtype, MG_U8, [&](auto t, auto) {
         using T = decltype(t);
+        if (l->k <= SHORT)
+            return with_size(l->k, [&](auto size) {
+                hipLaunchKernelGGL((draw_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0,
+                                   static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), uniforms_dev, uniforms_type, tokens_dev, logprob_dev);
+            });
         hipLaunchKernelGGL((draw_kernel<T>), dim3(blocks_for(l->n)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *l,
                            static_cast<const T *>(logits_dev), uniforms_dev, uniforms_type, tokens_dev, logprob_dev);
     });
@@ -1256,6 +1508,11 @@ int mg_token_logprobs(const MgLogits *l, const void *logits_dev, const void *tok
     (void)workspace_bytes;
     with_types(l->dtype, MG_U8, [&](auto t, auto) {
         using T = decltype(t);
+        if (l->k <= SHORT)
+            return with_size(l->k, [&](auto size) {
+                hipLaunchKernelGGL((logprob_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0,
+                                   static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), tokens_dev, logprob_dev, entropy_dev, stats_dev);
+            });
         hipLaunchKernelGGL((logprob_kernel<T>), dim3(blocks_for(l->n)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *l,
                            static_cast<const T *>(logits_dev), tokens_dev, logprob_dev, entropy_dev, stats_dev);
     });
@@ -1267,11 +1524,17 @@ int mg_token_logprobs_grad(const MgLogits *l, const void *logits_dev, const void
                            int64_t grad_entropy_stride, void *out_dev, void *stream) {
     const int rc = logits_args("mg_token_logprobs_grad", l);
     if (rc != MG_OK || l->n == 0) return rc;
-    if (!logits_dev || !stats_dev || !out_dev || (grad_logprob_dev && !tokens_dev)) return refuse(MG_EINVAL, "mg_token_logprobs_grad: null argument");
+    if (!logits_dev || (!stats_dev && l->k > SHORT) || !out_dev || (grad_logprob_dev && !tokens_dev)) return refuse(MG_EINVAL, "mg_token_logprobs_grad: null argument");
     if (reinterpret_cast<uintptr_t>(stats_dev) % 16) return refuse(MG_EINVAL, "mg_token_logprobs_grad: stats_dev must be 16-byte aligned");
     if (grad_logprob_stride < 0 || grad_entropy_stride < 0) return refuse(MG_EINVAL, "mg_token_logprobs_grad: negative stride");
     with_types(l->dtype, MG_U8, [&](auto t, auto) {
         using T = decltype(t);
+        if (l->k <= SHORT)
+            return with_size(l->k, [&](auto size) {
+                hipLaunchKernelGGL((logprob_grad_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0,
+                                   static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), tokens_dev, grad_logprob_dev, grad_logprob_stride,
+                                   grad_entropy_dev, grad_entropy_stride, static_cast<T *>(out_dev));
+            });
         hipLaunchKernelGGL((logprob_grad_kernel<T>), dim3(blocks_for(l->n)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *l,
                            static_cast<const T *>(logits_dev), tokens_dev, stats_dev, grad_logprob_dev, grad_logprob_stride, grad_entropy_dev,
                            grad_entropy_stride, static_cast<T *>(out_dev));

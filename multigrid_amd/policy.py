@@ -381,7 +381,7 @@ def _logprobs_forward(logits, tokens, temperature, stats: bool):
     tokens = tokens.contiguous()
     logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
     entropies = torch.empty(lead, dtype=torch.float32, device=dev)
-    kept = torch.empty((l.n, 4), dtype=torch.float32, device=dev) if stats else None
+    kept = torch.empty((l.n, 4), dtype=torch.float32, device=dev) if stats and l.k > 32 else None
     with _on(dev) as stream:
         lib = _lib.lib()
         ws = _workspace(lib.mg_token_logprobs_workspace(ctypes.byref(l)), dev)

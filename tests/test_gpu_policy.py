@@ -225,7 +225,7 @@ def test_cell_embedding_is_the_one_hot_image_times_the_table(policy):
 
 
 ADJUST = [  # rows, tokens, history, mask
-    (1, 1, 1, None), (1, 7, 0, "bool"), (3, 7, 5, "bits"), (1000, 7, 16, "bool"), (129, 32, 3, "bits"), (77, 33, 300, "bits"), (64, 63, 9, "bool"),
+    (1, 1, 1, None), (1, 7, 0, "bool"), (3, 7, 5, "bits"), (1000, 7, 16, "bool"), (129, 32, 3, "bits"), (300, 8, 40, "bits"), (70, 9, 3, "bool"), (70, 16, 17, "bits"), (70, 17, 33, "bool"), (77, 33, 300, "bits"), (64, 63, 9, "bool"),
     (64, 64, 9, None), (65, 65, 70, "bits"), (9, 1000, 33, "bits"), (2, 4099, 1025, "bool"), (3, 8191, 40, "bits"), (2, 8192, 40, "bool"),
     (2, 8193, 3000, "bits"), (1, 40007, 512, "bits"), (300, 511, 2, None),
 ]
@@ -346,7 +346,7 @@ def test_adjust_gradient_against_differences(policy):
 # ---- draw ----------------------------------------------------------------------------------------------------------------
 
 
-ROWS = [(1, 1), (1, 2), (5, 7), (1000, 7), (4099, 7), (100, 8), (100, 9), (65, 33), (65, 63), (65, 64), (65, 65), (17, 255), (17, 256), (9, 257), (9, 1000),
+ROWS = [(1, 1), (1, 2), (5, 7), (1000, 7), (4099, 7), (100, 8), (100, 9), (65, 15), (65, 16), (65, 17), (65, 32), (65, 33), (65, 63), (65, 64), (65, 65), (17, 255), (17, 256), (9, 257), (9, 1000),
         (3, 4097), (2, 8193), (1, 40007), (300, 2000), (2, 131072)]
 
 

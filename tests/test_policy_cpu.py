@@ -119,9 +119,12 @@ def test_draw_and_logprobs_refuse_missing_pointers():
     assert L.mg_draw(r, P, P, _lib.BF16, P, P, P, 0, None) == -1 and b"uniform" in L.mg_last_error(None)
     assert L.mg_token_logprobs(r, None, P, P, P, P, P, 0, None) == -1 and L.mg_token_logprobs(r, P, None, P, P, P, P, 0, None) == -1
     assert L.mg_token_logprobs(r, P, P, P, P, ctypes.c_void_p(4104), P, 1 << 40, None) == -1 and b"aligned" in L.mg_last_error(None)
-    for args in ((None, P, P, P, 1, P, 1, P), (P, None, P, P, 1, P, 1, P), (P, P, None, P, 1, P, 1, P), (P, P, P, P, 1, P, 1, None),
+    long = ctypes.byref(logits_spec(k=33, stride=33))
+    for args in ((None, P, P, P, 1, P, 1, P), (P, None, P, P, 1, P, 1, P), (P, P, P, P, 1, P, 1, None),
                  (P, P, ctypes.c_void_p(4104), P, 1, P, 1, P), (P, P, P, P, -1, P, 1, P), (P, P, P, P, 1, P, -1, P)):
         assert L.mg_token_logprobs_grad(r, *args, None) == -1
+        assert L.mg_token_logprobs_grad(long, *args, None) == -1
+    assert L.mg_token_logprobs_grad(long, P, P, None, P, 1, P, 1, P, None) == -1
     none = ctypes.byref(logits_spec(n=0))
     assert L.mg_draw(none, None, None, 0, None, None, None, 0, None) == 0
     assert L.mg_token_logprobs(none, None, None, None, None, None, None, 0, None) == 0
