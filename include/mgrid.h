@@ -399,8 +399,8 @@ typedef struct MgLogits {
 } MgLogits;
 
 /* Draws one token of every row: the lowest j whose p_0 + ... + p_j exceeds uniforms[i] (in [0, 1), `uniforms_type`
- * MG_F32 or MG_F64), worked out in 64 bits; uniforms_dev NULL: the lowest j of the largest logit.  logprob[i] (float32,
- * may be NULL) = log p of that token.  A row that is no distribution (all -inf, or a NaN or +inf in it) gives token -1
+ * MG_F32 or MG_F64), decided in 64 bits; uniforms_dev NULL: the lowest j of the largest logit.  logprob[i] (may be NULL)
+ * = log p of that token, as mg_token_logprobs gives it but for roundings.  A row that is no distribution (all -inf, or a NaN or +inf in it) gives token -1
  * (255 as MG_U8, which mg_step takes for no action at all) and log-probability -inf (all -inf) or NaN.
  * `workspace_dev`: mg_draw_workspace(l) bytes, 16-byte aligned (NULL where that is 0). */
 int64_t mg_draw_workspace(const MgLogits *l);

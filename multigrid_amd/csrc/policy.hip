@@ -51,6 +51,65 @@ __device__ __forceinline__ void store(T *p, const float (&x)[V]) {
 template <class T>
 constexpr int WIDE = 16 / static_cast<int>(sizeof(T));
 
+// Words of W adjacent elements, which stay packed until they are used; elements from `left` on are `fill` (an element's bits).
+template <class T, int W>
+__device__ __forceinline__ void load_words(const T *p, int left, uint32_t fill, uint32_t (&w)[(W * sizeof(T) + 3) / 4]) {
+    constexpr int WORDS = (W * sizeof(T) + 3) / 4;
+    if (left >= W) {
+        if constexpr (W * sizeof(T) >= 4) {
+            const Vec<T, W> r = *reinterpret_cast<const Vec<T, W> *>(p);
+            __builtin_memcpy(w, &r, sizeof r);
+        } else {
+            w[0] = __builtin_bit_cast(uint16_t, p[0]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = sizeof(T) == 4 ? fill : (W == 1 ? fill : fill * 0x10001u);
+        if (left > 0)
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (i < left) {
+                    if constexpr (sizeof(T) == 4)
+                        w[i] = __builtin_bit_cast(uint32_t, p[i]);
+                    else
+                        w[i / 2] = (w[i / 2] & (i & 1 ? 0xFFFFu : 0xFFFF0000u)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, p[i])) << (16 * (i & 1));
+                }
+    }
+}
+
+// element i of words
+template <class T>
+__device__ __forceinline__ float element(const uint32_t *w, int i) {
+    if constexpr (sizeof(T) == 4)
+        return __builtin_bit_cast(float, w[i]);
+    else
+        return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)))));
+}
+
+template <class T>
+constexpr uint32_t NEG_INF_BITS = sizeof(T) == 4 ? 0xFF800000u : (__is_same(T, f16) ? 0xFC00u : 0xFF80u);
+
+template <class T, int V>
+__device__ __forceinline__ void load_part(const T *p, int left, float (&x)[V]) {
+    if (left >= V) {
+        load<T, V>(p, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = i < left ? static_cast<float>(p[i]) : 0.f;
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void store_part(T *p, int left, const float (&x)[V]) {
+    if (left >= V) {
+        store<T, V>(p, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < left) p[i] = static_cast<T>(x[i]);
+    }
+}
+
 // ---- embedding -----------------------------------------------------------------------------------------------------
 
 struct EmbedArgs {
@@ -157,31 +216,6 @@ union Fragment {
     }
 };
 
-// Words of W adjacent elements; elements from `left` on are 0.
-template <class T, int W>
-__device__ __forceinline__ void load_words(const T *p, int left, uint32_t (&w)[(W * sizeof(T) + 3) / 4]) {
-    constexpr int WORDS = (W * sizeof(T) + 3) / 4;
-    if (left >= W) {
-        if constexpr (W * sizeof(T) >= 4) {
-            const Vec<T, W> r = *reinterpret_cast<const Vec<T, W> *>(p);
-            __builtin_memcpy(w, &r, sizeof r);
-        } else {
-            w[0] = __builtin_bit_cast(uint16_t, p[0]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = 0;
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-            if (i < left) {
-                if constexpr (sizeof(T) == 4)
-                    w[i] = __builtin_bit_cast(uint32_t, p[i]);
-                else
-                    w[i / 2] |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, p[i])) << (16 * (i & 1));
-            }
-    }
-}
-
 template <class T, int W, int TILES>
 __global__ __launch_bounds__(THREADS) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
     constexpr int COLS = 16 * W, WORDS = (W * sizeof(T) + 3) / 4;
@@ -214,7 +248,7 @@ __global__ __launch_bounds__(THREADS) void embed_grad_few_kernel(EmbedArgs a, co
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int64_t t = t0 + s * 32 + quad * 8 + j;
-                load_words<T, W>(grad + t * a.row_stride + d0 + col, t < a.n ? left : 0, x[s][j]);
+                load_words<T, W>(grad + t * a.row_stride + d0 + col, t < a.n ? left : 0, 0, x[s][j]);
             }
         int base = 0;
         for (int f = 0; f < a.fields; ++f) {
@@ -536,27 +570,6 @@ __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const
     }
 }
 
-template <class T, int V>
-__device__ __forceinline__ void load_part(const T *p, int left, float (&x)[V]) {
-    if (left >= V) {
-        load<T, V>(p, x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = i < left ? static_cast<float>(p[i]) : 0.f;
-    }
-}
-
-template <class T, int V>
-__device__ __forceinline__ void store_part(T *p, int left, const float (&x)[V]) {
-    if (left >= V) {
-        store<T, V>(p, x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) p[i] = static_cast<T>(x[i]);
-    }
-}
-
 struct Sorted {
     const uint32_t *rows, *tokens;  // [entries], by row; a.rows behind the last row
     const uint8_t *touched;         // [a.rows]
@@ -706,63 +719,207 @@ __device__ __forceinline__ void store_row(T *p, int k, const float (&x)[K]) {
     }
 }
 
-// ---- adjustment of logits ------------------------------------------------------------------------------------------
+// ---- longer rows ---------------------------------------------------------------------------------------------------
 
-// How often each token of a chunk stands in a row's history is counted in LDS (a chunk is what LDS holds counters for), then
-// the chunk streams through once.
-constexpr int CHUNK = 8192;
+// LANES threads (8 to 64: several rows to a block of THREADS; 256 or 1024: a block to a row) hold a row of up to
+// LANES * HELD 16-byte vectors in registers, vector j * LANES + lane with each: one pass over memory, whose loads are all under
+// way at once; the maximum is known before the first exponential.  HELD = 0: rows that no block holds are read again from
+// the cache or memory for each use, 1024 threads to a row.
+template <int LANES>
+constexpr int BLOCK = LANES > THREADS ? LANES : THREADS;
 
-template <class H>
-__device__ __forceinline__ void count_history(const MgAdjust &a, int64_t row, int first, int width, uint32_t *counts, int tid, int threads) {
-    int len = a.lengths_dev ? min(max(a.lengths_dev[row], 0), a.t) : a.t;
-    const H *h = static_cast<const H *>(a.history_dev) + row * a.history_stride;
-    for (int i = tid; i < len; i += threads) {
-        const int64_t j = static_cast<int64_t>(h[i]) - first;
-        if (j >= 0 && j < width) atomicAdd(&counts[j], 1u);
+template <class T, int LANES, int HELD>
+struct Row {
+    static constexpr int V = WIDE<T>;
+    const T *x;
+    int k, lane, vecs;
+    uint32_t held[HELD ? HELD : 1][4];
+
+    __device__ __forceinline__ void fetch(int j, uint32_t (&w)[4]) const {
+        const int at = (j * LANES + lane) * V;
+        // all lanes of the row have whole vectors (the same answer for all of them), or this is the last one
+        load_words<T, V>(x + at, (j + 1) * LANES * V <= k ? V : k - at, NEG_INF_BITS<T>, w);
     }
-}
-
-__device__ __forceinline__ bool allowed(const MgAdjust &a, int64_t row, int j) {
-    if (a.mask_kind == MG_MASK_BYTES) return static_cast<const uint8_t *>(a.mask_dev)[row * a.mask_stride + j] != 0;
-    if (a.mask_kind == MG_MASK_BITS) return (static_cast<const uint32_t *>(a.mask_dev)[row * a.mask_stride + (j >> 5)] >> (j & 31)) & 1;
-    return true;
-}
-
-template <class T, class H, bool GRAD>
-__global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, const T *logits, const T *grad, T *out) {
-#pragma clang fp contract(off)
-    __shared__ uint32_t counts[CHUNK];
-    const int chunks = (a.k + CHUNK - 1) / CHUNK;
-    const int64_t items = a.n * chunks;
-    const bool history = a.history_dev != nullptr && a.t > 0;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t row = item / chunks;
-        const int first = static_cast<int>(item - row * chunks) * CHUNK, width = min(CHUNK, a.k - first);
-        if (history) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < width; i += THREADS) counts[i] = 0;
-            __syncthreads();
-            count_history<H>(a, row, first, width, counts, threadIdx.x, THREADS);
-            __syncthreads();
-        }
-        const float rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
-        const float presence = a.presence_dev ? a.presence_dev[row] : a.presence;
-        const float frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
-        for (int i = threadIdx.x; i < width; i += THREADS) {
-            const int j = first + i;
-            const uint32_t c = history ? counts[i] : 0;
-            float x = static_cast<float>(logits[row * a.logits_stride + j]);
-            if (GRAD) {
-                float g = static_cast<float>(grad[row * a.grad_stride + j]);
-                if (c > 0) g = x > 0.f ? g / rep : g * rep;
-                out[row * a.out_stride + j] = static_cast<T>(allowed(a, row, j) ? g : 0.f);
-            } else {
-                if (c > 0) x = (x > 0.f ? x / rep : x * rep) - presence;
-                x = x - frequency * static_cast<float>(c);
-                if (a.bias_dev) x = x + a.bias_dev[row * a.bias_stride + j];
-                out[row * a.out_stride + j] = static_cast<T>(allowed(a, row, j) ? x : NEG_INF);
+    __device__ __forceinline__ Row(const T *row, int tokens, int thread) : x(row), k(tokens), lane(thread), vecs((tokens + LANES * V - 1) / (LANES * V)) {
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) fetch(j, held[j]);
+    }
+    // f(number of the vector, its words) for all of this thread's vectors.  The empty statements keep a pass from sharing its
+    // conversions with the next one and the barriers keep the vectors apart: either would take several times the registers.
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+        if constexpr (HELD > 0) {
+#pragma unroll
+            for (int j = 0; j < HELD; ++j) {
+                asm volatile("" : "+v"(held[j][0]), "+v"(held[j][1]), "+v"(held[j][2]), "+v"(held[j][3]));
+                f(j, held[j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            for (int j = 0; j < vecs; j += 4) {  // four loads under way; what lies behind the row is -inf
+                uint32_t w[4][4];
+#pragma unroll
+                for (int o = 0; o < 4; ++o) fetch(j + o, w[o]);
+#pragma unroll
+                for (int o = 0; o < 4; ++o) f(j + o, w[o]);
             }
         }
+    }
+    __device__ __forceinline__ int token(int j, int i) const { return (j * LANES + lane) * V + i; }
+};
+
+// f combined over the threads of a row, known to all of them
+template <int LANES, class X, class F>
+__device__ __forceinline__ X over_row(X v, X *shared, F f) {
+#pragma unroll
+    for (int by = (LANES < 64 ? LANES : 64) / 2; by > 0; by /= 2) v = f(v, __shfl_xor(v, by, 64));
+    if constexpr (LANES > 64) {
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = shared[0];
+#pragma unroll
+        for (int w = 1; w < LANES / 64; ++w) v = f(v, shared[w]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // NaN if one of them is
+template <class X>
+__device__ __forceinline__ X sum_of(X a, X b) { return a + b; }
+
+// exp(2 ln 2 * z) for z <= 0, NaN for NaN: the exponential instruction gives nothing below 2^-126, the square of half as much
+// goes down to the smallest float.
+__device__ __forceinline__ float exp_twice(float z) {
+    const float h = __builtin_amdgcn_exp2f(z);
+    return h * h;
+}
+constexpr float HALF_LOG2E = 0.72134752044448170368f, TWICE_LN2 = 1.38629436111989061883f;
+constexpr float DEEP = -200.f;  // exp_twice of it is 0
+
+// ---- adjustment of logits ------------------------------------------------------------------------------------------
+
+// A block counts a stretch of tokens' occurrences in their rows' histories in LDS, then the stretch streams through once: of
+// `lanes` threads to a row (a power of two) each takes up to STRETCH 16-byte vectors, whose loads are under way while the
+// history is counted.  Short rows share a block, a row longer than a block's stretch is cut, and each piece looks through the
+// whole history (a few KB that the cache holds).
+constexpr int STRETCH = 4;
+
+template <class T, class H, bool GRAD>
+__global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, const T *logits, const T *grad, T *out) {
+#pragma clang fp contract(off)
+    constexpr int V = WIDE<T>, PIECE = THREADS * STRETCH * V;
+    __shared__ __align__(16) uint32_t counts_s[PIECE];
+    const int lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * STRETCH * V;
+    const int pieces = (a.k + width - 1) / width;  // 1 where rows share a block
+    const int64_t items = (a.n + per_block - 1) / per_block * pieces;
+    const bool history = a.history_dev != nullptr && a.t > 0;
+    uint32_t *counts = counts_s + sub * width;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t block_row = pieces == 1 ? item : item / pieces;
+        const int first = static_cast<int>(item - block_row * pieces) * width;
+        const int64_t row = block_row * per_block + sub;
+        const bool live = row < a.n;
+        Vec<T, V> x[STRETCH], g[STRETCH];
+#pragma unroll
+        for (int j = 0; j < STRETCH; ++j) {
+            const int at = first + (j * lanes + lane) * V;
+            if (live && at + V <= a.k) {
+                x[j] = *reinterpret_cast<const Vec<T, V> *>(logits + row * a.logits_stride + at);
+                if (GRAD) g[j] = *reinterpret_cast<const Vec<T, V> *>(grad + row * a.grad_stride + at);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[j].v[i] = live && at + i < a.k ? logits[row * a.logits_stride + at + i] : static_cast<T>(0.f);
+                    if (GRAD) g[j].v[i] = live && at + i < a.k ? grad[row * a.grad_stride + at + i] : static_cast<T>(0.f);
+                }
+            }
+        }
+        if (history) {
+            const int len = !live ? 0 : (a.lengths_dev ? min(max(a.lengths_dev[row], 0), a.t) : a.t);
+            const H *h = static_cast<const H *>(a.history_dev) + row * a.history_stride;
+#pragma unroll
+            for (int j = 0; j < STRETCH; ++j)
+#pragma unroll
+                for (int i = 0; i < V; i += 4) *reinterpret_cast<uint4 *>(&counts[(j * lanes + lane) * V + i]) = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            const int end = min(width, a.k - first);
+            for (int i = lane; i < len; i += lanes) {
+                const int64_t j = static_cast<int64_t>(h[i]) - first;
+                if (j >= 0 && j < end) atomicAdd(&counts[j], 1u);
+            }
+            __syncthreads();
+        }
+        if (live) {
+            const float rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
+            const float presence = a.presence_dev ? a.presence_dev[row] : a.presence;
+            const float frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
+#pragma unroll
+            for (int j = 0; j < STRETCH; ++j) {
+                const int at = first + (j * lanes + lane) * V;
+                if (at >= a.k) break;
+                const bool whole = at + V <= a.k;
+                uint32_t allow = ~0u;  // bit i: token at + i
+                if (a.mask_kind == MG_MASK_BITS) {  // `at` is a multiple of V, 4 or 8: its bits lie in one byte
+                    allow = static_cast<const uint8_t *>(a.mask_dev)[4 * row * a.mask_stride + (at >> 3)] >> (at & 7);
+                } else if (a.mask_kind == MG_MASK_BYTES) {
+                    const uint8_t *m = static_cast<const uint8_t *>(a.mask_dev) + row * a.mask_stride + at;
+                    allow = 0;
+                    if (whole) {
+                        const Vec<uint8_t, V> v = *reinterpret_cast<const Vec<uint8_t, V> *>(m);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) allow |= (v.v[i] != 0) << i;
+                    } else {
+                        for (int i = 0; at + i < a.k; ++i) allow |= (m[i] != 0) << i;
+                    }
+                }
+                uint32_t c[V] = {};
+                if (history)
+#pragma unroll
+                    for (int i = 0; i < V; i += 4) {
+                        const uint4 q = *reinterpret_cast<const uint4 *>(&counts[(j * lanes + lane) * V + i]);
+                        c[i] = q.x, c[i + 1] = q.y, c[i + 2] = q.z, c[i + 3] = q.w;
+                    }
+                float y[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    y[i] = static_cast<float>(x[j].v[i]);
+                    if (GRAD) {
+                        const bool up = y[i] > 0.f;
+                        y[i] = static_cast<float>(g[j].v[i]);
+                        if (c[i] > 0) y[i] = up ? y[i] / rep : y[i] * rep;
+                    } else {
+                        if (c[i] > 0) y[i] = (y[i] > 0.f ? y[i] / rep : y[i] * rep) - presence;
+                        y[i] = y[i] - frequency * static_cast<float>(c[i]);
+                    }
+                }
+                if (!GRAD && a.bias_dev) {
+                    const float *b = a.bias_dev + row * a.bias_stride + at;
+                    if (whole) {
+                        float v[V];
+                        load<float, V>(b, v);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) y[i] = y[i] + v[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            if (at + i < a.k) y[i] = y[i] + b[i];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (!((allow >> i) & 1)) y[i] = GRAD ? 0.f : NEG_INF;
+                T *to = out + row * a.out_stride + at;
+                if (whole) {
+                    store<T, V>(to, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (at + i < a.k) to[i] = static_cast<T>(y[i]);
+                }
+            }
+        }
+        if (history) __syncthreads();  // the counters are read
     }
 }
 
@@ -831,9 +988,6 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
 
 // ---- draw ----------------------------------------------------------------------------------------------------------
 
-template <class T>
-__device__ __forceinline__ T shuffle_down(T v, int by) { return __shfl_down(v, by, 64); }
-
 __device__ __forceinline__ void put_token(void *tokens, int type, int64_t row, int64_t token) {
     if (type == MG_U8)
         static_cast<uint8_t *>(tokens)[row] = static_cast<uint8_t>(token);
@@ -849,84 +1003,278 @@ __device__ __forceinline__ int64_t get_token(const void *tokens, int type, int64
     return static_cast<const int64_t *>(tokens)[row];
 }
 
-// One block per row: the maximum, then every thread's share of the total (a run of adjacent tokens), then the thread whose run
-// holds the border walks it.
-template <class T>
-__global__ __launch_bounds__(THREADS) void draw_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type,
-                                                       void *tokens, float *logprob) {
-    __shared__ float best_s[THREADS];
-    __shared__ int arg_s[THREADS];
-    __shared__ double sum_s[THREADS];
-    const int tid = threadIdx.x;
-    const int run = (l.k + THREADS - 1) / THREADS;
-    for (int64_t row = blockIdx.x; row < l.n; row += gridDim.x) {
-        const T *x = logits + row * l.stride;
-        const double inv_t = 1.0 / static_cast<double>(l.temperature_dev ? l.temperature_dev[row] : l.temperature);
-        const int lo = min(tid * run, l.k), hi = min(lo + run, l.k);
-        float best = NEG_INF;
-        int arg = l.k;
-        for (int j = lo; j < hi; ++j) {
-            const float v = static_cast<float>(x[j]);
-            if (v > best) {
-                best = v;
-                arg = j;
+// The draw from a row: total of the probabilities, then the vector, the thread and the token at whose sum the border lies.  All
+// sums are in 64 bits.  The exponentials first are 32-bit ones, each off by at most (5 |z| + 5) 2^-24 of itself (z: five
+// roundings; a square of something off by 2^-23), a vector's sum by 8 more, and sum p |z| / sum p <= ln k (an entropy), so a sum
+// of them and the border are off by at most (5 ln k + 13) 2^-24 of the total each.  Where the border comes nearer to either end of the token found than
+// one and a half times both, the row is done again with 64-bit exponentials, at ten times the instructions.
+struct DrawShared {
+    double sums[16 * 16], reduce[16], before;
+    float reduce_f[16];
+    int reduce_i[16], place;
+};
+
+template <class T, int LANES, int HELD>
+struct Draw {
+    using R = Row<T, LANES, HELD>;
+    static constexpr int V = R::V, WAVES = LANES > 64 ? LANES / 64 : 1, VECS = HELD ? HELD : 1;
+
+    template <bool EXACT>
+    static __device__ __forceinline__ double p(float x, float m, float c, double inv_t) {
+        if constexpr (EXACT)
+            return exp((static_cast<double>(x) - m) * inv_t);
+        else
+            return exp_twice((x - m) * c);
+    }
+
+    // a vector's sum; of 32-bit exponentials in 32 bits
+    template <bool EXACT>
+    static __device__ __forceinline__ double sum_of_vector(const uint32_t *v, float m, float c, double inv_t) {
+        if constexpr (EXACT) {
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum += p<true>(element<T>(v, i), m, c, inv_t);
+            return sum;
+        } else {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float h = __builtin_amdgcn_exp2f((element<T>(v, i) - m) * c);
+                sum = fmaf(h, h, sum);
+            }
+            return sum;
+        }
+    }
+
+    // token (or -1 where rounding left none), the total, and the sums before and behind the token
+    template <bool EXACT>
+    static __device__ __forceinline__ int find(R &row, DrawShared &s, float m, double inv_t, double u, bool draws, double &total, double &before, double &behind) {
+        const float c = static_cast<float>(inv_t) * HALF_LOG2E;
+        double mine = 0.0, part[VECS];
+        row.each([&](int j, const uint32_t *v) {
+            double sum = sum_of_vector<EXACT>(v, m, c, inv_t);
+            mine += sum;
+            if (HELD) {
+                asm volatile("" : "+v"(sum));
+                part[HELD ? j : 0] = sum;
+            }
+        });
+        const int wave = LANES > 64 ? threadIdx.x / 64 : 0, lane = row.lane % 64;
+        constexpr int SPAN = LANES < 64 ? LANES : 64;
+        // inclusive sums over the threads of a wave (or of a shorter row)
+        auto upto = [&](double v) {
+#pragma unroll
+            for (int by = 1; by < SPAN; by *= 2) {
+                const double o = __shfl_up(v, by, SPAN);
+                if ((lane & (SPAN - 1)) >= by) v += o;
+            }
+            return v;
+        };
+        int vec = -1, at_wave = 0;  // where the border lies
+        before = 0.0;
+        double border = 0.0;
+        if constexpr (HELD > 0 && WAVES > 1) {
+            // the waves' sums of each vector: every exchange halves the vectors that a thread adds up
+            int of = 0;
+#pragma unroll
+            for (int half = VECS / 2, by = 32; half > 0; half /= 2, by /= 2) {
+                const bool upper = lane & by;
+                of += upper ? half : 0;
+#pragma unroll
+                for (int j = 0; j < half; ++j) {
+                    const double give = upper ? part[j] : part[j + half], keep = upper ? part[j + half] : part[j];
+                    part[j] = keep + __shfl_xor(give, by, 64);
+                }
+            }
+#pragma unroll
+            for (int by = 32 / VECS; by > 0; by /= 2) part[0] += __shfl_xor(part[0], by, 64);
+            __syncthreads();
+            if (lane % (64 / VECS) == 0) s.sums[of * WAVES + wave] = part[0];
+            __syncthreads();
+            // in the order of the tokens: vectors, then waves; every wave does this by itself, four sums a thread at most
+            constexpr int N = VECS * WAVES, EACH = (N + 63) / 64;
+            double own[EACH], run = 0.0;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                own[i] = lane * EACH + i < N ? s.sums[lane * EACH + i] : 0.0;
+                run += own[i];
+            }
+            const double end = upto(run);
+            total = __shfl(end, 63, 64);
+            if (!draws) return -1;
+            border = u * total;
+            double sum = lane ? end - run : 0.0, start = 0.0;
+            int found = N;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                if (found == N && sum + own[i] > border && lane * EACH + i < N) {
+                    found = lane * EACH + i;
+                    start = sum;
+                }
+                sum += own[i];
+            }
+            const uint64_t any = __ballot(found < N);
+            if (any) {
+                const int from = __builtin_ctzll(any);
+                found = __shfl(found, from, 64);
+                before = __shfl(start, from, 64);
+                vec = found / WAVES;
+                at_wave = found % WAVES;
+            }
+        } else if constexpr (HELD > 0) {
+            total = over_row<LANES>(mine, s.reduce, sum_of<double>);
+            if (!draws) return -1;
+            border = u * total;
+            double sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < VECS; ++j) {
+                const double all = VECS == 1 ? total : over_row<LANES>(part[j], s.reduce, sum_of<double>);
+                if (vec < 0 && sum + all > border) {
+                    vec = j;
+                    before = sum;
+                }
+                sum += all;
+            }
+        } else {
+            // one vector of every thread after another: the waves' sums, the border
+            total = over_row<LANES>(mine, s.reduce, sum_of<double>);
+            if (!draws) return -1;
+            border = u * total;
+            double sum = 0.0;
+            bool done = false;
+            for (int j = 0; j < row.vecs && !done; ++j) {
+                uint32_t v[4];
+                row.fetch(j, v);
+                double all = sum_of_vector<EXACT>(v, m, c, inv_t);
+#pragma unroll
+                for (int by = SPAN / 2; by > 0; by /= 2) all += __shfl_xor(all, by, 64);
+                if constexpr (WAVES > 1) {
+                    __syncthreads();
+                    if (lane == 0) s.reduce[wave] = all;
+                    __syncthreads();
+                }
+#pragma unroll 1
+                for (int w = 0; w < WAVES; ++w) {
+                    const double of_wave = WAVES > 1 ? s.reduce[w] : all;
+                    if (!done && sum + of_wave > border) {
+                        done = true;
+                        vec = j;
+                        at_wave = w;
+                        before = sum;
+                    }
+                    sum += of_wave;
+                }
             }
         }
-        __syncthreads();
-        best_s[tid] = best;
-        arg_s[tid] = arg;
-        __syncthreads();
-        for (int half = THREADS / 2; half > 0; half /= 2) {  // runs are in order: the left one wins a tie
-            if (tid < half && (best_s[tid + half] > best_s[tid] || (best_s[tid + half] == best_s[tid] && arg_s[tid + half] < arg_s[tid]))) {
-                best_s[tid] = best_s[tid + half];
-                arg_s[tid] = arg_s[tid + half];
+        // the thread, then the token; told to all threads of the row
+        if (wave != at_wave) vec = -1;
+        int token = -1;
+        if (vec >= 0) {
+            uint32_t v[4];  // read again: an index into registers would cost more
+            row.fetch(vec, v);
+            const double here = sum_of_vector<EXACT>(v, m, c, inv_t), end = before + upto(here);
+            const int shift = (threadIdx.x % 64) / SPAN * SPAN;
+            const uint64_t threads = (~0ull >> (64 - SPAN)) << shift;
+            const uint64_t above = __ballot(end > border) & threads, some = __ballot(here > 0.0) & threads;
+            // rounding may leave none above it: the last one that has any then
+            const int at = (above ? __builtin_ctzll(above) : (some ? 63 - __builtin_clzll(some) : shift)) - shift;
+            if ((lane & (SPAN - 1)) == at) {
+                double sum = end - here;
+                if (at == 0) sum = before;
+                before = sum;
+                behind = sum;
+                bool done = false;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const double q = p<EXACT>(element<T>(v, i), m, c, inv_t);
+                    if (!done && q > 0.0) {
+                        token = row.token(vec, i);
+                        before = sum;
+                        behind = sum + q;
+                        done = sum + q > border;
+                    }
+                    sum += q;
+                }
+            }
+            token = __shfl(token, shift + at, 64);
+            before = __shfl(before, shift + at, 64);
+            behind = __shfl(behind, shift + at, 64);
+        }
+        if constexpr (WAVES > 1) {
+            __syncthreads();
+            if (threadIdx.x == 0) s.place = -1;
+            __syncthreads();
+            if (vec >= 0 && lane == 0) {
+                s.place = token;
+                s.before = before;
+                s.reduce[0] = behind;
             }
             __syncthreads();
+            token = s.place;
+            before = s.before;
+            behind = s.reduce[0];
         }
-        best = best_s[0];
-        arg = arg_s[0];
-        double sum = 0.0;
-        if (best != NEG_INF)
-            for (int j = lo; j < hi; ++j) sum += exp((static_cast<double>(static_cast<float>(x[j])) - best) * inv_t);
-        else  // nothing to draw from, unless a NaN is among them
-            for (int j = lo; j < hi; ++j)
-                if (static_cast<float>(x[j]) != NEG_INF) sum = __builtin_nan("");
-        sum_s[tid] = sum;
-        __syncthreads();
-        if (tid == 0) {
-            double total = 0.0;
-            for (int i = 0; i < THREADS; ++i) total += sum_s[i];
-            int64_t token = -1;
-            double lp = total == 0.0 ? -__builtin_inf() : __builtin_nan("");
-            if (total > 0.0) {
-                token = arg;
-                if (uniforms) {
-                    const double u = uniforms_type == MG_F64 ? static_cast<const double *>(uniforms)[row] : static_cast<double>(static_cast<const float *>(uniforms)[row]);
-                    const double border = u * total;
-                    double upto = 0.0;
-                    int last = arg;
-                    bool done = false;
-                    for (int i = 0; i < THREADS && !done; ++i) {
-                        if (!(upto + sum_s[i] > border) && i * run + run < l.k) {
-                            upto += sum_s[i];
-                            continue;
-                        }
-                        for (int j = i * run; j < min(i * run + run, l.k); ++j) {
-                            const double p = exp((static_cast<double>(static_cast<float>(x[j])) - best) * inv_t);
-                            upto += p;
-                            if (p > 0.0) last = j;
-                            if (upto > border) {
-                                done = true;
-                                break;
-                            }
-                        }
-                    }
-                    token = last;
+        return token;
+    }
+};
+
+template <class T, int LANES, int HELD>
+__global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type, void *tokens, float *logprob) {
+    using D = Draw<T, LANES, HELD>;
+    __shared__ DrawShared s;
+    constexpr int ROWS = BLOCK<LANES> / LANES;
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += static_cast<int64_t>(gridDim.x) * ROWS) {
+        typename D::R row(logits + i * l.stride, l.k, lane);
+        const double inv_t = 1.0 / static_cast<double>(l.temperature_dev ? l.temperature_dev[i] : l.temperature);
+        float m = NEG_INF;
+        row.each([&](int, const uint32_t *v) {
+#pragma unroll
+            for (int e = 0; e < D::V; ++e) m = larger(m, element<T>(v, e));
+        });
+        m = over_row<LANES>(m, s.reduce_f, larger);
+        int token = -1;
+        double total = 0.0, before = 0.0, behind = 0.0;
+        if (fabsf(m) < -NEG_INF) {
+            const double u = !uniforms ? 0.0 : (uniforms_type == MG_F64 ? static_cast<const double *>(uniforms)[i] : static_cast<double>(static_cast<const float *>(uniforms)[i]));
+            token = D::template find<false>(row, s, m, inv_t, u, uniforms != nullptr, total, before, behind);
+            if (uniforms) {
+                const double off = total * 1.5 * (10.0 * __logf(static_cast<float>(l.k)) + 26.0) * 0x1p-24, border = u * total;
+                if (token < 0 || behind - border < off || border - before < off) {
+                    Row<T, LANES, 0> again(logits + i * l.stride, l.k, lane);
+                    token = Draw<T, LANES, 0>::template find<true>(again, s, m, inv_t, u, true, total, before, behind);
                 }
-                lp = (static_cast<double>(static_cast<float>(x[token])) - best) * inv_t - log(total);
             }
-            put_token(tokens, l.tokens_type, row, token);
-            if (logprob) logprob[row] = static_cast<float>(lp);
+            if (logprob && total < 1.0625) {  // little beside the maximum, whose 1 took some of it: each added in 64 bits
+                double sum = 0.0;
+                const float c = static_cast<float>(inv_t) * HALF_LOG2E;
+                row.each([&](int, const uint32_t *v) {
+#pragma unroll
+                    for (int e = 0; e < D::V; ++e) sum += exp_twice((element<T>(v, e) - m) * c);
+                });
+                total = over_row<LANES>(sum, s.reduce, sum_of<double>);
+            }
+            if (token < 0) {  // the largest, the lowest of equal ones; for a draw: no sum passed the border, the last that has any
+                const bool last = uniforms != nullptr;
+                int found = last ? -1 : l.k;
+#pragma unroll 1
+                for (int j = 0; j < row.vecs; ++j) {
+                    uint32_t v[4];
+                    row.fetch(j, v);
+#pragma unroll
+                    for (int e = 0; e < D::V; ++e) {
+                        const float x = element<T>(v, e);
+                        if (last ? exp((static_cast<double>(x) - m) * inv_t) > 0.0 : x == m) found = last ? max(found, row.token(j, e)) : min(found, row.token(j, e));
+                    }
+                }
+                token = over_row<LANES>(found, s.reduce_i, [last](int a, int b) { return last ? max(a, b) : min(a, b); });
+            }
+        }
+        if (lane == 0) {
+            put_token(tokens, l.tokens_type, i, token);
+            if (logprob)
+                logprob[i] = token < 0 ? (m == NEG_INF ? NEG_INF : __builtin_nanf(""))
+                                       : static_cast<float>((static_cast<double>(static_cast<float>(logits[i * l.stride + token])) - m) * inv_t - log(total));
         }
     }
 }
@@ -1000,51 +1348,6 @@ struct Soft {
     float m, r, t;
 };
 
-__device__ __forceinline__ void take(Soft &s, float x, float inv_t) {
-    if (x > s.m) {
-        if (s.m == NEG_INF) {
-            s.r += 1.f;  // 0, or NaN if a NaN came before
-        } else {
-            const float d = (s.m - x) * inv_t, e = expf(d);
-            s.t = e > 0.f ? e * (s.t + (1.f + s.r) * d) : 0.f;
-            s.r = (1.f + s.r) * e;
-        }
-        s.m = x;
-    } else if (x != NEG_INF) {
-        const float z = (x - s.m) * inv_t, e = expf(z);
-        s.r += e;
-        if (e > 0.f) s.t += e * z;
-    }
-}
-
-__device__ __forceinline__ Soft merge(Soft a, Soft b, float inv_t) {
-    if (b.m > a.m) {
-        const Soft c = a;
-        a = b;
-        b = c;
-    }
-    if (b.m == NEG_INF) {
-        a.r += b.r + 1.f;  // 0, or NaN
-        return a;
-    }
-    const float d = (b.m - a.m) * inv_t, e = expf(d), s = 1.f + b.r;
-    a.r += s * e;
-    if (e > 0.f) a.t += e * (b.t + s * d);
-    return a;
-}
-
-__device__ __forceinline__ Soft merge_wave(Soft s, float inv_t) {
-#pragma unroll
-    for (int by = 32; by > 0; by /= 2) {
-        Soft o;
-        o.m = shuffle_down(s.m, by);
-        o.r = shuffle_down(s.r, by);
-        o.t = shuffle_down(s.t, by);
-        s = merge(s, o, inv_t);
-    }
-    return s;
-}
-
 // What the slope of a finished row needs: its maximum, the logarithm of its total, its entropy.
 __device__ __forceinline__ float4 row_stats(const Soft &s) {
     const bool empty = s.m == NEG_INF && s.r == -1.f;
@@ -1067,23 +1370,54 @@ __device__ __forceinline__ void row_result(const MgLogits &l, const T *x, int64_
     if (stats) reinterpret_cast<float4 *>(stats)[row] = st;
 }
 
-template <class T>
-__global__ __launch_bounds__(THREADS) void logprob_kernel(MgLogits l, const T *logits, const void *tokens, float *logprob,
-                                                          float *entropy, float *stats) {
-    __shared__ Soft part[THREADS / 64];
-    for (int64_t row = blockIdx.x; row < l.n; row += gridDim.x) {
-        const T *x = logits + row * l.stride;
-        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
+template <class T, int LANES, int HELD>
+__global__ __launch_bounds__(BLOCK<LANES>) void logprob_kernel(MgLogits l, const T *logits, const void *tokens, float *logprob, float *entropy, float *stats) {
+    constexpr int ROWS = BLOCK<LANES> / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
+    __shared__ float shared[WAVES];
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += static_cast<int64_t>(gridDim.x) * ROWS) {
+        Row<T, LANES, HELD> row(logits + i * l.stride, l.k, lane);
+        constexpr int V = WIDE<T>;
+        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature), c = inv_t * HALF_LOG2E;
         Soft s{NEG_INF, -1.f, 0.f};
-        for (int j = threadIdx.x; j < l.k; j += THREADS) take(s, static_cast<float>(x[j]), inv_t);
-        s = merge_wave(s, inv_t);
-        __syncthreads();
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < THREADS / 64; ++w) s = merge(s, part[w], inv_t);
-            row_result(l, x, row, s, inv_t, tokens, logprob, entropy, stats);
+        row.each([&](int, const uint32_t *v) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) s.m = larger(s.m, element<T>(v, e));
+        });
+        s.m = over_row<LANES>(s.m, shared, larger);
+        if (s.m > NEG_INF && s.m < -NEG_INF) {
+            float sum = 0.f, t = 0.f;
+            row.each([&](int, const uint32_t *v) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float z = fmaxf((element<T>(v, e) - s.m) * c, DEEP), p = exp_twice(z);
+                    sum += p;
+                    t = fmaf(p, z, t);
+                }
+            });
+            asm volatile("" : "+v"(sum), "+v"(t));  // t now, not where it is used: every p and z would wait for it
+            sum = over_row<LANES>(sum, shared, sum_of<float>);
+            s.t = over_row<LANES>(t, shared, sum_of<float>) * TWICE_LN2;
+            s.r = sum - 1.f;
+            if (sum < 1.0625f) {  // little beside the maximum: the sum again without it
+                float rest = 0.f;
+                int equal = 0;
+                row.each([&](int, const uint32_t *v) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float x = element<T>(v, e);
+                        equal += x == s.m;
+                        rest += x == s.m ? 0.f : exp_twice(fmaxf((x - s.m) * c, DEEP));
+                    }
+                });
+                s.r = over_row<LANES>(rest + static_cast<float>(equal), shared, sum_of<float>);
+                if (over_row<LANES>(equal, reinterpret_cast<int *>(shared), sum_of<int>) == 1) s.r = over_row<LANES>(rest, shared, sum_of<float>);
+                else s.r -= 1.f;
+            }
+        } else if (s.m != NEG_INF) {
+            s.r = __builtin_nanf("");
         }
+        if (lane == 0) row_result(l, logits + i * l.stride, i, s, inv_t, tokens, logprob, entropy, stats);
     }
 }
 
@@ -1095,19 +1429,42 @@ __device__ __forceinline__ float logprob_slope(float x, bool is_token, float4 st
     return is_token ? -g * expm1f(lp) - p * hs : -p * (g + hs);
 }
 
+// One pass over the logits, `lanes` threads (a power of two) to a row or to a piece of one.
 template <class T>
-__global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, const T *logits, const void *tokens, const float *stats,
-                                                               const float *grad_lp, int64_t lp_stride, const float *grad_h,
-                                                               int64_t h_stride, T *out) {
-    for (int64_t row = blockIdx.x; row < l.n; row += gridDim.x) {
+__global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int lanes, const T *logits, const void *tokens, const float *stats,
+                                                               const float *grad_lp, int64_t lp_stride, const float *grad_h, int64_t h_stride, T *out) {
+    constexpr int V = WIDE<T>, TAKES = 4;
+    const int lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * TAKES * V;
+    const int pieces = (l.k + width - 1) / width;
+    const int64_t items = (l.n + per_block - 1) / per_block * pieces;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t block_row = pieces == 1 ? item : item / pieces;
+        const int first = static_cast<int>(item - block_row * pieces) * width;
+        const int64_t row = block_row * per_block + sub;
+        if (row >= l.n) continue;
         const T *x = logits + row * l.stride;
+        T *to = out + row * l.k;
         const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
         const float4 st = reinterpret_cast<const float4 *>(stats)[row];
         const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
         const float g = token >= 0 && token < l.k ? grad_lp[row * lp_stride] * inv_t : 0.f;
         const float h = grad_h ? grad_h[row * h_stride] * inv_t : 0.f;
-        for (int j = threadIdx.x; j < l.k; j += THREADS)
-            out[row * l.k + j] = static_cast<T>(logprob_slope(static_cast<float>(x[j]), j == token, st, inv_t, g, h));
+#pragma unroll
+        for (int j = 0; j < TAKES; ++j) {
+            const int at = first + (j * lanes + lane) * V;
+            if (at >= l.k) break;
+            float v[V];
+            load_part<T, V>(x + at, l.k - at, v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = logprob_slope(v[i], false, st, inv_t, g, h);
+            if (token >= at && token < at + V) {
+                const float own = logprob_slope(static_cast<float>(x[token]), true, st, inv_t, g, h);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (at + i == token) v[i] = own;
+            }
+            store_part<T, V>(to + at, l.k - at, v);
+        }
     }
 }
 
@@ -1366,6 +1723,42 @@ void with_size(int k, F f) {
         f(Size<SHORT>{});
 }
 
+// f(threads to a row, vectors that each holds): the fewest threads that hold a row of `vecs` vectors with one each, a wave up to
+// four each, then blocks of 256 and of 1024 for as many as their registers take beside what f's kernel needs
+template <int LANES, int HELD>
+struct Shape {
+    static constexpr int lanes = LANES, held = HELD;
+};
+template <int WIDEST, class F>
+void with_shape(int64_t vecs, F f) {
+    if (vecs <= 8)
+        f(Shape<8, 1>{});
+    else if (vecs <= 16)
+        f(Shape<16, 1>{});
+    else if (vecs <= 32)
+        f(Shape<32, 1>{});
+    else if (vecs <= 64)
+        f(Shape<64, 1>{});
+    else if (vecs <= 128)
+        f(Shape<64, 2>{});
+    else if (vecs <= 256)
+        f(Shape<64, 4>{});
+    else if (vecs <= 512)
+        f(Shape<256, 2>{});
+    else if (vecs <= 1024)
+        f(Shape<256, 4>{});
+    else if (vecs <= 2048)
+        f(Shape<256, 8>{});
+    else if (vecs <= 4096)
+        f(Shape<256, 16>{});
+    else if (WIDEST >= 8 && vecs <= 8192)
+        f(Shape<1024, WIDEST < 8 ? WIDEST : 8>{});
+    else if (WIDEST >= 16 && vecs <= 16384)
+        f(Shape<1024, WIDEST>{});
+    else
+        f(Shape<1024, 0>{});
+}
+
 int adjust_args(const char *who, const MgAdjust *a) {
     if (!a) return refuse(MG_EINVAL, "%s: null argument", who);
     if (a->n < 0 || a->n > MOST_ROWS) return refuse(MG_EINVAL, "%s: n %lld not supported (0..2^31 - 1)", who, static_cast<long long>(a->n));
@@ -1396,8 +1789,11 @@ void launch_adjust(const MgAdjust &a, const void *logits, const void *grad, void
                 hipLaunchKernelGGL((adjust_short_kernel<T, H, GRAD, K>), dim3((a.n + ROWS - 1) / ROWS), dim3(ROWS), 0, stream, a, x, g, y);
             });
         } else {
-            const int64_t chunks = (a.k + CHUNK - 1) / CHUNK;
-            hipLaunchKernelGGL((adjust_kernel<T, H, GRAD>), dim3(blocks_for(a.n * chunks)), dim3(THREADS), 0, stream, a, x, g, y);
+            constexpr int TAKES = STRETCH * WIDE<T>;
+            int lanes = 8;  // the fewest that take a row at once
+            while (lanes < THREADS && lanes * TAKES < a.k) lanes *= 2;
+            const int64_t per_block = THREADS / lanes, pieces = (a.k + lanes * TAKES - 1) / (lanes * TAKES);
+            hipLaunchKernelGGL((adjust_kernel<T, H, GRAD>), dim3(blocks_for((a.n + per_block - 1) / per_block * pieces)), dim3(THREADS), 0, stream, a, lanes, x, g, y);
         }
     });
 }
@@ -1490,8 +1886,12 @@ int mg_draw(const MgLogits *l, const void *logits_dev, const void *uniforms_dev,
                 hipLaunchKernelGGL((draw_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0,
                                    static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), uniforms_dev, uniforms_type, tokens_dev, logprob_dev);
             });
-        hipLaunchKernelGGL((draw_kernel<T>), dim3(blocks_for(l->n)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *l,
-                           static_cast<const T *>(logits_dev), uniforms_dev, uniforms_type, tokens_dev, logprob_dev);
+        with_shape<0>((l->k + WIDE<T> - 1) / WIDE<T>, [&](auto shape) {
+            using S = decltype(shape);
+            constexpr int ROWS = BLOCK<S::lanes> / S::lanes;
+            hipLaunchKernelGGL((draw_kernel<T, S::lanes, S::held>), dim3(blocks_for((l->n + ROWS - 1) / ROWS)), dim3(BLOCK<S::lanes>), 0,
+                               static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), uniforms_dev, uniforms_type, tokens_dev, logprob_dev);
+        });
     });
     return launched("mg_draw");
 }
@@ -1513,8 +1913,12 @@ int mg_token_logprobs(const MgLogits *l, const void *logits_dev, const void *tok
                 hipLaunchKernelGGL((logprob_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0,
                                    static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), tokens_dev, logprob_dev, entropy_dev, stats_dev);
             });
-        hipLaunchKernelGGL((logprob_kernel<T>), dim3(blocks_for(l->n)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *l,
-                           static_cast<const T *>(logits_dev), tokens_dev, logprob_dev, entropy_dev, stats_dev);
+        with_shape<16>((l->k + WIDE<T> - 1) / WIDE<T>, [&](auto shape) {
+            using S = decltype(shape);
+            constexpr int ROWS = BLOCK<S::lanes> / S::lanes;
+            hipLaunchKernelGGL((logprob_kernel<T, S::lanes, S::held>), dim3(blocks_for((l->n + ROWS - 1) / ROWS)), dim3(BLOCK<S::lanes>), 0,
+                               static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), tokens_dev, logprob_dev, entropy_dev, stats_dev);
+        });
     });
     return launched("mg_token_logprobs");
 }
@@ -1535,9 +1939,13 @@ int mg_token_logprobs_grad(const MgLogits *l, const void *logits_dev, const void
                                    static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), tokens_dev, grad_logprob_dev, grad_logprob_stride,
                                    grad_entropy_dev, grad_entropy_stride, static_cast<T *>(out_dev));
             });
-        hipLaunchKernelGGL((logprob_grad_kernel<T>), dim3(blocks_for(l->n)), dim3(THREADS), 0, static_cast<hipStream_t>(stream), *l,
-                           static_cast<const T *>(logits_dev), tokens_dev, stats_dev, grad_logprob_dev, grad_logprob_stride, grad_entropy_dev,
-                           grad_entropy_stride, static_cast<T *>(out_dev));
+        constexpr int TAKES = 4 * WIDE<T>;
+        int lanes = 8;
+        while (lanes < THREADS && lanes * TAKES < l->k) lanes *= 2;
+        const int64_t per_block = THREADS / lanes, pieces = (l->k + lanes * TAKES - 1) / (lanes * TAKES);
+        hipLaunchKernelGGL((logprob_grad_kernel<T>), dim3(blocks_for((l->n + per_block - 1) / per_block * pieces)), dim3(THREADS), 0,
+                           static_cast<hipStream_t>(stream), *l, lanes, static_cast<const T *>(logits_dev), tokens_dev, stats_dev, grad_logprob_dev,
+                           grad_logprob_stride, grad_entropy_dev, grad_entropy_stride, static_cast<T *>(out_dev));
     });
     return launched("mg_token_logprobs_grad");
 }

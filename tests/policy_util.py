@@ -133,8 +133,10 @@ def draw(logits, uniforms, temperature=1.0):
 def logprobs(logits, tokens, temperature, grad=None, grad_entropy=None):
     """Values and bounds of the log-probabilities, the entropies and (with gradients) the logits' gradient.
 
-    z = (x - m) / T is off by 4 half steps of itself (difference, 1 / T, product, and T's own rounding when it is no float32
-    number), so an exponential by (4 |z| + 4) of them; a sum over k numbers, in at least 64 parts, by k / 64 + 16."""
+    z = (x - m) / T is off by 5 half steps of itself (difference, 1 / T, its product with log2(e) / 2, that constant, the product
+    of both), so an exponential, the square of an instruction's result within one step, by (5 |z| + 5) of them; a sum over k
+    numbers, in at least 64 parts, by k / 64 + 16.  The sum r of all exponentials but the maximum's own 1 is taken without that
+    1 where it is small; from 1 / 17 on it may be a sum with it, less 1, whose roundings are of 1 + r."""
     x = np64(logits)
     n, k = x.shape
     t = per_row(temperature, n)
@@ -152,9 +154,9 @@ def logprobs(logits, tokens, temperature, grad=None, grad_entropy=None):
         # an exponential below 2^-126 is held in steps of 2^-149 (of e^-101 and less nothing is left: 8.8e-44 of an entropy
         # becomes 0): 2 steps each, times |z| where z multiplies it; |z| above 110 adds less than a step
         grid = 2 * 2.0 ** -149
-        dr = U32 * ((rest * (4 * az + 4)).sum(1, keepdims=True) + depth * r) + k * grid
+        dr = U32 * ((rest * (5 * az + 5)).sum(1, keepdims=True) + depth * np.where(r > 1 / 17, 1 + r, r)) + k * grid
         tz = np.where(live, e * z, 0.0).sum(1, keepdims=True)
-        dt = U32 * ((e * az * (4 * az + 8)).sum(1, keepdims=True) + depth * np.abs(tz)) + grid * (1 + np.minimum(az, 110.0)).sum(1, keepdims=True)
+        dt = U32 * ((e * az * (5 * az + 9)).sum(1, keepdims=True) + depth * np.abs(tz)) + grid * (1 + np.minimum(az, 110.0)).sum(1, keepdims=True)
         entropy = log_total - tz / (1 + r)
         d_log = dr / (1 + r) + 4 * U32 * log_total
         d_entropy = d_log + dt / (1 + r) + np.abs(tz) * dr / (1 + r) ** 2 + 4 * U32 * (log_total + np.abs(tz) / (1 + r))
