@@ -32,48 +32,87 @@ struct __attribute__((packed, aligned(sizeof(T)))) Vec {
     T v[V];
 };
 
-template <class T, int V>
-__device__ __forceinline__ void load(const T *p, float (&x)[V]) {
-    const Vec<T, V> r = *reinterpret_cast<const Vec<T, V> *>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = static_cast<float>(r.v[i]);
-}
-
+// Words, not elements, go to memory: as elements a store and the one of a row's end beside it would be taken apart and merged.
 template <class T, int V>
 __device__ __forceinline__ void store(T *p, const float (&x)[V]) {
+    constexpr int WORDS = V * sizeof(T) / 4;
     Vec<T, V> r;
 #pragma unroll
     for (int i = 0; i < V; ++i) r.v[i] = static_cast<T>(x[i]);
-    *reinterpret_cast<Vec<T, V> *>(p) = r;
+    uint32_t w[WORDS];
+    __builtin_memcpy(w, &r, sizeof r);
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {
+        uint32_t w[WORDS];
+    } q;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+        asm("" : "+v"(w[i]));
+        q.w[i] = w[i];
+    }
+    *reinterpret_cast<Words *>(p) = q;
 }
 
 // elements in 16 bytes
 template <class T>
 constexpr int WIDE = 16 / static_cast<int>(sizeof(T));
 
-// Words of W adjacent elements, which stay packed until they are used; elements from `left` on are `fill` (an element's bits).
+// Words of W adjacent elements at p, which stay packed until they are used.  `left` elements are the row's, the others become
+// `fill` (an element's bits).  A row of at least W elements is never read element by element (each would be waited for): the W
+// elements that end where the row does are read and moved down.
 template <class T, int W>
-__device__ __forceinline__ void load_words(const T *p, int left, uint32_t fill, uint32_t (&w)[(W * sizeof(T) + 3) / 4]) {
-    constexpr int WORDS = (W * sizeof(T) + 3) / 4;
-    if (left >= W) {
-        if constexpr (W * sizeof(T) >= 4) {
-            const Vec<T, W> r = *reinterpret_cast<const Vec<T, W> *>(p);
-            __builtin_memcpy(w, &r, sizeof r);
-        } else {
-            w[0] = __builtin_bit_cast(uint16_t, p[0]);
-        }
+__device__ __forceinline__ void load_words(const T *p, int left, int length, uint32_t fill, uint32_t (&w)[(W * sizeof(T) + 3) / 4]) {
+    constexpr int WORDS = (W * sizeof(T) + 3) / 4, BITS = 8 * sizeof(T);
+    if constexpr (W * sizeof(T) < 4) {
+        w[0] = left > 0 ? *reinterpret_cast<const uint16_t *>(p) : fill;
+        return;
     } else {
+        struct __attribute__((packed, aligned(sizeof(T)))) Words {
+            uint32_t w[WORDS];
+        };
+        const uint32_t fills = BITS == 32 ? fill : fill * 0x10001u;
+        if (left >= W) {
+            const Words r = *reinterpret_cast<const Words *>(p);
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = sizeof(T) == 4 ? fill : (W == 1 ? fill : fill * 0x10001u);
-        if (left > 0)
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (i < left) {
-                    if constexpr (sizeof(T) == 4)
-                        w[i] = __builtin_bit_cast(uint32_t, p[i]);
-                    else
-                        w[i / 2] = (w[i / 2] & (i & 1 ? 0xFFFFu : 0xFFFF0000u)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, p[i])) << (16 * (i & 1));
+            for (int i = 0; i < WORDS; ++i) w[i] = r.w[i];
+        } else if (left > 0 && length >= W) {
+            const Words r = *reinterpret_cast<const Words *>(p - (W - left));
+            const int down = (W - left) * BITS;
+            if constexpr (WORDS == 1) {
+                w[0] = r.w[0] >> 16 | fills << 16;
+            } else {
+                const uint64_t all = static_cast<uint64_t>(fills) << 32 | fills, lo = static_cast<uint64_t>(r.w[1]) << 32 | r.w[0];
+                uint64_t to = 0, top = 0;
+                if constexpr (WORDS == 2) {
+                    to = lo >> down | all << (64 - down);
+                } else {
+                    const uint64_t hi = static_cast<uint64_t>(r.w[3]) << 32 | r.w[2];
+                    if (down < 64) {
+                        to = lo >> down | hi << (64 - down);
+                        top = hi >> down | all << (64 - down);
+                    } else {
+                        to = down == 64 ? hi : hi >> (down - 64) | all << (128 - down);
+                        top = all;
+                    }
+                    w[2] = static_cast<uint32_t>(top);
+                    w[3] = static_cast<uint32_t>(top >> 32);
                 }
+                w[0] = static_cast<uint32_t>(to);
+                w[1] = static_cast<uint32_t>(to >> 32);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = fills;
+            if (left > 0) {
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (i < left) {
+                        if constexpr (BITS == 32)
+                            w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+                        else
+                            w[i / 2] = (w[i / 2] & (i & 1 ? 0xFFFFu : 0xFFFF0000u)) | static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i]) << (16 * (i & 1));
+                    }
+            }
+        }
     }
 }
 
@@ -86,17 +125,53 @@ __device__ __forceinline__ float element(const uint32_t *w, int i) {
         return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)))));
 }
 
+// N vectors of a row, number j at first + (j * lanes + lane) * V; behind the row's k elements `fill`.  Only one thread's vector
+// can hold the row's end in part; it is loaded apart from the others, once.
+template <class T, int N>
+__device__ __forceinline__ void load_vectors(const T *row, int k, int first, int lanes, int lane, uint32_t fill, uint32_t (&w)[N][4]) {
+    constexpr int V = WIDE<T>;
+    const uint32_t fills = sizeof(T) == 4 ? fill : fill * 0x10001u;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int at = first + (j * lanes + lane) * V;
+        if (at + V <= k) {
+            load_words<T, V>(row + at, V, V, fill, w[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[j][i] = fills;
+        }
+    }
+    const int end = k / V * V;
+    if (end < k && end >= first) {
+        const int v = (end - first) / V, j = v >> __builtin_ctz(lanes);  // (a power of two)
+        if (j < N && v - j * lanes == lane) {
+            uint32_t q[4];
+            load_words<T, V>(row + end, k - end, k, fill, q);
+#pragma unroll
+            for (int o = 0; o < N; ++o)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[o][i] = o == j ? q[i] : w[o][i];
+        }
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void load(const T *p, float (&x)[V]) {
+    uint32_t w[V * sizeof(T) / 4];
+    load_words<T, V>(p, V, V, 0, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = element<T>(w, i);
+}
+
 template <class T>
 constexpr uint32_t NEG_INF_BITS = sizeof(T) == 4 ? 0xFF800000u : (__is_same(T, f16) ? 0xFC00u : 0xFF80u);
 
 template <class T, int V>
-__device__ __forceinline__ void load_part(const T *p, int left, float (&x)[V]) {
-    if (left >= V) {
-        load<T, V>(p, x);
-    } else {
+__device__ __forceinline__ void load_part(const T *p, int left, int length, float (&x)[V]) {
+    uint32_t w[V * sizeof(T) / 4];
+    load_words<T, V>(p, left, length, 0, w);
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = i < left ? static_cast<float>(p[i]) : 0.f;
-    }
+    for (int i = 0; i < V; ++i) x[i] = element<T>(w, i);
 }
 
 template <class T, int V>
@@ -132,36 +207,85 @@ __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *id
         T *to = out + n * a.dim;
         for (int c = col; c < vecs; c += cols) {
             const int d0 = c * V;
-            const bool whole = d0 + V <= a.dim;
             float acc[V] = {};
             int64_t base = 0;
             for (int f = 0; f < a.fields; ++f) {
                 const int64_t id = static_cast<int64_t>(id_at[f * a.field_stride]);
                 if (id >= 0 && id < a.sizes[f]) {
-                    const T *row = table + (base + id) * a.row_stride + d0;
-                    if (whole) {
-                        float x[V];
-                        load<T, V>(row, x);
+                    float x[V];
+                    load_part<T, V>(table + (base + id) * a.row_stride + d0, a.dim - d0, a.dim, x);
 #pragma unroll
-                        for (int i = 0; i < V; ++i) acc[i] += x[i];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            if (d0 + i < a.dim) acc[i] += static_cast<float>(row[i]);
-                    }
+                    for (int i = 0; i < V; ++i) acc[i] += x[i];
                 }
                 base += a.sizes[f];
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] *= a.scale;
-            if (whole) {
-                store<T, V>(to + d0, acc);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (d0 + i < a.dim) to[d0 + i] = static_cast<T>(acc[i]);
-            }
+            store_part<T, V>(to + d0, a.dim - d0, acc);
         }
+    }
+}
+
+// A table that LDS holds (cells: 24 rows): a block copies it there once, then takes FAR tokens' ids at a time into LDS as row
+// numbers, and writes those tokens' outputs 16 bytes a thread, four tokens to a thread at once.  Bound by the writes; from memory
+// or L1 each output waited for a chain of id, row and store.
+constexpr int TABLE_BYTES = 32768, FAR = 512, TABLE_BLOCKS = 2048;
+
+template <class T, class I>
+__global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, const I *ids, const T *table, T *out) {
+    constexpr int V = WIDE<T>, TOGETHER = 4;
+    extern __shared__ __align__(16) char lds[];
+    const int vecs = (a.dim + V - 1) / V, pitch = vecs * V;
+    T *table_s = reinterpret_cast<T *>(lds);                                                  // [rows + 1][pitch], zeros in the last row
+    uint16_t *rows_s = reinterpret_cast<uint16_t *>(lds + (a.rows + 1) * pitch * sizeof(T));  // [fields][FAR]
+    for (int i = threadIdx.x; i < (a.rows + 1) * pitch; i += THREADS) {
+        const int r = i / pitch, d = i - r * pitch;
+        table_s[i] = r < a.rows && d < a.dim ? table[r * a.row_stride + d] : static_cast<T>(0.f);
+    }
+    const int cols = min(vecs, THREADS), per_block = THREADS / cols;
+    const int sub = threadIdx.x / cols, col = threadIdx.x - sub * cols;
+    for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * FAR; n0 < a.n; n0 += static_cast<int64_t>(gridDim.x) * FAR) {
+        const int tokens = static_cast<int>(min(static_cast<int64_t>(FAR), a.n - n0));
+        __syncthreads();
+        int base = 0;
+        for (int f = 0; f < a.fields; ++f) {
+            const I *from = ids + n0 * a.ids_stride + f * a.field_stride;
+            I id[FAR / THREADS];
+#pragma unroll
+            for (int j = 0; j < FAR / THREADS; ++j) {
+                const int t = j * THREADS + threadIdx.x;
+                id[j] = t < tokens ? from[t * a.ids_stride] : static_cast<I>(0);
+            }
+#pragma unroll
+            for (int j = 0; j < FAR / THREADS; ++j) {
+                const int64_t v = static_cast<int64_t>(id[j]);
+                rows_s[f * FAR + j * THREADS + threadIdx.x] = static_cast<uint16_t>(v >= 0 && v < a.sizes[f] ? base + v : a.rows);
+            }
+            base += a.sizes[f];
+        }
+        __syncthreads();
+        if (sub < per_block)
+            for (int c = col; c < vecs; c += cols)
+                for (int t0 = sub; t0 < tokens; t0 += per_block * TOGETHER) {
+                    float acc[TOGETHER][V] = {};
+                    for (int f = 0; f < a.fields; ++f)
+#pragma unroll
+                        for (int u = 0; u < TOGETHER; ++u) {
+                            const int t = min(t0 + u * per_block, FAR - 1);
+                            const uint4 q = *reinterpret_cast<const uint4 *>(table_s + rows_s[f * FAR + t] * pitch + c * V);
+                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int i = 0; i < V; ++i) acc[u][i] += element<T>(w, i);
+                        }
+#pragma unroll
+                    for (int u = 0; u < TOGETHER; ++u) {
+                        const int t = t0 + u * per_block;
+                        if (t >= tokens) break;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) acc[u][i] *= a.scale;
+                        store_part<T, V>(out + (n0 + t) * a.dim + c * V, a.dim - c * V, acc[u]);
+                    }
+                }
     }
 }
 
@@ -188,7 +312,7 @@ __device__ __forceinline__ int row_of(const EmbedArgs &a, const void *ids, int i
 //
 // 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
 // again, one after the other, each added to its own rows only.
-constexpr int FEW = 64, FEW_BLOCKS = 1024;
+constexpr int FEW = 64, FEW_BLOCKS = 1024;  // four to a compute unit
 
 template <class T>
 struct Operand {
@@ -217,11 +341,11 @@ union Fragment {
 };
 
 template <class T, int W, int TILES>
-__global__ __launch_bounds__(THREADS) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
+__global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
     constexpr int COLS = 16 * W, WORDS = (W * sizeof(T) + 3) / 4;
     __shared__ __align__(16) uint16_t rows_s[THREADS / 64][MG_MAX_FIELDS][64];  // 0xFFFF: none
     __shared__ float sum_s[TILES * 16][COLS];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, l16 = lane % 16, quad = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, l16 = lane % 16, quad = lane / 16;
     const int d0 = blockIdx.y * COLS, col = l16 * W, left = a.dim - d0 - col;
     // the field that this lane's row of each tile belongs to, and the row twice in a word (a row that is none never matches)
     int field[TILES];
@@ -241,24 +365,46 @@ __global__ __launch_bounds__(THREADS) void embed_grad_few_kernel(EmbedArgs a, co
         for (int i = 0; i < W; ++i) acc[m][i] = float4_t{0.f, 0.f, 0.f, 0.f};
 
     const int64_t step = static_cast<int64_t>(gridDim.x) * THREADS;
-    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64; t0 < a.n; t0 += step) {
-        uint32_t x[2][8][WORDS];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t t = t0 + s * 32 + quad * 8 + j;
-                load_words<T, W>(grad + t * a.row_stride + d0 + col, t < a.n ? left : 0, 0, x[s][j]);
-            }
+    // whole columns and short rows: one offset of the lane's own, everything else is the same for the wave
+    const bool near = a.dim - d0 >= COLS && a.row_stride < (1 << 20);
+    const uint32_t own = (static_cast<uint32_t>(quad) * 8 * static_cast<uint32_t>(a.row_stride) + col) * static_cast<uint32_t>(sizeof(T));
+    auto fetch_rows = [&](int64_t t0, int (&r)[MG_MAX_FIELDS]) {
+        const int64_t t = t0 + lane;
         int base = 0;
-        for (int f = 0; f < a.fields; ++f) {
-            const int64_t t = t0 + lane;
-            rows_s[wave][f][lane] = static_cast<uint16_t>(t < a.n ? row_of(a, ids, ids_type, t, f, base) : -1);
-            base += a.sizes[f];
+#pragma unroll
+        for (int f = 0; f < MG_MAX_FIELDS; ++f)
+            if (f < a.fields) {
+                r[f] = t < a.n ? row_of(a, ids, ids_type, t, f, base) : -1;
+                base += a.sizes[f];
+            }
+    };
+    auto fetch = [&](int64_t t0, uint32_t (&x)[2][8][WORDS]) {
+        if (near && t0 + 64 <= a.n) {
+            const char *from = reinterpret_cast<const char *>(grad + t0 * a.row_stride + d0);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) load_words<T, W>(reinterpret_cast<const T *>(from + (s * 32 + j) * a.row_stride * sizeof(T) + own), W, W, 0, x[s][j]);
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t t = t0 + s * 32 + quad * 8 + j;
+                    load_words<T, W>(grad + t * a.row_stride + d0 + col, t < a.n ? left : 0, a.dim, 0, x[s][j]);
+                }
         }
+    };
+    auto put_rows = [&](const int (&r)[MG_MAX_FIELDS]) {
+        __builtin_amdgcn_wave_barrier();  // the last tokens' rows are read
+#pragma unroll
+        for (int f = 0; f < MG_MAX_FIELDS; ++f)
+            if (f < a.fields) rows_s[wave][f][lane] = static_cast<uint16_t>(r[f]);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto add = [&](uint32_t (&x)[2][8][WORDS]) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             Fragment hot[TILES];
@@ -301,7 +447,34 @@ __global__ __launch_bounds__(THREADS) void embed_grad_few_kernel(EmbedArgs a, co
                 }
             }
         }
-        __builtin_amdgcn_wave_barrier();  // the next tokens' rows come after these reads
+    };
+    // two sets of registers in turn: the next 64 tokens are under way while these are multiplied
+    int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64;
+    if (t0 < a.n) {
+        uint32_t x0[2][8][WORDS], x1[2][8][WORDS];
+        int r[MG_MAX_FIELDS];
+        fetch_rows(t0, r);
+        fetch(t0, x0);
+        while (true) {
+            put_rows(r);
+            const bool more = t0 + step < a.n;
+            if (more) {
+                fetch_rows(t0 + step, r);
+                fetch(t0 + step, x1);
+            }
+            add(x0);
+            if (!more) break;
+            t0 += step;
+            put_rows(r);
+            const bool again = t0 + step < a.n;
+            if (again) {
+                fetch_rows(t0 + step, r);
+                fetch(t0 + step, x0);
+            }
+            add(x1);
+            if (!again) break;
+            t0 += step;
+        }
     }
 
     bool fine = true;
@@ -619,7 +792,7 @@ __global__ __launch_bounds__(THREADS) void embed_runs_kernel(EmbedArgs a, Sorted
             t[j] = e + j < e1 ? s.tokens[e + j] : 0;
         }
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) load_part<T, V>(grad + static_cast<int64_t>(t[j]) * a.row_stride + d0, r[j] == none ? 0 : left, x[j]);
+        for (int j = 0; j < AHEAD; ++j) load_part<T, V>(grad + static_cast<int64_t>(t[j]) * a.row_stride + d0, r[j] == none ? 0 : left, a.dim, x[j]);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             if (e + j >= e1) break;
@@ -685,19 +858,14 @@ __global__ __launch_bounds__(THREADS) void embed_span_kernel(EmbedArgs a, Sorted
 constexpr int SHORT = 32;
 
 template <class T, int K>
-__device__ __forceinline__ void load_row(const T *p, int k, float (&x)[K], float fill) {
+__device__ __forceinline__ void load_row(const T *p, int k, float (&x)[K], uint32_t fill) {
     constexpr int V = WIDE<T>;
 #pragma unroll
     for (int i = 0; i < K; i += V) {
-        if (i + V <= k) {
-            float v[V];
-            load<T, V>(p + i, v);
+        uint32_t w[4];
+        load_words<T, V>(p + i, k - i, k, fill, w);
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[i + j] = v[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[i + j] = i + j < k ? static_cast<float>(p[i + j]) : fill;
-        }
+        for (int j = 0; j < V; ++j) x[i + j] = element<T>(w, j);
     }
 }
 
@@ -721,7 +889,7 @@ __device__ __forceinline__ void store_row(T *p, int k, const float (&x)[K]) {
 
 // ---- longer rows ---------------------------------------------------------------------------------------------------
 
-// LANES threads (8 to 64: several rows to a block of THREADS; 256 or 1024: a block to a row) hold a row of up to
+// LANES threads (8 to 64: several rows to a block of THREADS; 256 and more: a block to a row) hold a row of up to
 // LANES * HELD 16-byte vectors in registers, vector j * LANES + lane with each: one pass over memory, whose loads are all under
 // way at once; the maximum is known before the first exponential.  HELD = 0: rows that no block holds are read again from
 // the cache or memory for each use, 1024 threads to a row.
@@ -737,12 +905,10 @@ struct Row {
 
     __device__ __forceinline__ void fetch(int j, uint32_t (&w)[4]) const {
         const int at = (j * LANES + lane) * V;
-        // all lanes of the row have whole vectors (the same answer for all of them), or this is the last one
-        load_words<T, V>(x + at, (j + 1) * LANES * V <= k ? V : k - at, NEG_INF_BITS<T>, w);
+        load_words<T, V>(x + at, k - at, k, NEG_INF_BITS<T>, w);
     }
     __device__ __forceinline__ Row(const T *row, int tokens, int thread) : x(row), k(tokens), lane(thread), vecs((tokens + LANES * V - 1) / (LANES * V)) {
-#pragma unroll
-        for (int j = 0; j < HELD; ++j) fetch(j, held[j]);
+        if constexpr (HELD > 0) load_vectors<T, HELD>(x, k, 0, LANES, lane, NEG_INF_BITS<T>, held);
     }
     // f(number of the vector, its words) for all of this thread's vectors.  The empty statements keep a pass from sharing its
     // conversions with the next one and the barriers keep the vectors apart: either would take several times the registers.
@@ -758,8 +924,7 @@ struct Row {
         } else {
             for (int j = 0; j < vecs; j += 4) {  // four loads under way; what lies behind the row is -inf
                 uint32_t w[4][4];
-#pragma unroll
-                for (int o = 0; o < 4; ++o) fetch(j + o, w[o]);
+                load_vectors<T, 4>(x, k, j * LANES * V, LANES, lane, NEG_INF_BITS<T>, w);
 #pragma unroll
                 for (int o = 0; o < 4; ++o) f(j + o, w[o]);
             }
@@ -768,13 +933,50 @@ struct Row {
     __device__ __forceinline__ int token(int j, int i) const { return (j * LANES + lane) * V + i; }
 };
 
-// f combined over the threads of a row, known to all of them
+// v of another lane, chosen by a DPP control (a row is 16 lanes): several times quicker than a shuffle through LDS
+template <int CONTROL, class X>
+__device__ __forceinline__ X of_lane(X v) {
+    constexpr int N = sizeof(X) / 4;
+    int w[N];
+    __builtin_memcpy(w, &v, sizeof v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_mov_dpp(w[i], CONTROL, 0xF, 0xF, true);
+    __builtin_memcpy(&v, w, sizeof v);
+    return v;
+}
+template <class X>
+__device__ __forceinline__ X read_lane(X v, int lane) {
+    constexpr int N = sizeof(X) / 4;
+    int w[N];
+    __builtin_memcpy(w, &v, sizeof v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_readlane(w[i], lane);
+    __builtin_memcpy(&v, w, sizeof v);
+    return v;
+}
+
+template <class X>
+__device__ __forceinline__ X other_half(X v) {  // of 32 lanes
+    constexpr int N = sizeof(X) / 4;
+    int w[N];
+    __builtin_memcpy(w, &v, sizeof v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __shfl_xor(w[i], 16, 64);
+    __builtin_memcpy(&v, w, sizeof v);
+    return v;
+}
+
+// f combined over the threads of a row, known to all of them; f is commutative.  `shared` holds one value a wave and is not to be
+// used again before another barrier: callers take a slot of their own for each of a row's combinations.
 template <int LANES, class X, class F>
 __device__ __forceinline__ X over_row(X v, X *shared, F f) {
-#pragma unroll
-    for (int by = (LANES < 64 ? LANES : 64) / 2; by > 0; by /= 2) v = f(v, __shfl_xor(v, by, 64));
+    v = f(v, of_lane<0xB1>(v));                    // the neighbour
+    v = f(v, of_lane<0x4E>(v));                    // the other pair of four
+    v = f(v, of_lane<0x141>(v));                   // mirrored in eight
+    if constexpr (LANES > 8) v = f(v, of_lane<0x140>(v));  // mirrored in sixteen
+    if constexpr (LANES == 32) v = f(v, other_half(v));
+    if constexpr (LANES >= 64) v = f(f(read_lane(v, 0), read_lane(v, 16)), f(read_lane(v, 32), read_lane(v, 48)));
     if constexpr (LANES > 64) {
-        __syncthreads();
         if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = v;
         __syncthreads();
         v = shared[0];
@@ -811,29 +1013,22 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
     constexpr int V = WIDE<T>, PIECE = THREADS * STRETCH * V;
     __shared__ __align__(16) uint32_t counts_s[PIECE];
     const int lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * STRETCH * V;
-    const int pieces = (a.k + width - 1) / width;  // 1 where rows share a block
-    const int64_t items = (a.n + per_block - 1) / per_block * pieces;
+    const int first = blockIdx.y * width;  // 0 where rows share a block
     const bool history = a.history_dev != nullptr && a.t > 0;
     uint32_t *counts = counts_s + sub * width;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t block_row = pieces == 1 ? item : item / pieces;
-        const int first = static_cast<int>(item - block_row * pieces) * width;
-        const int64_t row = block_row * per_block + sub;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * per_block; row0 < a.n; row0 += static_cast<int64_t>(gridDim.x) * per_block) {
+        const int64_t row = row0 + sub;
         const bool live = row < a.n;
-        Vec<T, V> x[STRETCH], g[STRETCH];
-#pragma unroll
-        for (int j = 0; j < STRETCH; ++j) {
-            const int at = first + (j * lanes + lane) * V;
-            if (live && at + V <= a.k) {
-                x[j] = *reinterpret_cast<const Vec<T, V> *>(logits + row * a.logits_stride + at);
-                if (GRAD) g[j] = *reinterpret_cast<const Vec<T, V> *>(grad + row * a.grad_stride + at);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x[j].v[i] = live && at + i < a.k ? logits[row * a.logits_stride + at + i] : static_cast<T>(0.f);
-                    if (GRAD) g[j].v[i] = live && at + i < a.k ? grad[row * a.grad_stride + at + i] : static_cast<T>(0.f);
-                }
-            }
+        uint32_t x[STRETCH][4], g[STRETCH][4];
+        if (live) {
+            load_vectors<T, STRETCH>(logits + row * a.logits_stride, a.k, first, lanes, lane, 0, x);
+            if (GRAD) load_vectors<T, STRETCH>(grad + row * a.grad_stride, a.k, first, lanes, lane, 0, g);
+        }
+        float rep = 1.f, presence = 0.f, frequency = 0.f;
+        if (live) {
+            rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
+            presence = a.presence_dev ? a.presence_dev[row] : a.presence;
+            frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
         }
         if (history) {
             const int len = !live ? 0 : (a.lengths_dev ? min(max(a.lengths_dev[row], 0), a.t) : a.t);
@@ -844,16 +1039,20 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                 for (int i = 0; i < V; i += 4) *reinterpret_cast<uint4 *>(&counts[(j * lanes + lane) * V + i]) = make_uint4(0, 0, 0, 0);
             __syncthreads();
             const int end = min(width, a.k - first);
-            for (int i = lane; i < len; i += lanes) {
-                const int64_t j = static_cast<int64_t>(h[i]) - first;
-                if (j >= 0 && j < end) atomicAdd(&counts[j], 1u);
+            constexpr int AHEAD = 8;
+            for (int i = lane; i < len; i += AHEAD * lanes) {
+                H entry[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) entry[u] = h[min(i + u * lanes, len - 1)];
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int64_t j = static_cast<int64_t>(entry[u]) - first;
+                    if (i + u * lanes < len && j >= 0 && j < end) atomicAdd(&counts[j], 1u);
+                }
             }
             __syncthreads();
         }
         if (live) {
-            const float rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
-            const float presence = a.presence_dev ? a.presence_dev[row] : a.presence;
-            const float frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
 #pragma unroll
             for (int j = 0; j < STRETCH; ++j) {
                 const int at = first + (j * lanes + lane) * V;
@@ -883,10 +1082,10 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                 float y[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    y[i] = static_cast<float>(x[j].v[i]);
+                    y[i] = element<T>(x[j], i);
                     if (GRAD) {
                         const bool up = y[i] > 0.f;
-                        y[i] = static_cast<float>(g[j].v[i]);
+                        y[i] = element<T>(g[j], i);
                         if (c[i] > 0) y[i] = up ? y[i] / rep : y[i] * rep;
                     } else {
                         if (c[i] > 0) y[i] = (y[i] > 0.f ? y[i] / rep : y[i] * rep) - presence;
@@ -895,28 +1094,26 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                 }
                 if (!GRAD && a.bias_dev) {
                     const float *b = a.bias_dev + row * a.bias_stride + at;
-                    if (whole) {
-                        float v[V];
-                        load<float, V>(b, v);
+                    float v[V];
 #pragma unroll
-                        for (int i = 0; i < V; ++i) y[i] = y[i] + v[i];
-                    } else {
+                    for (int i = 0; i < V; i += 4) {
+                        uint32_t q[4];
+                        if (whole) {
+                            load_words<float, 4>(b + i, 4, 4, 0, q);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            if (at + i < a.k) y[i] = y[i] + b[i];
+                            for (int o = 0; o < 4; ++o) q[o] = at + i + o < a.k ? __builtin_bit_cast(uint32_t, b[i + o]) : 0;
+                        }
+#pragma unroll
+                        for (int o = 0; o < 4; ++o) v[i + o] = element<float>(q, o);
                     }
+#pragma unroll
+                    for (int i = 0; i < V; ++i) y[i] = y[i] + v[i];
                 }
 #pragma unroll
                 for (int i = 0; i < V; ++i)
                     if (!((allow >> i) & 1)) y[i] = GRAD ? 0.f : NEG_INF;
-                T *to = out + row * a.out_stride + at;
-                if (whole) {
-                    store<T, V>(to, y);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (at + i < a.k) to[i] = static_cast<T>(y[i]);
-                }
+                store_part<T, V>(out + row * a.out_stride + at, a.k - at, y);
             }
         }
         if (history) __syncthreads();  // the counters are read
@@ -935,8 +1132,8 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
     if (row >= a.n) return;
     const bool history = a.history_dev != nullptr && a.t > 0;
     float x[K], g[K];
-    load_row<T, K>(logits + row * a.logits_stride, a.k, x, 0.f);
-    if (GRAD) load_row<T, K>(grad + row * a.grad_stride, a.k, g, 0.f);
+    load_row<T, K>(logits + row * a.logits_stride, a.k, x, 0);
+    if (GRAD) load_row<T, K>(grad + row * a.grad_stride, a.k, g, 0);
     uint32_t allow = ~0u;
     if (a.mask_kind == MG_MASK_BYTES) {
         const uint8_t *m = static_cast<const uint8_t *>(a.mask_dev) + row * a.mask_stride;
@@ -1008,10 +1205,10 @@ __device__ __forceinline__ int64_t get_token(const void *tokens, int type, int64
 // roundings; a square of something off by 2^-23), a vector's sum by 8 more, and sum p |z| / sum p <= ln k (an entropy), so a sum
 // of them and the border are off by at most (5 ln k + 13) 2^-24 of the total each.  Where the border comes nearer to either end of the token found than
 // one and a half times both, the row is done again with 64-bit exponentials, at ten times the instructions.
-struct DrawShared {
-    double sums[16 * 16], reduce[16], before;
-    float reduce_f[16];
-    int reduce_i[16], place;
+struct DrawShared {  // a slot for each of a row's combinations
+    double sums[16 * 16], total[16], again[16], step[16], before, behind;
+    float most[16];
+    int last[16], place;
 };
 
 template <class T, int LANES, int HELD>
@@ -1122,13 +1319,13 @@ struct Draw {
                 at_wave = found % WAVES;
             }
         } else if constexpr (HELD > 0) {
-            total = over_row<LANES>(mine, s.reduce, sum_of<double>);
+            total = over_row<LANES>(mine, EXACT ? s.again : s.total, sum_of<double>);
             if (!draws) return -1;
             border = u * total;
             double sum = 0.0;
 #pragma unroll
             for (int j = 0; j < VECS; ++j) {
-                const double all = VECS == 1 ? total : over_row<LANES>(part[j], s.reduce, sum_of<double>);
+                const double all = VECS == 1 ? total : over_row<LANES>(part[j], s.step, sum_of<double>);
                 if (vec < 0 && sum + all > border) {
                     vec = j;
                     before = sum;
@@ -1137,7 +1334,7 @@ struct Draw {
             }
         } else {
             // one vector of every thread after another: the waves' sums, the border
-            total = over_row<LANES>(mine, s.reduce, sum_of<double>);
+            total = over_row<LANES>(mine, EXACT ? s.again : s.total, sum_of<double>);
             if (!draws) return -1;
             border = u * total;
             double sum = 0.0;
@@ -1150,12 +1347,12 @@ struct Draw {
                 for (int by = SPAN / 2; by > 0; by /= 2) all += __shfl_xor(all, by, 64);
                 if constexpr (WAVES > 1) {
                     __syncthreads();
-                    if (lane == 0) s.reduce[wave] = all;
+                    if (lane == 0) s.step[wave] = all;
                     __syncthreads();
                 }
 #pragma unroll 1
                 for (int w = 0; w < WAVES; ++w) {
-                    const double of_wave = WAVES > 1 ? s.reduce[w] : all;
+                    const double of_wave = WAVES > 1 ? s.step[w] : all;
                     if (!done && sum + of_wave > border) {
                         done = true;
                         vec = j;
@@ -1207,12 +1404,12 @@ struct Draw {
             if (vec >= 0 && lane == 0) {
                 s.place = token;
                 s.before = before;
-                s.reduce[0] = behind;
+                s.behind = behind;
             }
             __syncthreads();
             token = s.place;
             before = s.before;
-            behind = s.reduce[0];
+            behind = s.behind;
         }
         return token;
     }
@@ -1232,7 +1429,7 @@ __global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T 
 #pragma unroll
             for (int e = 0; e < D::V; ++e) m = larger(m, element<T>(v, e));
         });
-        m = over_row<LANES>(m, s.reduce_f, larger);
+        m = over_row<LANES>(m, s.most, larger);
         int token = -1;
         double total = 0.0, before = 0.0, behind = 0.0;
         if (fabsf(m) < -NEG_INF) {
@@ -1252,7 +1449,8 @@ __global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T 
 #pragma unroll
                     for (int e = 0; e < D::V; ++e) sum += exp_twice((element<T>(v, e) - m) * c);
                 });
-                total = over_row<LANES>(sum, s.reduce, sum_of<double>);
+                if constexpr (D::WAVES > 1) __syncthreads();
+                total = over_row<LANES>(sum, s.step, sum_of<double>);
             }
             if (token < 0) {  // the largest, the lowest of equal ones; for a draw: no sum passed the border, the last that has any
                 const bool last = uniforms != nullptr;
@@ -1267,7 +1465,7 @@ __global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T 
                         if (last ? exp((static_cast<double>(x) - m) * inv_t) > 0.0 : x == m) found = last ? max(found, row.token(j, e)) : min(found, row.token(j, e));
                     }
                 }
-                token = over_row<LANES>(found, s.reduce_i, [last](int a, int b) { return last ? max(a, b) : min(a, b); });
+                token = over_row<LANES>(found, s.last, [last](int a, int b) { return last ? max(a, b) : min(a, b); });
             }
         }
         if (lane == 0) {
@@ -1276,6 +1474,7 @@ __global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T 
                 logprob[i] = token < 0 ? (m == NEG_INF ? NEG_INF : __builtin_nanf(""))
                                        : static_cast<float>((static_cast<double>(static_cast<float>(logits[i * l.stride + token])) - m) * inv_t - log(total));
         }
+        if (D::WAVES > 1 && i + static_cast<int64_t>(gridDim.x) * ROWS < l.n) __syncthreads();  // the slots are read
     }
 }
 
@@ -1286,7 +1485,7 @@ __global__ __launch_bounds__(THREADS) void draw_short_kernel(MgLogits l, const T
     const int64_t row = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
     if (row >= l.n) return;
     float x[K];
-    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF);
+    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF_BITS<T>);
     const double inv_t = 1.0 / static_cast<double>(l.temperature_dev ? l.temperature_dev[row] : l.temperature);
     float best = x[0];
     int arg = 0;
@@ -1355,17 +1554,26 @@ __device__ __forceinline__ float4 row_stats(const Soft &s) {
     return make_float4(empty ? NEG_INF : (s.r == s.r ? s.m : s.r), log_total, empty ? 0.f : log_total - s.t / (1.f + s.r), 0.f);
 }
 
-// What a finished row gives.
+// The token whose log-probability is wanted and its logit, read before anything is waited for; -1: none.
+struct Taken {
+    int64_t token;
+    float x;
+};
 template <class T>
-__device__ __forceinline__ void row_result(const MgLogits &l, const T *x, int64_t row, const Soft &s, float inv_t, const void *tokens,
-                                           float *logprob, float *entropy, float *stats) {
-    const float4 st = row_stats(s);
-    if (logprob) {
-        const int64_t token = get_token(tokens, l.tokens_type, row);
-        float lp = 0.f;
-        if (token >= 0 && token < l.k) lp = st.x == NEG_INF ? NEG_INF : (static_cast<float>(x[token]) - s.m) * inv_t - st.y;
-        logprob[row] = lp;
+__device__ __forceinline__ Taken taken(const MgLogits &l, const T *x, int64_t row, const void *tokens, bool wanted) {
+    Taken t{-1, 0.f};
+    if (wanted) {
+        t.token = get_token(tokens, l.tokens_type, row);
+        if (t.token >= l.k) t.token = -1;
+        if (t.token >= 0) t.x = static_cast<float>(x[t.token]);
     }
+    return t;
+}
+
+// What a finished row gives.
+__device__ __forceinline__ void row_result(int64_t row, const Soft &s, float inv_t, const Taken &t, float *logprob, float *entropy, float *stats) {
+    const float4 st = row_stats(s);
+    if (logprob) logprob[row] = t.token < 0 ? 0.f : (st.x == NEG_INF ? NEG_INF : (t.x - s.m) * inv_t - st.y);
     if (entropy) entropy[row] = st.z;
     if (stats) reinterpret_cast<float4 *>(stats)[row] = st;
 }
@@ -1373,51 +1581,53 @@ __device__ __forceinline__ void row_result(const MgLogits &l, const T *x, int64_
 template <class T, int LANES, int HELD>
 __global__ __launch_bounds__(BLOCK<LANES>) void logprob_kernel(MgLogits l, const T *logits, const void *tokens, float *logprob, float *entropy, float *stats) {
     constexpr int ROWS = BLOCK<LANES> / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
-    __shared__ float shared[WAVES];
+    __shared__ float most_s[WAVES];
+    __shared__ float2 sums_s[WAVES], rest_s[WAVES];
+    const auto both = [](float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); };
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += static_cast<int64_t>(gridDim.x) * ROWS) {
         Row<T, LANES, HELD> row(logits + i * l.stride, l.k, lane);
         constexpr int V = WIDE<T>;
+        const Taken t = taken(l, logits + i * l.stride, i, tokens, logprob != nullptr);
         const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature), c = inv_t * HALF_LOG2E;
         Soft s{NEG_INF, -1.f, 0.f};
         row.each([&](int, const uint32_t *v) {
 #pragma unroll
             for (int e = 0; e < V; ++e) s.m = larger(s.m, element<T>(v, e));
         });
-        s.m = over_row<LANES>(s.m, shared, larger);
+        s.m = over_row<LANES>(s.m, most_s, larger);
         if (s.m > NEG_INF && s.m < -NEG_INF) {
-            float sum = 0.f, t = 0.f;
+            float sum = 0.f, slant = 0.f;
             row.each([&](int, const uint32_t *v) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float z = fmaxf((element<T>(v, e) - s.m) * c, DEEP), p = exp_twice(z);
                     sum += p;
-                    t = fmaf(p, z, t);
+                    slant = fmaf(p, z, slant);
                 }
             });
-            asm volatile("" : "+v"(sum), "+v"(t));  // t now, not where it is used: every p and z would wait for it
-            sum = over_row<LANES>(sum, shared, sum_of<float>);
-            s.t = over_row<LANES>(t, shared, sum_of<float>) * TWICE_LN2;
-            s.r = sum - 1.f;
-            if (sum < 1.0625f) {  // little beside the maximum: the sum again without it
-                float rest = 0.f;
-                int equal = 0;
+            asm volatile("" : "+v"(sum), "+v"(slant));  // now, not where it is used: every p and z would wait for it
+            const float2 sums = over_row<LANES>(make_float2(sum, slant), sums_s, both);
+            s.t = sums.y * TWICE_LN2;
+            s.r = sums.x - 1.f;
+            if (sums.x < 1.0625f) {  // little beside the maximum: the sum again without it, and how often it stands there
+                float rest = 0.f, equal = 0.f;
                 row.each([&](int, const uint32_t *v) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         const float x = element<T>(v, e);
-                        equal += x == s.m;
-                        rest += x == s.m ? 0.f : exp_twice(fmaxf((x - s.m) * c, DEEP));
+                        equal += x == s.m ? 1.f : 0.f;
+                        rest += x == s.m ? 0.f : exp_twice((x - s.m) * c);
                     }
                 });
-                s.r = over_row<LANES>(rest + static_cast<float>(equal), shared, sum_of<float>);
-                if (over_row<LANES>(equal, reinterpret_cast<int *>(shared), sum_of<int>) == 1) s.r = over_row<LANES>(rest, shared, sum_of<float>);
-                else s.r -= 1.f;
+                const float2 r = over_row<LANES>(make_float2(rest, equal), rest_s, both);
+                s.r = r.x + (r.y - 1.f);
             }
         } else if (s.m != NEG_INF) {
             s.r = __builtin_nanf("");
         }
-        if (lane == 0) row_result(l, logits + i * l.stride, i, s, inv_t, tokens, logprob, entropy, stats);
+        if (lane == 0) row_result(i, s, inv_t, t, logprob, entropy, stats);
+        if (WAVES > 1 && i + static_cast<int64_t>(gridDim.x) * ROWS < l.n) __syncthreads();  // the slots are read
     }
 }
 
@@ -1435,28 +1645,30 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int l
                                                                const float *grad_lp, int64_t lp_stride, const float *grad_h, int64_t h_stride, T *out) {
     constexpr int V = WIDE<T>, TAKES = 4;
     const int lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * TAKES * V;
-    const int pieces = (l.k + width - 1) / width;
-    const int64_t items = (l.n + per_block - 1) / per_block * pieces;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t block_row = pieces == 1 ? item : item / pieces;
-        const int first = static_cast<int>(item - block_row * pieces) * width;
-        const int64_t row = block_row * per_block + sub;
-        if (row >= l.n) continue;
+    const int first = blockIdx.y * width;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * per_block + sub; row < l.n; row += static_cast<int64_t>(gridDim.x) * per_block) {
         const T *x = logits + row * l.stride;
         T *to = out + row * l.k;
-        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
+        uint32_t w[TAKES][4];
+        load_vectors<T, TAKES>(x, l.k, first, lanes, lane, NEG_INF_BITS<T>, w);
+        // (none of these waits for another)
+        const float temperature = l.temperature_dev ? l.temperature_dev[row] : l.temperature;
         const float4 st = reinterpret_cast<const float4 *>(stats)[row];
         const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
-        const float g = token >= 0 && token < l.k ? grad_lp[row * lp_stride] * inv_t : 0.f;
-        const float h = grad_h ? grad_h[row * h_stride] * inv_t : 0.f;
+        const float grad_of_lp = grad_lp ? grad_lp[row * lp_stride] : 0.f, grad_of_h = grad_h ? grad_h[row * h_stride] : 0.f;
+        const float inv_t = 1.f / temperature, g = token >= 0 && token < l.k ? grad_of_lp * inv_t : 0.f, h = grad_of_h * inv_t;
+        // what a p of 0 must not hide: NaN where the row has one
+        const float whole = fmaf(h, st.z, g);
 #pragma unroll
         for (int j = 0; j < TAKES; ++j) {
             const int at = first + (j * lanes + lane) * V;
             if (at >= l.k) break;
             float v[V];
-            load_part<T, V>(x + at, l.k - at, v);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = logprob_slope(v[i], false, st, inv_t, g, h);
+            for (int i = 0; i < V; ++i) {
+                const float lp = fmaxf((element<T>(w[j], i) - st.x) * inv_t - st.y, 2.f * DEEP), p = exp_twice(lp * HALF_LOG2E);
+                v[i] = -p * fmaf(h, lp, whole);
+            }
             if (token >= at && token < at + V) {
                 const float own = logprob_slope(static_cast<float>(x[token]), true, st, inv_t, g, h);
 #pragma unroll
@@ -1497,9 +1709,10 @@ __global__ __launch_bounds__(THREADS) void logprob_short_kernel(MgLogits l, cons
     const int64_t row = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
     if (row >= l.n) return;
     float x[K];
-    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF);
+    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF_BITS<T>);
+    const Taken t = taken(l, logits + row * l.stride, row, tokens, logprob != nullptr);
     const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
-    row_result(l, logits + row * l.stride, row, soft_short<K>(x, l.k, inv_t), inv_t, tokens, logprob, entropy, stats);
+    row_result(row, soft_short<K>(x, l.k, inv_t), inv_t, t, logprob, entropy, stats);
 }
 
 template <class T, int K>
@@ -1508,12 +1721,12 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_short_kernel(MgLogits l,
     const int64_t row = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
     if (row >= l.n) return;
     float x[K];
-    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF);
-    const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
-    const float4 st = row_stats(soft_short<K>(x, l.k, inv_t));
+    load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF_BITS<T>);
+    const float temperature = l.temperature_dev ? l.temperature_dev[row] : l.temperature;
     const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
-    const float g = token >= 0 && token < l.k ? grad_lp[row * lp_stride] * inv_t : 0.f;
-    const float h = grad_h ? grad_h[row * h_stride] * inv_t : 0.f;
+    const float grad_of_lp = grad_lp ? grad_lp[row * lp_stride] : 0.f, grad_of_h = grad_h ? grad_h[row * h_stride] : 0.f;
+    const float inv_t = 1.f / temperature, g = token >= 0 && token < l.k ? grad_of_lp * inv_t : 0.f, h = grad_of_h * inv_t;
+    const float4 st = row_stats(soft_short<K>(x, l.k, inv_t));
 #pragma unroll
     for (int j = 0; j < K; ++j)
         if (j < l.k) x[j] = logprob_slope(x[j], j == token, st, inv_t, g, h);
@@ -1607,11 +1820,12 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
     };
     p.few = a.rows <= FEW;
     if (p.few) {
-        p.width = wide;  // the narrowest that holds a token's columns at once, or 16 bytes
+        p.width = wide / 2;  // the narrowest that holds a token's columns at once, or 8 bytes: two sets of 16 loads are held
         while (p.width > 1 && 16 * (p.width / 2) >= a.dim) p.width /= 2;
         p.tiles = a.rows <= 16 ? 1 : (a.rows <= 32 ? 2 : 4);
         const int64_t blocks = (a.n + THREADS - 1) / THREADS;
-        p.blocks = static_cast<int>(blocks < 1 ? 1 : (blocks < FEW_BLOCKS ? blocks : FEW_BLOCKS));
+        const int64_t slabs = (a.dim + 16 * p.width - 1) / (16 * p.width), most = slabs < FEW_BLOCKS / 64 ? FEW_BLOCKS / slabs : 64;
+        p.blocks = static_cast<int>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
         if (p.blocks > 1) take(static_cast<int64_t>(p.blocks) * a.rows * a.dim * 4);
         return p;
     }
@@ -1666,10 +1880,8 @@ void launch_grad(const EmbedArgs &a, GradPlan p, const void *ids, int ids_type, 
             launch_few<T, 1>(a, p, ids, ids_type, grad, out, parts, stream);
         else if (p.width == 2)
             launch_few<T, 2>(a, p, ids, ids_type, grad, out, parts, stream);
-        else if (p.width == 4)
-            launch_few<T, 4>(a, p, ids, ids_type, grad, out, parts, stream);
         else if constexpr (sizeof(T) == 2)
-            launch_few<T, 8>(a, p, ids, ids_type, grad, out, parts, stream);
+            launch_few<T, 4>(a, p, ids, ids_type, grad, out, parts, stream);
         if (parts) {
             const int64_t elements = static_cast<int64_t>(a.rows) * a.dim;
             hipLaunchKernelGGL((embed_join_kernel<T>), dim3((elements + JOIN_COLS - 1) / JOIN_COLS), dim3(JOIN_COLS * JOIN_SHARES), 0, stream, parts, p.blocks,
@@ -1724,7 +1936,7 @@ void with_size(int k, F f) {
 }
 
 // f(threads to a row, vectors that each holds): the fewest threads that hold a row of `vecs` vectors with one each, a wave up to
-// four each, then blocks of 256 and of 1024 for as many as their registers take beside what f's kernel needs
+// four each, then blocks of 256, 512 and 1024 for as many as their registers take beside what f's kernel needs
 template <int LANES, int HELD>
 struct Shape {
     static constexpr int lanes = LANES, held = HELD;
@@ -1750,7 +1962,7 @@ void with_shape(int64_t vecs, F f) {
     else if (vecs <= 2048)
         f(Shape<256, 8>{});
     else if (vecs <= 4096)
-        f(Shape<256, 16>{});
+        f(Shape<512, 8>{});
     else if (WIDEST >= 8 && vecs <= 8192)
         f(Shape<1024, WIDEST < 8 ? WIDEST : 8>{});
     else if (WIDEST >= 16 && vecs <= 16384)
@@ -1793,7 +2005,7 @@ void launch_adjust(const MgAdjust &a, const void *logits, const void *grad, void
             int lanes = 8;  // the fewest that take a row at once
             while (lanes < THREADS && lanes * TAKES < a.k) lanes *= 2;
             const int64_t per_block = THREADS / lanes, pieces = (a.k + lanes * TAKES - 1) / (lanes * TAKES);
-            hipLaunchKernelGGL((adjust_kernel<T, H, GRAD>), dim3(blocks_for((a.n + per_block - 1) / per_block * pieces)), dim3(THREADS), 0, stream, a, lanes, x, g, y);
+            hipLaunchKernelGGL((adjust_kernel<T, H, GRAD>), dim3(blocks_for((a.n + per_block - 1) / per_block), pieces), dim3(THREADS), 0, stream, a, lanes, x, g, y);
         }
     });
 }
@@ -1824,6 +2036,13 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
         using T = decltype(t);
         using I = decltype(i);
         const int vecs = (a.dim + WIDE<T> - 1) / WIDE<T>, per_block = THREADS / (vecs < THREADS ? vecs : THREADS);
+        const int64_t held = static_cast<int64_t>(a.rows + 1) * vecs * 16;
+        // worth its copy from a few blocks' tokens on
+        if (held <= TABLE_BYTES && a.n >= 4 * FAR) {
+            hipLaunchKernelGGL((embed_table_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, TABLE_BLOCKS)), dim3(THREADS), held + a.fields * FAR * 2,
+                               static_cast<hipStream_t>(stream), a, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
+            return;
+        }
         hipLaunchKernelGGL((embed_kernel<T, I>), dim3(blocks_for((a.n + per_block - 1) / per_block)), dim3(THREADS), 0,
                            static_cast<hipStream_t>(stream), a, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev),
                            static_cast<T *>(out_dev));
@@ -1943,7 +2162,7 @@ int mg_token_logprobs_grad(const MgLogits *l, const void *logits_dev, const void
         int lanes = 8;
         while (lanes < THREADS && lanes * TAKES < l->k) lanes *= 2;
         const int64_t per_block = THREADS / lanes, pieces = (l->k + lanes * TAKES - 1) / (lanes * TAKES);
-        hipLaunchKernelGGL((logprob_grad_kernel<T>), dim3(blocks_for((l->n + per_block - 1) / per_block * pieces)), dim3(THREADS), 0,
+        hipLaunchKernelGGL((logprob_grad_kernel<T>), dim3(blocks_for((l->n + per_block - 1) / per_block), pieces), dim3(THREADS), 0,
                            static_cast<hipStream_t>(stream), *l, lanes, static_cast<const T *>(logits_dev), tokens_dev, stats_dev, grad_logprob_dev,
                            grad_logprob_stride, grad_entropy_dev, grad_entropy_stride, static_cast<T *>(out_dev));
     });
