@@ -889,46 +889,42 @@ __device__ __forceinline__ void store_row(T *p, int k, const float (&x)[K]) {
 
 // ---- longer rows ---------------------------------------------------------------------------------------------------
 
-// LANES threads (8 to 64: several rows to a block of THREADS; 256 and more: a block to a row) hold a row of up to
-// LANES * HELD 16-byte vectors in registers, vector j * LANES + lane with each: one pass over memory, whose loads are all under
-// way at once; the maximum is known before the first exponential.  HELD = 0: rows that no block holds are read again from
-// the cache or memory for each use, 1024 threads to a row.
+// LANES threads (8 to 64: several rows to a block of THREADS; 256 and 512: a block to a row) hold a row of up to LANES * HELD
+// 16-byte vectors in registers, vector j * LANES + lane with each: one pass over memory, whose loads are all under way at
+// once; the maximum is known before the first exponential.  A row that no block holds is cut into pieces of
+// PIECE_LANES * PIECE_HELD vectors, each taken as a row, and a second kernel joins what they give: many blocks to a row also
+// where there are few rows.
 template <int LANES>
 constexpr int BLOCK = LANES > THREADS ? LANES : THREADS;
+constexpr int HELD_MOST = 4096, PIECE_LANES = 256, PIECE_HELD = 4;  // vectors of a row in one piece; a piece
+template <class T>
+constexpr int PIECE = PIECE_LANES * PIECE_HELD * WIDE<T>;  // tokens
 
 template <class T, int LANES, int HELD>
 struct Row {
     static constexpr int V = WIDE<T>;
     const T *x;
-    int k, lane, vecs;
-    uint32_t held[HELD ? HELD : 1][4];
+    int k, lane;
+    uint32_t held[HELD][4];
 
-    __device__ __forceinline__ void fetch(int j, uint32_t (&w)[4]) const {
-        const int at = (j * LANES + lane) * V;
-        load_words<T, V>(x + at, k - at, k, NEG_INF_BITS<T>, w);
-    }
-    __device__ __forceinline__ Row(const T *row, int tokens, int thread) : x(row), k(tokens), lane(thread), vecs((tokens + LANES * V - 1) / (LANES * V)) {
-        if constexpr (HELD > 0) load_vectors<T, HELD>(x, k, 0, LANES, lane, NEG_INF_BITS<T>, held);
+    __device__ __forceinline__ Row(const T *row, int tokens, int thread) : x(row), k(tokens), lane(thread) {
+        load_vectors<T, HELD>(x, k, 0, LANES, lane, NEG_INF_BITS<T>, held);
     }
     // f(number of the vector, its words) for all of this thread's vectors.  The empty statements keep a pass from sharing its
     // conversions with the next one and the barriers keep the vectors apart: either would take several times the registers.
     template <class F>
     __device__ __forceinline__ void each(F f) {
-        if constexpr (HELD > 0) {
 #pragma unroll
-            for (int j = 0; j < HELD; ++j) {
-                asm volatile("" : "+v"(held[j][0]), "+v"(held[j][1]), "+v"(held[j][2]), "+v"(held[j][3]));
-                f(j, held[j]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        } else {
-            for (int j = 0; j < vecs; j += 4) {  // four loads under way; what lies behind the row is -inf
-                uint32_t w[4][4];
-                load_vectors<T, 4>(x, k, j * LANES * V, LANES, lane, NEG_INF_BITS<T>, w);
-#pragma unroll
-                for (int o = 0; o < 4; ++o) f(j + o, w[o]);
-            }
+        for (int j = 0; j < HELD; ++j) {
+            asm volatile("" : "+v"(held[j][0]), "+v"(held[j][1]), "+v"(held[j][2]), "+v"(held[j][3]));
+            f(j, held[j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+    }
+    // vector j again, from the cache: an index into registers would cost more
+    __device__ __forceinline__ void fetch(int j, uint32_t (&w)[4]) const {
+        const int at = token(j, 0);
+        load_words<T, V>(x + at, k - at, k, NEG_INF_BITS<T>, w);
     }
     __device__ __forceinline__ int token(int j, int i) const { return (j * LANES + lane) * V + i; }
 };
@@ -1200,281 +1196,353 @@ __device__ __forceinline__ int64_t get_token(const void *tokens, int type, int64
     return static_cast<const int64_t *>(tokens)[row];
 }
 
-// The draw from a row: total of the probabilities, then the vector, the thread and the token at whose sum the border lies.  All
-// sums are in 64 bits.  The exponentials first are 32-bit ones, each off by at most (5 |z| + 5) 2^-24 of itself (z: five
-// roundings; a square of something off by 2^-23), a vector's sum by 8 more, and sum p |z| / sum p <= ln k (an entropy), so a sum
-// of them and the border are off by at most (5 ln k + 13) 2^-24 of the total each.  Where the border comes nearer to either end of the token found than
-// one and a half times both, the row is done again with 64-bit exponentials, at ten times the instructions.
-struct DrawShared {  // a slot for each of a row's combinations
-    double sums[16 * 16], total[16], again[16], step[16], before, behind;
-    float most[16];
-    int last[16], place;
+// 2^t in 64 bits for t <= 0: the nearest whole number to the exponent, the rest, at most 1/2, through the polynomial of degree
+// ten that meets 2^f at the Chebyshev points of that interval (3e-16 off; 1 at 0).  Half the instructions of a library
+// exponential, which also has to deal with what does not come here.
+__device__ __forceinline__ double exp2_64(double t) {
+    t = fmax(t, -1100.0);  // nothing is left there, and -inf has no rest
+    const double n = rint(t), f = t - n;
+    double p = 7.072585949269224e-09;
+    p = fma(p, f, 1.0208690299958306e-07);
+    p = fma(p, f, 1.321544258792169e-06);
+    p = fma(p, f, 1.5252657260200837e-05);
+    p = fma(p, f, 0.0001540353044173605);
+    p = fma(p, f, 0.0013333558230164974);
+    p = fma(p, f, 0.009618129107606888);
+    p = fma(p, f, 0.05550410866444772);
+    p = fma(p, f, 0.24022650695910097);
+    p = fma(p, f, 0.69314718055995);
+    p = fma(p, f, 1.0);
+    return ldexp(p, static_cast<int>(n));
+}
+
+// A row as a distribution: its largest logit and log2(e) / temperature.
+struct Spread {
+    double m, c;
+    __device__ __forceinline__ double p(float x) const { return exp2_64((static_cast<double>(x) - m) * c); }
+    template <class T>
+    __device__ __forceinline__ double of_vector(const uint32_t *v) const {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < WIDE<T>; ++i) sum += p(element<T>(v, i));
+        return sum;
+    }
+};
+__device__ __forceinline__ Spread spread(const MgLogits &l, int64_t row, float m) {
+    return Spread{m, 1.4426950408889634 / static_cast<double>(l.temperature_dev ? l.temperature_dev[row] : l.temperature)};
+}
+
+__device__ __forceinline__ double uniform_at(const void *uniforms, int type, int64_t row) {
+    return type == MG_F64 ? static_cast<const double *>(uniforms)[row] : static_cast<double>(static_cast<const float *>(uniforms)[row]);
+}
+
+// log p of a token from its logit; total - 1 is exact where little stands beside the maximum
+__device__ __forceinline__ float drawn_logprob(float x, const Spread &s, double total) {
+    return static_cast<float>((static_cast<double>(x) - s.m) * s.c * 0.6931471805599453 - log1pf(static_cast<float>(total - 1.0)));
+}
+
+struct DrawShared {
+    double sums[HELD_MOST / 64], total[8];
+    float most[8];
+    int token;
 };
 
+// The token of a row (or of a piece of one) at whose sum of probabilities the border lies, known to all of its threads, and
+// the total.  `share`: the border is that share of the total; otherwise `border` is it, `before` what stands before the row.
 template <class T, int LANES, int HELD>
-struct Draw {
-    using R = Row<T, LANES, HELD>;
-    static constexpr int V = R::V, WAVES = LANES > 64 ? LANES / 64 : 1, VECS = HELD ? HELD : 1;
-
-    template <bool EXACT>
-    static __device__ __forceinline__ double p(float x, float m, float c, double inv_t) {
-        if constexpr (EXACT)
-            return exp((static_cast<double>(x) - m) * inv_t);
-        else
-            return exp_twice((x - m) * c);
-    }
-
-    // a vector's sum; of 32-bit exponentials in 32 bits
-    template <bool EXACT>
-    static __device__ __forceinline__ double sum_of_vector(const uint32_t *v, float m, float c, double inv_t) {
-        if constexpr (EXACT) {
-            double sum = 0.0;
+__device__ __forceinline__ int find_border(Row<T, LANES, HELD> &row, DrawShared &sh, const Spread &s, bool share, double border, double before, double &total) {
+    constexpr int V = WIDE<T>, SPAN = LANES < 64 ? LANES : 64, WAVES = LANES > 64 ? LANES / 64 : 1;
+    const int wave = LANES > 64 ? threadIdx.x / 64 : 0, lane = row.lane % 64;
+    double part[HELD];
+    row.each([&](int j, const uint32_t *v) { part[j] = s.of_vector<T>(v); });
+    // inclusive sums over the threads of a wave (or of a shorter row)
+    auto upto = [&](double v) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum += p<true>(element<T>(v, i), m, c, inv_t);
-            return sum;
-        } else {
-            float sum = 0.f;
+        for (int by = 1; by < SPAN; by *= 2) {
+            const double o = __shfl_up(v, by, SPAN);
+            if ((lane & (SPAN - 1)) >= by) v += o;
+        }
+        return v;
+    };
+    int vec = -1, at_wave = 0;  // where the border lies
+    if constexpr (WAVES > 1) {
+        // the waves' sums of each vector: every exchange halves the vectors that a thread adds up
+        int of = 0;
+#pragma unroll
+        for (int half = HELD / 2, by = 32; half > 0; half /= 2, by /= 2) {
+            const bool upper = lane & by;
+            of += upper ? half : 0;
+#pragma unroll
+            for (int j = 0; j < half; ++j) {
+                const double give = upper ? part[j] : part[j + half], keep = upper ? part[j + half] : part[j];
+                part[j] = keep + __shfl_xor(give, by, 64);
+            }
+        }
+#pragma unroll
+        for (int by = 32 / HELD; by > 0; by /= 2) part[0] += __shfl_xor(part[0], by, 64);
+        if (lane % (64 / HELD) == 0) sh.sums[of * WAVES + wave] = part[0];
+        __syncthreads();
+        // in the order of the tokens: vectors, then waves; every wave does this by itself
+        constexpr int N = HELD * WAVES, EACH = (N + 63) / 64;
+        double own[EACH], run = 0.0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            own[i] = lane * EACH + i < N ? sh.sums[lane * EACH + i] : 0.0;
+            run += own[i];
+        }
+        const double end = upto(run);
+        total = read_lane(end, 63);
+        if (share) border *= total;
+        double sum = before + (lane ? end - run : 0.0), start = 0.0;
+        int found = N;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            if (found == N && sum + own[i] > border && lane * EACH + i < N) {
+                found = lane * EACH + i;
+                start = sum;
+            }
+            sum += own[i];
+        }
+        const uint64_t any = __ballot(found < N);
+        if (any) {
+            const int from = __builtin_ctzll(any);
+            found = __shfl(found, from, 64);
+            before = __shfl(start, from, 64);
+            vec = found / WAVES;
+            at_wave = found % WAVES;
+        }
+    } else {
+        double sums[HELD];
+        total = 0.0;
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) {
+            sums[j] = over_row<LANES>(part[j], sh.total, sum_of<double>);
+            total += sums[j];
+        }
+        if (share) border *= total;
+        double sum = before;
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) {
+            if (vec < 0 && sum + sums[j] > border) {
+                vec = j;
+                before = sum;
+            }
+            sum += sums[j];
+        }
+    }
+    // the thread, then the token
+    int token = -1;
+    if (vec >= 0 && wave == at_wave) {
+        uint32_t v[4];
+        row.fetch(vec, v);
+        const double here = s.of_vector<T>(v), end = before + upto(here);
+        const int shift = (threadIdx.x % 64) / SPAN * SPAN;
+        const uint64_t threads = (~0ull >> (64 - SPAN)) << shift;
+        const uint64_t above = __ballot(end > border) & threads, some = __ballot(here > 0.0) & threads;
+        // rounding may leave none above it: the last one that has any then
+        const int at = (above ? __builtin_ctzll(above) : (some ? 63 - __builtin_clzll(some) : shift)) - shift;
+        if ((lane & (SPAN - 1)) == at) {
+            double sum = at == 0 ? before : end - here;
+            bool done = false;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float h = __builtin_amdgcn_exp2f((element<T>(v, i) - m) * c);
-                sum = fmaf(h, h, sum);
+                const double q = s.p(element<T>(v, i));
+                sum += q;
+                if (!done && q > 0.0) token = row.token(vec, i);
+                done |= sum > border;
             }
-            return sum;
         }
+        token = __shfl(token, shift + at, 64);
     }
-
-    // token (or -1 where rounding left none), the total, and the sums before and behind the token
-    template <bool EXACT>
-    static __device__ __forceinline__ int find(R &row, DrawShared &s, float m, double inv_t, double u, bool draws, double &total, double &before, double &behind) {
-        const float c = static_cast<float>(inv_t) * HALF_LOG2E;
-        double mine = 0.0, part[VECS];
-        row.each([&](int j, const uint32_t *v) {
-            double sum = sum_of_vector<EXACT>(v, m, c, inv_t);
-            mine += sum;
-            if (HELD) {
-                asm volatile("" : "+v"(sum));
-                part[HELD ? j : 0] = sum;
-            }
-        });
-        const int wave = LANES > 64 ? threadIdx.x / 64 : 0, lane = row.lane % 64;
-        constexpr int SPAN = LANES < 64 ? LANES : 64;
-        // inclusive sums over the threads of a wave (or of a shorter row)
-        auto upto = [&](double v) {
+    if (vec < 0 || WAVES > 1) {  // (the same for all threads of the row)
+        if (vec < 0) {           // rounding left no sum above it: the last token that has any
+            int last = -1;
+            row.each([&](int j, const uint32_t *v) {
 #pragma unroll
-            for (int by = 1; by < SPAN; by *= 2) {
-                const double o = __shfl_up(v, by, SPAN);
-                if ((lane & (SPAN - 1)) >= by) v += o;
-            }
-            return v;
-        };
-        int vec = -1, at_wave = 0;  // where the border lies
-        before = 0.0;
-        double border = 0.0;
-        if constexpr (HELD > 0 && WAVES > 1) {
-            // the waves' sums of each vector: every exchange halves the vectors that a thread adds up
-            int of = 0;
+                for (int i = 0; i < V; ++i)
+                    if (s.p(element<T>(v, i)) > 0.0) last = max(last, row.token(j, i));
+            });
 #pragma unroll
-            for (int half = VECS / 2, by = 32; half > 0; half /= 2, by /= 2) {
-                const bool upper = lane & by;
-                of += upper ? half : 0;
-#pragma unroll
-                for (int j = 0; j < half; ++j) {
-                    const double give = upper ? part[j] : part[j + half], keep = upper ? part[j + half] : part[j];
-                    part[j] = keep + __shfl_xor(give, by, 64);
-                }
-            }
-#pragma unroll
-            for (int by = 32 / VECS; by > 0; by /= 2) part[0] += __shfl_xor(part[0], by, 64);
-            __syncthreads();
-            if (lane % (64 / VECS) == 0) s.sums[of * WAVES + wave] = part[0];
-            __syncthreads();
-            // in the order of the tokens: vectors, then waves; every wave does this by itself, four sums a thread at most
-            constexpr int N = VECS * WAVES, EACH = (N + 63) / 64;
-            double own[EACH], run = 0.0;
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                own[i] = lane * EACH + i < N ? s.sums[lane * EACH + i] : 0.0;
-                run += own[i];
-            }
-            const double end = upto(run);
-            total = __shfl(end, 63, 64);
-            if (!draws) return -1;
-            border = u * total;
-            double sum = lane ? end - run : 0.0, start = 0.0;
-            int found = N;
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                if (found == N && sum + own[i] > border && lane * EACH + i < N) {
-                    found = lane * EACH + i;
-                    start = sum;
-                }
-                sum += own[i];
-            }
-            const uint64_t any = __ballot(found < N);
-            if (any) {
-                const int from = __builtin_ctzll(any);
-                found = __shfl(found, from, 64);
-                before = __shfl(start, from, 64);
-                vec = found / WAVES;
-                at_wave = found % WAVES;
-            }
-        } else if constexpr (HELD > 0) {
-            total = over_row<LANES>(mine, EXACT ? s.again : s.total, sum_of<double>);
-            if (!draws) return -1;
-            border = u * total;
-            double sum = 0.0;
-#pragma unroll
-            for (int j = 0; j < VECS; ++j) {
-                const double all = VECS == 1 ? total : over_row<LANES>(part[j], s.step, sum_of<double>);
-                if (vec < 0 && sum + all > border) {
-                    vec = j;
-                    before = sum;
-                }
-                sum += all;
-            }
-        } else {
-            // one vector of every thread after another: the waves' sums, the border
-            total = over_row<LANES>(mine, EXACT ? s.again : s.total, sum_of<double>);
-            if (!draws) return -1;
-            border = u * total;
-            double sum = 0.0;
-            bool done = false;
-            for (int j = 0; j < row.vecs && !done; ++j) {
-                uint32_t v[4];
-                row.fetch(j, v);
-                double all = sum_of_vector<EXACT>(v, m, c, inv_t);
-#pragma unroll
-                for (int by = SPAN / 2; by > 0; by /= 2) all += __shfl_xor(all, by, 64);
-                if constexpr (WAVES > 1) {
-                    __syncthreads();
-                    if (lane == 0) s.step[wave] = all;
-                    __syncthreads();
-                }
-#pragma unroll 1
-                for (int w = 0; w < WAVES; ++w) {
-                    const double of_wave = WAVES > 1 ? s.step[w] : all;
-                    if (!done && sum + of_wave > border) {
-                        done = true;
-                        vec = j;
-                        at_wave = w;
-                        before = sum;
-                    }
-                    sum += of_wave;
-                }
-            }
-        }
-        // the thread, then the token; told to all threads of the row
-        if (wave != at_wave) vec = -1;
-        int token = -1;
-        if (vec >= 0) {
-            uint32_t v[4];  // read again: an index into registers would cost more
-            row.fetch(vec, v);
-            const double here = sum_of_vector<EXACT>(v, m, c, inv_t), end = before + upto(here);
-            const int shift = (threadIdx.x % 64) / SPAN * SPAN;
-            const uint64_t threads = (~0ull >> (64 - SPAN)) << shift;
-            const uint64_t above = __ballot(end > border) & threads, some = __ballot(here > 0.0) & threads;
-            // rounding may leave none above it: the last one that has any then
-            const int at = (above ? __builtin_ctzll(above) : (some ? 63 - __builtin_clzll(some) : shift)) - shift;
-            if ((lane & (SPAN - 1)) == at) {
-                double sum = end - here;
-                if (at == 0) sum = before;
-                before = sum;
-                behind = sum;
-                bool done = false;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const double q = p<EXACT>(element<T>(v, i), m, c, inv_t);
-                    if (!done && q > 0.0) {
-                        token = row.token(vec, i);
-                        before = sum;
-                        behind = sum + q;
-                        done = sum + q > border;
-                    }
-                    sum += q;
-                }
-            }
-            token = __shfl(token, shift + at, 64);
-            before = __shfl(before, shift + at, 64);
-            behind = __shfl(behind, shift + at, 64);
+            for (int by = SPAN / 2; by > 0; by /= 2) last = max(last, __shfl_xor(last, by, 64));
+            token = last;
         }
         if constexpr (WAVES > 1) {
+            if (threadIdx.x == 0) sh.token = -1;
             __syncthreads();
-            if (threadIdx.x == 0) s.place = -1;
+            if (lane == 0 && token >= 0) atomicMax(&sh.token, token);
             __syncthreads();
-            if (vec >= 0 && lane == 0) {
-                s.place = token;
-                s.before = before;
-                s.behind = behind;
-            }
-            __syncthreads();
-            token = s.place;
-            before = s.before;
-            behind = s.behind;
+            token = sh.token;
         }
-        return token;
     }
-};
+    return token;
+}
+
+// the lowest token of the largest logit, and the total
+template <class T, int LANES, int HELD>
+__device__ __forceinline__ int find_largest(Row<T, LANES, HELD> &row, DrawShared &sh, const Spread &s, float m, double &total) {
+    constexpr int WAVES = LANES > 64 ? LANES / 64 : 1;
+    double sum = 0.0;
+    int found = 0x7FFFFFFF;
+    row.each([&](int j, const uint32_t *v) {
+        sum += s.of_vector<T>(v);
+#pragma unroll
+        for (int i = 0; i < WIDE<T>; ++i)
+            if (element<T>(v, i) == m) found = min(found, row.token(j, i));
+    });
+    total = over_row<LANES>(sum, sh.total, sum_of<double>);
+#pragma unroll
+    for (int by = (LANES < 64 ? LANES : 64) / 2; by > 0; by /= 2) found = min(found, __shfl_xor(found, by, 64));
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x == 0) sh.token = 0x7FFFFFFF;
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) atomicMin(&sh.token, found);
+        __syncthreads();
+        found = sh.token;
+    }
+    return found;
+}
+
+template <class T, int LANES, int HELD>
+__device__ __forceinline__ float largest(Row<T, LANES, HELD> &row, float *shared) {
+    float m = NEG_INF;
+    row.each([&](int, const uint32_t *v) {
+#pragma unroll
+        for (int e = 0; e < WIDE<T>; ++e) m = larger(m, element<T>(v, e));
+    });
+    return over_row<LANES>(m, shared, larger);
+}
+
+__device__ __forceinline__ void put_drawn(const MgLogits &l, int64_t row, int token, float m, float lp, void *tokens, float *logprob) {
+    put_token(tokens, l.tokens_type, row, token);
+    if (logprob) logprob[row] = token >= 0 ? lp : (m == NEG_INF ? NEG_INF : __builtin_nanf(""));
+}
 
 template <class T, int LANES, int HELD>
 __global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type, void *tokens, float *logprob) {
-    using D = Draw<T, LANES, HELD>;
-    __shared__ DrawShared s;
+    __shared__ DrawShared sh;
     constexpr int ROWS = BLOCK<LANES> / LANES;
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += static_cast<int64_t>(gridDim.x) * ROWS) {
-        typename D::R row(logits + i * l.stride, l.k, lane);
-        const double inv_t = 1.0 / static_cast<double>(l.temperature_dev ? l.temperature_dev[i] : l.temperature);
-        float m = NEG_INF;
-        row.each([&](int, const uint32_t *v) {
-#pragma unroll
-            for (int e = 0; e < D::V; ++e) m = larger(m, element<T>(v, e));
-        });
-        m = over_row<LANES>(m, s.most, larger);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += step) {
+        Row<T, LANES, HELD> row(logits + i * l.stride, l.k, lane);
+        const double u = uniforms ? uniform_at(uniforms, uniforms_type, i) : 0.0;
+        const float m = largest(row, sh.most);
+        const Spread s = spread(l, i, m);
         int token = -1;
-        double total = 0.0, before = 0.0, behind = 0.0;
+        double total = 0.0;
+        if (fabsf(m) < -NEG_INF) token = uniforms ? find_border(row, sh, s, true, u, 0.0, total) : find_largest(row, sh, s, m, total);
+        if (lane == 0) put_drawn(l, i, token, m, token >= 0 && logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
+        if (LANES > 64 && i + step < l.n) __syncthreads();  // the shared values are read
+    }
+}
+
+// A long row's pieces: each one's largest logit and its total relative to that.
+struct DrawPiece {
+    double total;
+    float m, unused;
+};
+
+template <class T>
+__global__ __launch_bounds__(PIECE_LANES) void draw_pieces_kernel(MgLogits l, const T *logits, DrawPiece *pieces) {
+    __shared__ DrawShared sh;
+    const int first = blockIdx.x * PIECE<T>;
+    for (int64_t i = blockIdx.y; i < l.n; i += gridDim.y) {
+        Row<T, PIECE_LANES, PIECE_HELD> row(logits + i * l.stride + first, min(PIECE<T>, l.k - first), threadIdx.x);
+        const float m = largest(row, sh.most);
+        double sum = m == NEG_INF ? 0.0 : __builtin_nan("");
         if (fabsf(m) < -NEG_INF) {
-            const double u = !uniforms ? 0.0 : (uniforms_type == MG_F64 ? static_cast<const double *>(uniforms)[i] : static_cast<double>(static_cast<const float *>(uniforms)[i]));
-            token = D::template find<false>(row, s, m, inv_t, u, uniforms != nullptr, total, before, behind);
-            if (uniforms) {
-                const double off = total * 1.5 * (10.0 * __logf(static_cast<float>(l.k)) + 26.0) * 0x1p-24, border = u * total;
-                if (token < 0 || behind - border < off || border - before < off) {
-                    Row<T, LANES, 0> again(logits + i * l.stride, l.k, lane);
-                    token = Draw<T, LANES, 0>::template find<true>(again, s, m, inv_t, u, true, total, before, behind);
-                }
-            }
-            if (logprob && total < 1.0625) {  // little beside the maximum, whose 1 took some of it: each added in 64 bits
-                double sum = 0.0;
-                const float c = static_cast<float>(inv_t) * HALF_LOG2E;
-                row.each([&](int, const uint32_t *v) {
-#pragma unroll
-                    for (int e = 0; e < D::V; ++e) sum += exp_twice((element<T>(v, e) - m) * c);
-                });
-                if constexpr (D::WAVES > 1) __syncthreads();
-                total = over_row<LANES>(sum, s.step, sum_of<double>);
-            }
-            if (token < 0) {  // the largest, the lowest of equal ones; for a draw: no sum passed the border, the last that has any
-                const bool last = uniforms != nullptr;
-                int found = last ? -1 : l.k;
-#pragma unroll 1
-                for (int j = 0; j < row.vecs; ++j) {
-                    uint32_t v[4];
-                    row.fetch(j, v);
-#pragma unroll
-                    for (int e = 0; e < D::V; ++e) {
-                        const float x = element<T>(v, e);
-                        if (last ? exp((static_cast<double>(x) - m) * inv_t) > 0.0 : x == m) found = last ? max(found, row.token(j, e)) : min(found, row.token(j, e));
-                    }
-                }
-                token = over_row<LANES>(found, s.last, [last](int a, int b) { return last ? max(a, b) : min(a, b); });
-            }
+            const Spread s = spread(l, i, m);
+            sum = 0.0;
+            row.each([&](int, const uint32_t *v) { sum += s.of_vector<T>(v); });
+            sum = over_row<PIECE_LANES>(sum, sh.total, sum_of<double>);
         }
-        if (lane == 0) {
-            put_token(tokens, l.tokens_type, i, token);
-            if (logprob)
-                logprob[i] = token < 0 ? (m == NEG_INF ? NEG_INF : __builtin_nanf(""))
-                                       : static_cast<float>((static_cast<double>(static_cast<float>(logits[i * l.stride + token])) - m) * inv_t - log(total));
+        if (threadIdx.x == 0) pieces[i * gridDim.x + blockIdx.x] = DrawPiece{sum, m, 0.f};
+        __syncthreads();
+    }
+}
+
+// One block to a row: the pieces' totals, the piece in which the border lies, the token in that piece.
+template <class T>
+__global__ __launch_bounds__(PIECE_LANES) void draw_join_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type, const DrawPiece *pieces,
+                                                                int count, void *tokens, float *logprob) {
+    __shared__ DrawShared sh;
+    __shared__ double upto_s[PIECE_LANES], before_s;
+    __shared__ int piece_s;
+    const int tid = threadIdx.x;
+    for (int64_t i = blockIdx.x; i < l.n; i += gridDim.x) {
+        const DrawPiece *of = pieces + i * count;
+        float m = NEG_INF;
+        for (int p = tid; p < count; p += PIECE_LANES) m = larger(m, of[p].m);
+        m = over_row<PIECE_LANES>(m, sh.most, larger);
+        if (!(fabsf(m) < -NEG_INF)) {
+            if (tid == 0) put_drawn(l, i, -1, m, 0.f, tokens, logprob);
+            __syncthreads();
+            continue;
         }
-        if (D::WAVES > 1 && i + static_cast<int64_t>(gridDim.x) * ROWS < l.n) __syncthreads();  // the slots are read
+        const Spread s = spread(l, i, m);
+        auto total_of = [&](int p) { return of[p].m == NEG_INF ? 0.0 : of[p].total * exp2_64((static_cast<double>(of[p].m) - s.m) * s.c); };
+        // a run of adjacent pieces to each thread
+        const int run = (count + PIECE_LANES - 1) / PIECE_LANES, lo = min(tid * run, count), hi = min(lo + run, count);
+        double mine = 0.0;
+        for (int p = lo; p < hi; ++p) mine += total_of(p);
+        upto_s[tid] = mine;
+        if (tid == 0) piece_s = uniforms ? -1 : 0x7FFFFFFF;
+        __syncthreads();
+        for (int by = 1; by < PIECE_LANES; by *= 2) {
+            const double o = tid >= by ? upto_s[tid - by] : 0.0;
+            __syncthreads();
+            upto_s[tid] += o;
+            __syncthreads();
+        }
+        const double total = upto_s[PIECE_LANES - 1];
+        double border = 0.0;
+        if (uniforms) {
+            border = uniform_at(uniforms, uniforms_type, i) * total;
+            // the first piece whose sum passes the border; where rounding leaves none, the last one that has any
+            double sum = tid ? upto_s[tid - 1] : 0.0;
+            int last = -1, found = -1;
+            double start = 0.0, start_last = 0.0;
+            for (int p = lo; p < hi && found < 0; ++p) {
+                const double t = total_of(p);
+                if (t > 0.0) {
+                    last = p;
+                    start_last = sum;
+                }
+                if (sum + t > border) {
+                    found = p;
+                    start = sum;
+                }
+                sum += t;
+            }
+            const bool has = found >= 0;
+            if (has) last = -1;
+            // sums grow from thread to thread, so the first thread that found one has the piece
+            if (tid == 0) sh.token = PIECE_LANES;
+            __syncthreads();
+            if (has) atomicMin(&sh.token, tid);
+            if (last >= 0) atomicMax(&piece_s, last);
+            __syncthreads();
+            const int from = sh.token;
+            const int of_last = piece_s;
+            __syncthreads();
+            if (from < PIECE_LANES ? tid == from : last == of_last) {
+                piece_s = from < PIECE_LANES ? found : last;
+                before_s = from < PIECE_LANES ? start : start_last;
+            }
+        } else {
+            for (int p = lo; p < hi; ++p)
+                if (of[p].m == m) {
+                    atomicMin(&piece_s, p);
+                    break;
+                }
+        }
+        __syncthreads();
+        const int first = piece_s * PIECE<T>;
+        Row<T, PIECE_LANES, PIECE_HELD> row(logits + i * l.stride + first, min(PIECE<T>, l.k - first), tid);
+        double unused;
+        const int token = first + (uniforms ? find_border(row, sh, s, false, border, before_s, unused) : find_largest(row, sh, s, m, unused));
+        if (tid == 0) put_drawn(l, i, token, m, logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
+        __syncthreads();
     }
 }
 
@@ -1486,56 +1554,48 @@ __global__ __launch_bounds__(THREADS) void draw_short_kernel(MgLogits l, const T
     if (row >= l.n) return;
     float x[K];
     load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF_BITS<T>);
-    const double inv_t = 1.0 / static_cast<double>(l.temperature_dev ? l.temperature_dev[row] : l.temperature);
-    float best = x[0];
-    int arg = 0;
-    bool nan = x[0] != x[0];
+    const double u = uniforms ? uniform_at(uniforms, uniforms_type, row) : 0.0;
+    float m = x[0];
 #pragma unroll
-    for (int j = 1; j < K; ++j) {
-        nan |= x[j] != x[j];
-        if (x[j] > best) {
-            best = x[j];
-            arg = j;
-        }
-    }
-    int64_t token = -1;
-    double lp = nan || best != NEG_INF ? __builtin_nan("") : -__builtin_inf();
-    if (!nan && fabsf(best) < -NEG_INF) {
-        // p of a token; what is filled up behind the last one is -inf, so 0
-        auto p = [&](int j) { return exp((static_cast<double>(x[j]) - best) * inv_t); };
+    for (int j = 1; j < K; ++j) m = larger(m, x[j]);
+    const Spread s = spread(l, row, m);
+    int token = -1;
+    float lp = 0.f;
+    if (fabsf(m) < -NEG_INF) {
+        // what is filled up behind the last token is -inf, so 0
         constexpr bool KEEP = K <= 16;
-        double e[KEEP ? K : 1], total = 0.0;
+        double p[KEEP ? K : 1], total = 0.0;
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             if (j >= l.k) break;
-            const double v = p(j);
-            if (KEEP) e[j] = v;
+            const double v = s.p(x[j]);
+            if (KEEP) p[j] = v;
             total += v;
         }
+        float at = m;
         if (uniforms) {
-            const double u = uniforms_type == MG_F64 ? static_cast<const double *>(uniforms)[row] : static_cast<double>(static_cast<const float *>(uniforms)[row]);
             const double border = u * total;
             double upto = 0.0;
-            int last = arg;
             bool done = false;
 #pragma unroll
             for (int j = 0; j < K; ++j) {
                 if (j >= l.k) break;
-                const double v = KEEP ? e[KEEP ? j : 0] : p(j);
+                const double v = KEEP ? p[KEEP ? j : 0] : s.p(x[j]);
                 upto += v;
-                if (!done && v > 0.0) last = j;
+                if (!done && v > 0.0) {
+                    token = j;
+                    at = x[j];
+                }
                 done |= upto > border;
             }
-            arg = last;
-        }
-        token = arg;
-        float at = x[0];
+        } else {
 #pragma unroll
-        for (int j = 1; j < K; ++j) at = arg == j ? x[j] : at;
-        lp = (static_cast<double>(at) - best) * inv_t - log(total);
+            for (int j = K - 1; j >= 0; --j)
+                if (x[j] == m) token = j;
+        }
+        if (logprob) lp = drawn_logprob(at, s, total);
     }
-    put_token(tokens, l.tokens_type, row, token);
-    if (logprob) logprob[row] = static_cast<float>(lp);
+    put_drawn(l, row, token, m, lp, tokens, logprob);
 }
 
 // ---- log-probabilities and entropies -------------------------------------------------------------------------------
@@ -1546,6 +1606,35 @@ __global__ __launch_bounds__(THREADS) void draw_short_kernel(MgLogits l, const T
 struct Soft {
     float m, r, t;
 };
+
+// Two parts of a row as one.
+__device__ __forceinline__ Soft merge(Soft a, Soft b, float inv_t) {
+    if (b.m > a.m || b.m != b.m) {
+        const Soft c = a;
+        a = b;
+        b = c;
+    }
+    if (b.m == NEG_INF) {
+        a.r += b.r + 1.f;  // 0, or NaN
+        return a;
+    }
+    const float d = (b.m - a.m) * inv_t, e = expf(d), s = 1.f + b.r;
+    a.r += s * e;
+    if (e > 0.f) a.t += e * (b.t + s * d);
+    return a;
+}
+
+__device__ __forceinline__ Soft merge_wave(Soft s, float inv_t) {
+#pragma unroll
+    for (int by = 32; by > 0; by /= 2) {
+        Soft o;
+        o.m = __shfl_down(s.m, by, 64);
+        o.r = __shfl_down(s.r, by, 64);
+        o.t = __shfl_down(s.t, by, 64);
+        s = merge(s, o, inv_t);
+    }
+    return s;
+}
 
 // What the slope of a finished row needs: its maximum, the logarithm of its total, its entropy.
 __device__ __forceinline__ float4 row_stats(const Soft &s) {
@@ -1578,56 +1667,91 @@ __device__ __forceinline__ void row_result(int64_t row, const Soft &s, float inv
     if (stats) reinterpret_cast<float4 *>(stats)[row] = st;
 }
 
+struct SoftShared {
+    float most[8];
+    float2 sums[8], rest[8];
+};
+
 template <class T, int LANES, int HELD>
-__global__ __launch_bounds__(BLOCK<LANES>) void logprob_kernel(MgLogits l, const T *logits, const void *tokens, float *logprob, float *entropy, float *stats) {
-    constexpr int ROWS = BLOCK<LANES> / LANES, WAVES = LANES > 64 ? LANES / 64 : 1;
-    __shared__ float most_s[WAVES];
-    __shared__ float2 sums_s[WAVES], rest_s[WAVES];
+__device__ __forceinline__ Soft soft_of(Row<T, LANES, HELD> &row, SoftShared &sh, float inv_t) {
     const auto both = [](float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); };
-    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += static_cast<int64_t>(gridDim.x) * ROWS) {
-        Row<T, LANES, HELD> row(logits + i * l.stride, l.k, lane);
-        constexpr int V = WIDE<T>;
-        const Taken t = taken(l, logits + i * l.stride, i, tokens, logprob != nullptr);
-        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature), c = inv_t * HALF_LOG2E;
-        Soft s{NEG_INF, -1.f, 0.f};
+    const float c = inv_t * HALF_LOG2E;
+    Soft s{largest(row, sh.most), -1.f, 0.f};
+    if (s.m > NEG_INF && s.m < -NEG_INF) {
+        float sum = 0.f, slant = 0.f;
         row.each([&](int, const uint32_t *v) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) s.m = larger(s.m, element<T>(v, e));
+            for (int e = 0; e < WIDE<T>; ++e) {
+                const float z = fmaxf((element<T>(v, e) - s.m) * c, DEEP), p = exp_twice(z);
+                sum += p;
+                slant = fmaf(p, z, slant);
+            }
         });
-        s.m = over_row<LANES>(s.m, most_s, larger);
-        if (s.m > NEG_INF && s.m < -NEG_INF) {
-            float sum = 0.f, slant = 0.f;
+        asm volatile("" : "+v"(sum), "+v"(slant));  // now, not where it is used: every p and z would wait for it
+        const float2 sums = over_row<LANES>(make_float2(sum, slant), sh.sums, both);
+        s.t = sums.y * TWICE_LN2;
+        s.r = sums.x - 1.f;
+        if (sums.x < 1.0625f) {  // little beside the maximum: the sum again without it, and how often it stands there
+            float rest = 0.f, equal = 0.f;
             row.each([&](int, const uint32_t *v) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float z = fmaxf((element<T>(v, e) - s.m) * c, DEEP), p = exp_twice(z);
-                    sum += p;
-                    slant = fmaf(p, z, slant);
+                for (int e = 0; e < WIDE<T>; ++e) {
+                    const float x = element<T>(v, e);
+                    equal += x == s.m ? 1.f : 0.f;
+                    rest += x == s.m ? 0.f : exp_twice((x - s.m) * c);
                 }
             });
-            asm volatile("" : "+v"(sum), "+v"(slant));  // now, not where it is used: every p and z would wait for it
-            const float2 sums = over_row<LANES>(make_float2(sum, slant), sums_s, both);
-            s.t = sums.y * TWICE_LN2;
-            s.r = sums.x - 1.f;
-            if (sums.x < 1.0625f) {  // little beside the maximum: the sum again without it, and how often it stands there
-                float rest = 0.f, equal = 0.f;
-                row.each([&](int, const uint32_t *v) {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float x = element<T>(v, e);
-                        equal += x == s.m ? 1.f : 0.f;
-                        rest += x == s.m ? 0.f : exp_twice((x - s.m) * c);
-                    }
-                });
-                const float2 r = over_row<LANES>(make_float2(rest, equal), rest_s, both);
-                s.r = r.x + (r.y - 1.f);
-            }
-        } else if (s.m != NEG_INF) {
-            s.r = __builtin_nanf("");
+            const float2 r = over_row<LANES>(make_float2(rest, equal), sh.rest, both);
+            s.r = r.x + (r.y - 1.f);
         }
+    } else if (s.m != NEG_INF) {
+        s.r = __builtin_nanf("");
+    }
+    return s;
+}
+
+template <class T, int LANES, int HELD>
+__global__ __launch_bounds__(BLOCK<LANES>) void logprob_kernel(MgLogits l, const T *logits, const void *tokens, float *logprob, float *entropy, float *stats) {
+    __shared__ SoftShared sh;
+    constexpr int ROWS = BLOCK<LANES> / LANES;
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += step) {
+        Row<T, LANES, HELD> row(logits + i * l.stride, l.k, lane);
+        const Taken t = taken(l, logits + i * l.stride, i, tokens, logprob != nullptr);
+        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature);
+        const Soft s = soft_of(row, sh, inv_t);
         if (lane == 0) row_result(i, s, inv_t, t, logprob, entropy, stats);
-        if (WAVES > 1 && i + static_cast<int64_t>(gridDim.x) * ROWS < l.n) __syncthreads();  // the slots are read
+        if (LANES > 64 && i + step < l.n) __syncthreads();  // the shared values are read
+    }
+}
+
+// A long row's pieces, and their join by one wave.
+template <class T>
+__global__ __launch_bounds__(PIECE_LANES) void logprob_pieces_kernel(MgLogits l, const T *logits, float4 *pieces) {
+    __shared__ SoftShared sh;
+    const int first = blockIdx.x * PIECE<T>;
+    for (int64_t i = blockIdx.y; i < l.n; i += gridDim.y) {
+        Row<T, PIECE_LANES, PIECE_HELD> row(logits + i * l.stride + first, min(PIECE<T>, l.k - first), threadIdx.x);
+        const Soft s = soft_of(row, sh, 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature));
+        if (threadIdx.x == 0) pieces[i * gridDim.x + blockIdx.x] = make_float4(s.m, s.r, s.t, 0.f);
+        __syncthreads();
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(64) void logprob_join_kernel(MgLogits l, const T *logits, const float4 *pieces, int count, const void *tokens, float *logprob,
+                                                          float *entropy, float *stats) {
+    for (int64_t i = blockIdx.x; i < l.n; i += gridDim.x) {
+        const Taken t = taken(l, logits + i * l.stride, i, tokens, logprob != nullptr);
+        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature);
+        Soft s{NEG_INF, -1.f, 0.f};
+        for (int p = threadIdx.x; p < count; p += 64) {
+            const float4 q = pieces[i * count + p];
+            s = merge(s, Soft{q.x, q.y, q.z}, inv_t);
+        }
+        s = merge_wave(s, inv_t);
+        if (threadIdx.x == 0) row_result(i, s, inv_t, t, logprob, entropy, stats);
     }
 }
 
@@ -1935,13 +2059,13 @@ void with_size(int k, F f) {
         f(Size<SHORT>{});
 }
 
-// f(threads to a row, vectors that each holds): the fewest threads that hold a row of `vecs` vectors with one each, a wave up to
-// four each, then blocks of 256, 512 and 1024 for as many as their registers take beside what f's kernel needs
+// f(threads to a row, vectors that each holds), for up to HELD_MOST vectors: the fewest threads that hold the row with one each, a
+// wave up to four each, then blocks of 256 and of 512 up to eight
 template <int LANES, int HELD>
 struct Shape {
     static constexpr int lanes = LANES, held = HELD;
 };
-template <int WIDEST, class F>
+template <class F>
 void with_shape(int64_t vecs, F f) {
     if (vecs <= 8)
         f(Shape<8, 1>{});
@@ -1961,14 +2085,14 @@ void with_shape(int64_t vecs, F f) {
         f(Shape<256, 4>{});
     else if (vecs <= 2048)
         f(Shape<256, 8>{});
-    else if (vecs <= 4096)
-        f(Shape<512, 8>{});
-    else if (WIDEST >= 8 && vecs <= 8192)
-        f(Shape<1024, WIDEST < 8 ? WIDEST : 8>{});
-    else if (WIDEST >= 16 && vecs <= 16384)
-        f(Shape<1024, WIDEST>{});
     else
-        f(Shape<1024, 0>{});
+        f(Shape<512, 8>{});
+}
+
+// pieces of a row that no block holds, 0 where one does
+int64_t pieces_of(const MgLogits &l) {
+    const int64_t wide = l.dtype == MG_F32 ? WIDE<float> : WIDE<bf16>, piece = PIECE_LANES * PIECE_HELD * wide;
+    return l.k > HELD_MOST * wide ? (l.k + piece - 1) / piece : 0;
 }
 
 int adjust_args(const char *who, const MgAdjust *a) {
@@ -2088,7 +2212,10 @@ int mg_adjust_logits_grad(const MgAdjust *a, const void *logits_dev, const void 
     return launched("mg_adjust_logits_grad");
 }
 
-int64_t mg_draw_workspace(const MgLogits *l) { return logits_args("mg_draw_workspace", l); }
+int64_t mg_draw_workspace(const MgLogits *l) {
+    const int rc = logits_args("mg_draw_workspace", l);
+    return rc != MG_OK ? rc : l->n * pieces_of(*l) * static_cast<int64_t>(sizeof(DrawPiece));
+}
 
 int mg_draw(const MgLogits *l, const void *logits_dev, const void *uniforms_dev, int32_t uniforms_type, void *tokens_dev,
             float *logprob_dev, void *workspace_dev, int64_t workspace_bytes, void *stream) {
@@ -2096,26 +2223,38 @@ int mg_draw(const MgLogits *l, const void *logits_dev, const void *uniforms_dev,
     if (rc != MG_OK || l->n == 0) return rc;
     if (!logits_dev || !tokens_dev) return refuse(MG_EINVAL, "mg_draw: null argument");
     if (uniforms_dev && uniforms_type != MG_F32 && uniforms_type != MG_F64) return refuse(MG_EINVAL, "mg_draw: unknown type %d of the uniform numbers", uniforms_type);
-    (void)workspace_dev;
-    (void)workspace_bytes;
+    const int64_t pieces = pieces_of(*l);
+    if (!workspace_ok("mg_draw", workspace_dev, workspace_bytes, l->n * pieces * static_cast<int64_t>(sizeof(DrawPiece)))) return MG_EINVAL;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
     with_types(l->dtype, MG_U8, [&](auto t, auto) {
         using T = decltype(t);
-        if (l->k <= SHORT)
-            return with_size(l->k, [&](auto size) {
-                hipLaunchKernelGGL((draw_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0,
-                                   static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), uniforms_dev, uniforms_type, tokens_dev, logprob_dev);
+        const T *x = static_cast<const T *>(logits_dev);
+        if (l->k <= SHORT) {
+            with_size(l->k, [&](auto size) {
+                hipLaunchKernelGGL((draw_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0, s, *l, x, uniforms_dev,
+                                   uniforms_type, tokens_dev, logprob_dev);
             });
-        with_shape<0>((l->k + WIDE<T> - 1) / WIDE<T>, [&](auto shape) {
-            using S = decltype(shape);
-            constexpr int ROWS = BLOCK<S::lanes> / S::lanes;
-            hipLaunchKernelGGL((draw_kernel<T, S::lanes, S::held>), dim3(blocks_for((l->n + ROWS - 1) / ROWS)), dim3(BLOCK<S::lanes>), 0,
-                               static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), uniforms_dev, uniforms_type, tokens_dev, logprob_dev);
-        });
+        } else if (pieces == 0) {
+            with_shape((l->k + WIDE<T> - 1) / WIDE<T>, [&](auto shape) {
+                using S = decltype(shape);
+                constexpr int ROWS = BLOCK<S::lanes> / S::lanes;
+                hipLaunchKernelGGL((draw_kernel<T, S::lanes, S::held>), dim3(blocks_for((l->n + ROWS - 1) / ROWS)), dim3(BLOCK<S::lanes>), 0, s, *l, x, uniforms_dev,
+                                   uniforms_type, tokens_dev, logprob_dev);
+            });
+        } else {
+            DrawPiece *of = static_cast<DrawPiece *>(workspace_dev);
+            hipLaunchKernelGGL((draw_pieces_kernel<T>), dim3(static_cast<unsigned>(pieces), blocks_for(l->n, 65535)), dim3(PIECE_LANES), 0, s, *l, x, of);
+            hipLaunchKernelGGL((draw_join_kernel<T>), dim3(blocks_for(l->n)), dim3(PIECE_LANES), 0, s, *l, x, uniforms_dev, uniforms_type, of,
+                               static_cast<int>(pieces), tokens_dev, logprob_dev);
+        }
     });
     return launched("mg_draw");
 }
 
-int64_t mg_token_logprobs_workspace(const MgLogits *l) { return logits_args("mg_token_logprobs_workspace", l); }
+int64_t mg_token_logprobs_workspace(const MgLogits *l) {
+    const int rc = logits_args("mg_token_logprobs_workspace", l);
+    return rc != MG_OK ? rc : l->n * pieces_of(*l) * static_cast<int64_t>(sizeof(float4));
+}
 
 int mg_token_logprobs(const MgLogits *l, const void *logits_dev, const void *tokens_dev, float *logprob_dev, float *entropy_dev,
                       float *stats_dev, void *workspace_dev, int64_t workspace_bytes, void *stream) {
@@ -2123,21 +2262,30 @@ int mg_token_logprobs(const MgLogits *l, const void *logits_dev, const void *tok
     if (rc != MG_OK || l->n == 0) return rc;
     if (!logits_dev || (logprob_dev && !tokens_dev)) return refuse(MG_EINVAL, "mg_token_logprobs: null argument");
     if (reinterpret_cast<uintptr_t>(stats_dev) % 16) return refuse(MG_EINVAL, "mg_token_logprobs: stats_dev must be 16-byte aligned");
-    (void)workspace_dev;
-    (void)workspace_bytes;
+    const int64_t pieces = pieces_of(*l);
+    if (!workspace_ok("mg_token_logprobs", workspace_dev, workspace_bytes, l->n * pieces * static_cast<int64_t>(sizeof(float4)))) return MG_EINVAL;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
     with_types(l->dtype, MG_U8, [&](auto t, auto) {
         using T = decltype(t);
-        if (l->k <= SHORT)
-            return with_size(l->k, [&](auto size) {
-                hipLaunchKernelGGL((logprob_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0,
-                                   static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), tokens_dev, logprob_dev, entropy_dev, stats_dev);
+        const T *x = static_cast<const T *>(logits_dev);
+        if (l->k <= SHORT) {
+            with_size(l->k, [&](auto size) {
+                hipLaunchKernelGGL((logprob_short_kernel<T, decltype(size)::value>), dim3((l->n + THREADS - 1) / THREADS), dim3(THREADS), 0, s, *l, x, tokens_dev,
+                                   logprob_dev, entropy_dev, stats_dev);
             });
-        with_shape<16>((l->k + WIDE<T> - 1) / WIDE<T>, [&](auto shape) {
-            using S = decltype(shape);
-            constexpr int ROWS = BLOCK<S::lanes> / S::lanes;
-            hipLaunchKernelGGL((logprob_kernel<T, S::lanes, S::held>), dim3(blocks_for((l->n + ROWS - 1) / ROWS)), dim3(BLOCK<S::lanes>), 0,
-                               static_cast<hipStream_t>(stream), *l, static_cast<const T *>(logits_dev), tokens_dev, logprob_dev, entropy_dev, stats_dev);
-        });
+        } else if (pieces == 0) {
+            with_shape((l->k + WIDE<T> - 1) / WIDE<T>, [&](auto shape) {
+                using S = decltype(shape);
+                constexpr int ROWS = BLOCK<S::lanes> / S::lanes;
+                hipLaunchKernelGGL((logprob_kernel<T, S::lanes, S::held>), dim3(blocks_for((l->n + ROWS - 1) / ROWS)), dim3(BLOCK<S::lanes>), 0, s, *l, x, tokens_dev,
+                                   logprob_dev, entropy_dev, stats_dev);
+            });
+        } else {
+            float4 *of = static_cast<float4 *>(workspace_dev);
+            hipLaunchKernelGGL((logprob_pieces_kernel<T>), dim3(static_cast<unsigned>(pieces), blocks_for(l->n, 65535)), dim3(PIECE_LANES), 0, s, *l, x, of);
+            hipLaunchKernelGGL((logprob_join_kernel<T>), dim3(blocks_for(l->n)), dim3(64), 0, s, *l, x, of, static_cast<int>(pieces), tokens_dev, logprob_dev,
+                               entropy_dev, stats_dev);
+        }
     });
     return launched("mg_token_logprobs");
 }
