@@ -291,13 +291,25 @@ __global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, const
 
 // ---- gradient of the embedding -------------------------------------------------------------------------------------
 
-// id f of token n as a row of the table, or -1 if it reads none
-__device__ __forceinline__ int row_of(const EmbedArgs &a, const void *ids, int ids_type, int64_t n, int f, int base) {
-    const int64_t at = n * a.ids_stride + f * a.field_stride;
-    const int64_t id = ids_type == MG_U8 ? static_cast<const uint8_t *>(ids)[at]
-                                         : (ids_type == MG_I32 ? static_cast<const int32_t *>(ids)[at] : static_cast<const int64_t *>(ids)[at]);
-    return id >= 0 && id < a.sizes[f] ? base + static_cast<int>(id) : -1;
+// An id as it lies in memory (a negative one has a large upper or lower half), so that many can be under way before the first
+// is looked at; f(load of the id at an element's index) runs under one test of the ids' type.
+struct Id {
+    uint32_t low, high;
+};
+template <class F>
+__device__ __forceinline__ void with_ids(const void *ids, int type, F f) {
+    if (type == MG_U8)
+        f([=](int64_t at) { return Id{static_cast<const uint8_t *>(ids)[at], 0}; });
+    else if (type == MG_I32)
+        f([=](int64_t at) { return Id{static_cast<const uint32_t *>(ids)[at], 0}; });
+    else
+        f([=](int64_t at) {
+            const uint2 v = static_cast<const uint2 *>(ids)[at];
+            return Id{v.x, v.y};
+        });
 }
+// as a row of the table, or `none`
+__device__ __forceinline__ uint32_t row_of(Id id, uint32_t base, uint32_t size, uint32_t none) { return id.high == 0 && id.low < size ? base + id.low : none; }
 
 // Few rows (up to FEW): the gradient is the product of the rows' indicator [rows][n] (1 where token n reads the row) and the
 // incoming gradient [n][dim], which is what matrix instructions are for: 1 is exact in every type, so every product is, and
@@ -313,6 +325,7 @@ __device__ __forceinline__ int row_of(const EmbedArgs &a, const void *ids, int i
 // 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
 // again, one after the other, each added to its own rows only.
 constexpr int FEW = 64, FEW_BLOCKS = 1024;  // four to a compute unit
+constexpr int64_t FAR_ROWS = 1 << 24;       // a stride up to which 64 tokens lie within 32-bit offsets, and dim's limit
 
 template <class T>
 struct Operand {
@@ -346,7 +359,7 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
     __shared__ __align__(16) uint16_t rows_s[THREADS / 64][MG_MAX_FIELDS][64];  // 0xFFFF: none
     __shared__ float sum_s[TILES * 16][COLS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, l16 = lane % 16, quad = lane / 16;
-    const int d0 = blockIdx.y * COLS, col = l16 * W, left = a.dim - d0 - col;
+    const int d0 = blockIdx.y * COLS, col = l16 * W;
     // the field that this lane's row of each tile belongs to, and the row twice in a word (a row that is none never matches)
     int field[TILES];
     uint32_t twice[TILES];
@@ -365,41 +378,45 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
         for (int i = 0; i < W; ++i) acc[m][i] = float4_t{0.f, 0.f, 0.f, 0.f};
 
     const int64_t step = static_cast<int64_t>(gridDim.x) * THREADS;
-    // whole columns and short rows: one offset of the lane's own, everything else is the same for the wave
-    const bool near = a.dim - d0 >= COLS && a.row_stride < (1 << 20);
-    const uint32_t own = (static_cast<uint32_t>(quad) * 8 * static_cast<uint32_t>(a.row_stride) + col) * static_cast<uint32_t>(sizeof(T));
-    auto fetch_rows = [&](int64_t t0, int (&r)[MG_MAX_FIELDS]) {
-        const int64_t t = t0 + lane;
-        int base = 0;
+    // a lane at the row's end, or behind it, takes the last W columns and keeps of them those that are its own
+    const int from_col = min(col, a.dim - d0 - W);
+    const uint32_t stride = static_cast<uint32_t>(a.row_stride) * sizeof(T), at_col = (d0 + from_col) * sizeof(T), own = quad * 8 * stride + at_col;  // bytes, see FAR_ROWS
+    auto fetch_ids = [&](int64_t t0, Id (&id)[MG_MAX_FIELDS]) {
+        int64_t at = min(t0 + lane, a.n - 1) * a.ids_stride;
+        asm volatile("" : "+v"(at));  // one running address, not one for each field and type
+        with_ids(ids, ids_type, [&](auto load_id) {
+#pragma unroll
+            for (int f = 0; f < MG_MAX_FIELDS; ++f)
+                if (f < a.fields) id[f] = load_id(at + f * a.field_stride);
+        });
+    };
+    auto fetch = [&](int64_t t0, uint32_t (&x)[2][8][WORDS]) {
+        // an address that is the same for the wave, and this lane's offset
+        uint64_t from = reinterpret_cast<uint64_t>(grad + t0 * a.row_stride);
+        asm volatile("" : "+s"(from));
+        auto at = [&](int token, uint32_t offset) { return reinterpret_cast<const T *>(from + static_cast<uint64_t>(token) * stride + offset); };
+        if (t0 + 64 <= a.n) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) load_words<T, W>(at(s * 32 + j, own), W, W, 0, x[s][j]);
+        } else {  // tokens behind the last one read that one; no row takes them
+            const int last = static_cast<int>(a.n - 1 - t0);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) load_words<T, W>(at(0, min(s * 32 + quad * 8 + j, last) * stride + at_col), W, W, 0, x[s][j]);
+        }
+    };
+    auto put_rows = [&](int64_t t0, const Id (&id)[MG_MAX_FIELDS]) {
+        __builtin_amdgcn_wave_barrier();  // the last tokens' rows are read
+        uint32_t base = 0;
 #pragma unroll
         for (int f = 0; f < MG_MAX_FIELDS; ++f)
             if (f < a.fields) {
-                r[f] = t < a.n ? row_of(a, ids, ids_type, t, f, base) : -1;
+                rows_s[wave][f][lane] = static_cast<uint16_t>(t0 + lane < a.n ? row_of(id[f], base, a.sizes[f], 0xFFFF) : 0xFFFF);
                 base += a.sizes[f];
             }
-    };
-    auto fetch = [&](int64_t t0, uint32_t (&x)[2][8][WORDS]) {
-        if (near && t0 + 64 <= a.n) {
-            const char *from = reinterpret_cast<const char *>(grad + t0 * a.row_stride + d0);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) load_words<T, W>(reinterpret_cast<const T *>(from + (s * 32 + j) * a.row_stride * sizeof(T) + own), W, W, 0, x[s][j]);
-        } else {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int64_t t = t0 + s * 32 + quad * 8 + j;
-                    load_words<T, W>(grad + t * a.row_stride + d0 + col, t < a.n ? left : 0, a.dim, 0, x[s][j]);
-                }
-        }
-    };
-    auto put_rows = [&](const int (&r)[MG_MAX_FIELDS]) {
-        __builtin_amdgcn_wave_barrier();  // the last tokens' rows are read
-#pragma unroll
-        for (int f = 0; f < MG_MAX_FIELDS; ++f)
-            if (f < a.fields) rows_s[wave][f][lane] = static_cast<uint16_t>(r[f]);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -448,33 +465,26 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
             }
         }
     };
-    // two sets of registers in turn: the next 64 tokens are under way while these are multiplied
-    int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64;
-    if (t0 < a.n) {
-        uint32_t x0[2][8][WORDS], x1[2][8][WORDS];
-        int r[MG_MAX_FIELDS];
-        fetch_rows(t0, r);
-        fetch(t0, x0);
-        while (true) {
-            put_rows(r);
-            const bool more = t0 + step < a.n;
-            if (more) {
-                fetch_rows(t0 + step, r);
-                fetch(t0 + step, x1);
-            }
-            add(x0);
-            if (!more) break;
-            t0 += step;
-            put_rows(r);
-            const bool again = t0 + step < a.n;
-            if (again) {
-                fetch_rows(t0 + step, r);
-                fetch(t0 + step, x0);
-            }
-            add(x1);
-            if (!again) break;
-            t0 += step;
+    // the next 64 tokens are under way while these are multiplied
+    uint32_t now[2][8][WORDS], next[2][8][WORDS];
+    Id id[MG_MAX_FIELDS];
+    bool have = false;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64;; t0 += step) {
+        const bool more = t0 < a.n;
+        if (more) {
+            fetch_ids(t0, id);
+            fetch(t0, next);
         }
+        if (have) add(now);
+        if (!more) break;
+        put_rows(t0, id);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) now[s][j][i] = next[s][j][i];
+        have = true;
     }
 
     bool fine = true;
@@ -492,25 +502,28 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
 #pragma unroll
                     for (int i = 0; i < W; ++i)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            float &s = sum_s[m * 16 + quad * 4 + q][col + i];
-                            s = w ? s + acc[m][i][q] : acc[m][i][q];
-                        }
+                        for (int q = 0; q < 4; ++q)
+                            if (from_col + i >= col) {
+                                float &s = sum_s[m * 16 + quad * 4 + q][from_col + i];
+                                s = w ? s + acc[m][i][q] : acc[m][i][q];
+                            }
             }
             __syncthreads();
         }
     } else {  // one thread for a column and every (THREADS / COLS)th row
         const int c = threadIdx.x % COLS, share = threadIdx.x / COLS;
         for (int r = share; r < TILES * 16; r += THREADS / COLS) sum_s[r][c] = 0.f;
-        for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * THREADS; t0 < a.n; t0 += step)
-            for (int64_t t = t0; t < t0 + THREADS && t < a.n; ++t) {
-                int base = 0;
-                for (int f = 0; f < a.fields; ++f) {
-                    const int r = row_of(a, ids, ids_type, t, f, base);
-                    if (r >= 0 && r % (THREADS / COLS) == share && d0 + c < a.dim) sum_s[r][c] += static_cast<float>(grad[t * a.row_stride + d0 + c]);
-                    base += a.sizes[f];
+        with_ids(ids, ids_type, [&](auto load_id) {
+            for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * THREADS; t0 < a.n; t0 += step)
+                for (int64_t t = t0; t < t0 + THREADS && t < a.n; ++t) {
+                    uint32_t base = 0;
+                    for (int f = 0; f < a.fields; ++f) {
+                        const uint32_t r = row_of(load_id(t * a.ids_stride + f * a.field_stride), base, a.sizes[f], FEW);
+                        if (r < FEW && r % (THREADS / COLS) == static_cast<uint32_t>(share) && d0 + c < a.dim) sum_s[r][c] += static_cast<float>(grad[t * a.row_stride + d0 + c]);
+                        base += a.sizes[f];
+                    }
                 }
-            }
+        });
         __syncthreads();
     }
     for (int i = threadIdx.x; i < a.rows * COLS; i += THREADS) {
@@ -548,6 +561,29 @@ __global__ __launch_bounds__(JOIN_COLS *JOIN_SHARES) void embed_join_kernel(cons
 // list is cut into chunks of equal length whatever the rows' frequencies are.  A chunk adds up its runs of equal rows; a run
 // that lies inside one chunk is finished there, one that passes a border leaves float32 parts for embed_span_kernel.
 constexpr int MOST_BINS = 512, DIGIT = 9;
+
+// The entries e0, e0 + step, ... (N of them, those below `end`): row (a.rows where the id reads none) and token.
+template <int N>
+__device__ __forceinline__ void load_entries(const EmbedArgs &a, const void *ids, int ids_type, int64_t e0, int64_t step, int64_t end, uint2 (&entry)[N]) {
+    Id id[N];
+    with_ids(ids, ids_type, [&](auto load_id) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int64_t e = min(e0 + j * step, end - 1), n = a.fields == 1 ? e : e / a.fields;
+            id[j] = load_id(n * a.ids_stride + (e - n * a.fields) * a.field_stride);
+        }
+    });
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int64_t e = e0 + j * step, n = a.fields == 1 ? e : e / a.fields;
+        uint32_t base = 0, size = a.sizes[0];
+        for (int f = 1, at = static_cast<int>(e - n * a.fields); f <= at; ++f) {
+            base += size;
+            size = a.sizes[f];
+        }
+        entry[j] = make_uint2(row_of(id[j], base, size, a.rows), static_cast<uint32_t>(n));
+    }
+}
 
 // Lanes with the same digit as this one.
 __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool live) {
@@ -601,14 +637,15 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, c
     __shared__ uint32_t count_s[WAVES][MOST_BINS];
     __shared__ uint32_t wave_sums[WAVES];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    for (int r = tid; r < a.rows; r += SORT_THREADS) touched[r] = 0;
+    // (touched is 16-byte aligned and a multiple of 16 bytes long)
+    for (int r = tid * 16; r < a.rows; r += SORT_THREADS * 16) *reinterpret_cast<uint4 *>(touched + r) = make_uint4(0, 0, 0, 0);
     const int rounds = (entries + SORT_THREADS - 1) / SORT_THREADS, first = wave * rounds * 64 + lane;
-    for (int e = tid; e < entries; e += SORT_THREADS) {
-        const int n = a.fields == 1 ? e : e / a.fields, f = e - n * a.fields;
-        int base = 0;
-        for (int k = 0; k < f; ++k) base += a.sizes[k];
-        const int row = row_of(a, ids, ids_type, n, f, base);
-        word_s[e] = static_cast<uint32_t>(row < 0 ? a.rows : row) << 14 | e;
+    for (int e = tid; e < entries; e += SORT_THREADS * 8) {
+        uint2 entry[8];
+        load_entries(a, ids, ids_type, e, SORT_THREADS, entries, entry);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (e + j * SORT_THREADS < entries) word_s[e + j * SORT_THREADS] = entry[j].x << 14 | (e + j * SORT_THREADS);
     }
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = 14 + pass * bits, bins = 1 << bits;
@@ -652,16 +689,6 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, c
 // `span` adjacent entries (a multiple of SORT_TILE, so that there are at most SORT_BLOCKS blocks).
 constexpr int SORT_TILE = 4096, SORT_BLOCKS = 1024;
 
-__device__ __forceinline__ uint2 entry_at(const EmbedArgs &a, const void *ids, int ids_type, const uint2 *from, int64_t e) {
-    if (from) return from[e];
-    const int64_t n = a.fields == 1 ? e : e / a.fields;
-    const int f = static_cast<int>(e - n * a.fields);
-    int base = 0;
-    for (int k = 0; k < f; ++k) base += a.sizes[k];
-    const int row = row_of(a, ids, ids_type, n, f, base);
-    return make_uint2(static_cast<uint32_t>(row < 0 ? a.rows : row), static_cast<uint32_t>(n));
-}
-
 __global__ __launch_bounds__(THREADS) void embed_count_kernel(EmbedArgs a, const void *ids, int ids_type, const uint2 *from, int64_t entries, int span,
                                                               int shift, int bits, uint32_t *counts, uint8_t *touched) {
     __shared__ uint32_t count_s[MOST_BINS];
@@ -671,7 +698,17 @@ __global__ __launch_bounds__(THREADS) void embed_count_kernel(EmbedArgs a, const
         for (int64_t r = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; r < a.rows; r += static_cast<int64_t>(gridDim.x) * THREADS) touched[r] = 0;
     __syncthreads();
     const int64_t lo = static_cast<int64_t>(blockIdx.x) * span, hi = min(lo + span, entries);
-    for (int64_t e = lo + threadIdx.x; e < hi; e += THREADS) atomicAdd(&count_s[(entry_at(a, ids, ids_type, from, e).x >> shift) & (bins - 1)], 1u);
+    for (int64_t e = lo + threadIdx.x; e < hi; e += THREADS * 8) {
+        uint2 entry[8];
+        if (from)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) entry[j] = from[min(e + j * THREADS, hi - 1)];
+        else
+            load_entries(a, ids, ids_type, e, THREADS, hi, entry);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (e + j * THREADS < hi) atomicAdd(&count_s[(entry[j].x >> shift) & (bins - 1)], 1u);
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < bins; i += THREADS) counts[static_cast<int64_t>(i) * gridDim.x + blockIdx.x] = count_s[i];
 }
@@ -712,8 +749,11 @@ __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const
         const int64_t first = e0 + wave * (SORT_TILE / WAVES) + lane;
         uint2 entry[ROUNDS];
         uint32_t at[ROUNDS];
+        if (from)
 #pragma unroll
-        for (int j = 0; j < ROUNDS; ++j) entry[j] = first + j * 64 < hi ? entry_at(a, ids, ids_type, from, first + j * 64) : make_uint2(0, 0);
+            for (int j = 0; j < ROUNDS; ++j) entry[j] = from[min(first + j * 64, hi - 1)];
+        else
+            load_entries(a, ids, ids_type, first, 64, hi, entry);
 #pragma unroll
         for (int j = 0; j < ROUNDS; ++j) at[j] = place(count_s[wave], (entry[j].x >> shift) & (bins - 1), bits, first + j * 64 < hi, lane);
         __syncthreads();
@@ -1942,10 +1982,10 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
         p.bytes += (bytes + 15) / 16 * 16;
         return at;
     };
-    p.few = a.rows <= FEW;
+    p.few = a.rows <= FEW && a.row_stride <= FAR_ROWS;
     if (p.few) {
         p.width = wide / 2;  // the narrowest that holds a token's columns at once, or 8 bytes: two sets of 16 loads are held
-        while (p.width > 1 && 16 * (p.width / 2) >= a.dim) p.width /= 2;
+        while (p.width > 1 && (16 * (p.width / 2) >= a.dim || p.width > a.dim)) p.width /= 2;
         p.tiles = a.rows <= 16 ? 1 : (a.rows <= 32 ? 2 : 4);
         const int64_t blocks = (a.n + THREADS - 1) / THREADS;
         const int64_t slabs = (a.dim + 16 * p.width - 1) / (16 * p.width), most = slabs < FEW_BLOCKS / 64 ? FEW_BLOCKS / slabs : 64;
