@@ -289,6 +289,90 @@ __global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, const
     }
 }
 
+// The same where LDS holds the finished output of every combination of a token's ids, none included (cells: 12 x 7 x 8): worked
+// out once a block, then each 16 bytes of output are one read of LDS and one store.
+constexpr int COMBINED_BYTES = 49152, COMBINED_THREADS = 512, COMBINED_BLOCKS = 768;  // three blocks to a compute unit
+static_assert(FAR == COMBINED_THREADS, "a token's ids to each thread");
+
+template <class T, class I>
+__global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedArgs a, int combined, const I *ids, const T *table, T *out) {
+    constexpr int V = WIDE<T>, TOGETHER = 4;
+    extern __shared__ __align__(16) char lds[];
+    const int vecs = (a.dim + V - 1) / V, pitch = vecs * V;
+    T *done_s = reinterpret_cast<T *>(lds), *table_s = done_s + combined * pitch;  // [combined][pitch], [rows + 1][pitch]
+    uint16_t *which_s = reinterpret_cast<uint16_t *>(table_s + (a.rows + 1) * pitch);
+    for (int i = threadIdx.x; i < (a.rows + 1) * pitch; i += COMBINED_THREADS) {
+        const int r = i / pitch, d = i - r * pitch;
+        table_s[i] = r < a.rows && d < a.dim ? table[r * a.row_stride + d] : static_cast<T>(0.f);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < combined * vecs; i += COMBINED_THREADS) {
+        const int c = i / combined;
+        int rest = i - c * combined, base = a.rows;
+        const int at = rest;
+        float acc[V] = {};
+        for (int f = a.fields - 1; f >= 0; --f) {  // the last field varies first; the sum is over fields in any order
+            const int size = a.sizes[f], id = rest % (size + 1);
+            rest /= size + 1;
+            base -= size;
+            float x[V];
+            load<T, V>(table_s + (id < size ? base + id : a.rows) * pitch + c * V, x);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] *= a.scale;
+        store<T, V>(done_s + at * pitch + c * V, acc);
+    }
+    const int cols = min(vecs, COMBINED_THREADS), per_block = COMBINED_THREADS / cols;
+    const int sub = threadIdx.x / cols, col = threadIdx.x - sub * cols;
+    for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * FAR; n0 < a.n; n0 += static_cast<int64_t>(gridDim.x) * FAR) {
+        const int tokens = static_cast<int>(min(static_cast<int64_t>(FAR), a.n - n0));
+        __syncthreads();
+        {
+            const int t = min(static_cast<int>(threadIdx.x), tokens - 1);  // FAR is COMBINED_THREADS
+            const I *from = ids + (n0 + t) * a.ids_stride;
+            I id[MG_MAX_FIELDS];
+#pragma unroll
+            for (int f = 0; f < MG_MAX_FIELDS; ++f)
+                if (f < a.fields) id[f] = from[f * a.field_stride];
+            int which = 0;
+#pragma unroll
+            for (int f = 0; f < MG_MAX_FIELDS; ++f)
+                if (f < a.fields) {
+                    const int64_t v = static_cast<int64_t>(id[f]);
+                    which = which * (a.sizes[f] + 1) + (v >= 0 && v < a.sizes[f] ? static_cast<int>(v) : a.sizes[f]);
+                }
+            which_s[threadIdx.x] = static_cast<uint16_t>(which);
+        }
+        __syncthreads();
+        if (sub < per_block)
+            for (int c = col; c < vecs; c += cols)
+                for (int t0 = sub; t0 < tokens; t0 += per_block * TOGETHER) {
+                    uint4 q[TOGETHER];
+#pragma unroll
+                    for (int u = 0; u < TOGETHER; ++u) q[u] = *reinterpret_cast<const uint4 *>(done_s + which_s[min(t0 + u * per_block, FAR - 1)] * pitch + c * V);
+#pragma unroll
+                    for (int u = 0; u < TOGETHER; ++u) {
+                        const int t = t0 + u * per_block;
+                        if (t >= tokens) break;
+                        T *to = out + (n0 + t) * a.dim + c * V;
+                        if (c * V + V <= a.dim) {
+                            struct __attribute__((packed, aligned(sizeof(T)))) Words {
+                                uint32_t w[4];
+                            };
+                            *reinterpret_cast<Words *>(to) = Words{{q[u].x, q[u].y, q[u].z, q[u].w}};
+                        } else {
+                            const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+                            for (int e = 0; e < V; ++e)
+                                if (c * V + e < a.dim) to[e] = static_cast<T>(element<T>(w, e));
+                        }
+                    }
+                }
+    }
+}
+
 // ---- gradient of the embedding -------------------------------------------------------------------------------------
 
 // An id as it lies in memory (a negative one has a large upper or lower half), so that many can be under way before the first
@@ -319,12 +403,12 @@ __device__ __forceinline__ uint32_t row_of(Id id, uint32_t base, uint32_t size, 
 // columns.  The indicator's fragment (row l % 16, tokens 8 (l / 16) ...) is made from eight row numbers by three packed 16-bit
 // instructions per pair; the gradient's fragment (column l % 16, the same tokens) comes straight from memory, W adjacent
 // columns of a token to a lane, so that product i of W covers columns W * (0 .. 15) + i and pairs of tokens meet by one byte
-// permutation each.  Waves and blocks stride over the tokens, a block adds its four waves, embed_join_kernel the blocks, all
+// permutation each.  The order of the tokens within 32 is free: a load takes four adjacent tokens, whole lines of memory.  Waves and blocks stride over the tokens, a block adds its four waves, embed_join_kernel the blocks, all
 // in a fixed order.
 //
 // 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
 // again, one after the other, each added to its own rows only.
-constexpr int FEW = 64, FEW_BLOCKS = 1024;  // four to a compute unit
+constexpr int FEW = 64, FEW_BLOCKS = 768;  // three to a compute unit, two where a lane loads 8 bytes
 constexpr int64_t FAR_ROWS = 1 << 24;       // a stride up to which 64 tokens lie within 32-bit offsets, and dim's limit
 
 template <class T>
@@ -354,7 +438,7 @@ union Fragment {
 };
 
 template <class T, int W, int TILES>
-__global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
+__global__ __launch_bounds__(THREADS, TILES > 2 || W * sizeof(T) > 4 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
     constexpr int COLS = 16 * W, WORDS = (W * sizeof(T) + 3) / 4;
     __shared__ __align__(16) uint16_t rows_s[THREADS / 64][MG_MAX_FIELDS][64];  // 0xFFFF: none
     __shared__ float sum_s[TILES * 16][COLS];
@@ -380,7 +464,7 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
     const int64_t step = static_cast<int64_t>(gridDim.x) * THREADS;
     // a lane at the row's end, or behind it, takes the last W columns and keeps of them those that are its own
     const int from_col = min(col, a.dim - d0 - W);
-    const uint32_t stride = static_cast<uint32_t>(a.row_stride) * sizeof(T), at_col = (d0 + from_col) * sizeof(T), own = quad * 8 * stride + at_col;  // bytes, see FAR_ROWS
+    const uint32_t stride = static_cast<uint32_t>(a.row_stride) * sizeof(T), at_col = (d0 + from_col) * sizeof(T), own = quad * stride + at_col;  // bytes, see FAR_ROWS
     auto fetch_ids = [&](int64_t t0, Id (&id)[MG_MAX_FIELDS]) {
         int64_t at = min(t0 + lane, a.n - 1) * a.ids_stride;
         asm volatile("" : "+v"(at));  // one running address, not one for each field and type
@@ -399,22 +483,23 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) load_words<T, W>(at(s * 32 + j, own), W, W, 0, x[s][j]);
+                for (int j = 0; j < 8; ++j) load_words<T, W>(at(s * 32 + j * 4, own), W, W, 0, x[s][j]);
         } else {  // tokens behind the last one read that one; no row takes them
             const int last = static_cast<int>(a.n - 1 - t0);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) load_words<T, W>(at(0, min(s * 32 + quad * 8 + j, last) * stride + at_col), W, W, 0, x[s][j]);
+                for (int j = 0; j < 8; ++j) load_words<T, W>(at(0, min(s * 32 + j * 4 + quad, last) * stride + at_col), W, W, 0, x[s][j]);
         }
     };
     auto put_rows = [&](int64_t t0, const Id (&id)[MG_MAX_FIELDS]) {
         __builtin_amdgcn_wave_barrier();  // the last tokens' rows are read
+        const int place = (lane & 32) + (lane & 3) * 8 + (lane & 31) / 4;  // token j * 4 + quad is number j of the quad
         uint32_t base = 0;
 #pragma unroll
         for (int f = 0; f < MG_MAX_FIELDS; ++f)
             if (f < a.fields) {
-                rows_s[wave][f][lane] = static_cast<uint16_t>(t0 + lane < a.n ? row_of(id[f], base, a.sizes[f], 0xFFFF) : 0xFFFF);
+                rows_s[wave][f][place] = static_cast<uint16_t>(t0 + lane < a.n ? row_of(id[f], base, a.sizes[f], 0xFFFF) : 0xFFFF);
                 base += a.sizes[f];
             }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -465,26 +550,26 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
             }
         }
     };
-    // the next 64 tokens are under way while these are multiplied
-    uint32_t now[2][8][WORDS], next[2][8][WORDS];
+    // three sets of registers in turn: while one is multiplied, the loads of the next two are under way (one ahead leaves the
+    // memory idle whenever a wave waits: 3.6 TB/s).  Ids are loaded one set ahead, before the loads of the set behind that.
+    uint32_t x0[2][8][WORDS], x1[2][8][WORDS], x2[2][8][WORDS];
     Id id[MG_MAX_FIELDS];
-    bool have = false;
-    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64;; t0 += step) {
-        const bool more = t0 < a.n;
-        if (more) {
-            fetch_ids(t0, id);
-            fetch(t0, next);
-        }
-        if (have) add(now);
-        if (!more) break;
+    int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64;
+    auto turn = [&](uint32_t (&now)[2][8][WORDS], uint32_t (&far)[2][8][WORDS]) {
+        if (t0 >= a.n) return false;
         put_rows(t0, id);
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int i = 0; i < WORDS; ++i) now[s][j][i] = next[s][j][i];
-        have = true;
+        if (t0 + step < a.n) fetch_ids(t0 + step, id);
+        if (t0 + 2 * step < a.n) fetch(t0 + 2 * step, far);
+        add(now);
+        t0 += step;
+        return true;
+    };
+    if (t0 < a.n) {
+        fetch_ids(t0, id);
+        fetch(t0, x0);
+        if (t0 + step < a.n) fetch(t0 + step, x1);
+        while (turn(x0, x2) && turn(x1, x0) && turn(x2, x1)) {
+        }
     }
 
     bool fine = true;
@@ -627,18 +712,31 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t v, uint32_t *wave_sums, 
     return before + s - v;
 }
 
+// The gradient's bytes to 0, by the blocks beside those that sort: the rows that no token reads stay so, the others are written
+// when their sums are known.
+__device__ __forceinline__ void clear(char *out, int64_t bytes, int64_t block, int64_t blocks) {
+    struct __attribute__((packed, aligned(1))) Words {
+        uint32_t w[4];
+    };
+    for (int64_t i = (block * blockDim.x + threadIdx.x) * 16; i < bytes; i += blocks * blockDim.x * 16) {
+        if (i + 16 <= bytes)
+            *reinterpret_cast<Words *>(out + i) = Words{{0, 0, 0, 0}};
+        else
+            for (int64_t b = i; b < bytes; ++b) out[b] = 0;
+    }
+}
+
 // Up to SORT_ONE entries and 2^18 - 1 rows: one workgroup sorts words of row << 14 | entry in LDS.
 constexpr int SORT_THREADS = 1024, SORT_ONE = 1 << 14, SORT_ROWS = (1 << 18) - 1;
 
 __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, const void *ids, int ids_type, int entries, int passes, int bits,
-                                                                  uint32_t *rows_out, uint32_t *tokens_out, uint8_t *touched) {
+                                                                  uint32_t *rows_out, uint32_t *tokens_out, char *out, int64_t out_bytes) {
     constexpr int WAVES = SORT_THREADS / 64, ROUNDS = SORT_ONE / SORT_THREADS;
+    if (blockIdx.x > 0) return clear(out, out_bytes, blockIdx.x - 1, gridDim.x - 1);
     __shared__ uint32_t word_s[SORT_ONE];
     __shared__ uint32_t count_s[WAVES][MOST_BINS];
     __shared__ uint32_t wave_sums[WAVES];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    // (touched is 16-byte aligned and a multiple of 16 bytes long)
-    for (int r = tid * 16; r < a.rows; r += SORT_THREADS * 16) *reinterpret_cast<uint4 *>(touched + r) = make_uint4(0, 0, 0, 0);
     const int rounds = (entries + SORT_THREADS - 1) / SORT_THREADS, first = wave * rounds * 64 + lane;
     for (int e = tid; e < entries; e += SORT_THREADS * 8) {
         uint2 entry[8];
@@ -678,10 +776,9 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, c
         __syncthreads();
     }
     for (int i = tid; i < entries; i += SORT_THREADS) {
-        const uint32_t w = word_s[i], row = w >> 14;
-        rows_out[i] = row;
+        const uint32_t w = word_s[i];
+        rows_out[i] = w >> 14;
         tokens_out[i] = a.fields == 1 ? (w & (SORT_ONE - 1)) : (w & (SORT_ONE - 1)) / a.fields;
-        if (row < static_cast<uint32_t>(a.rows)) touched[row] = 1;
     }
 }
 
@@ -690,12 +787,11 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, c
 constexpr int SORT_TILE = 4096, SORT_BLOCKS = 1024;
 
 __global__ __launch_bounds__(THREADS) void embed_count_kernel(EmbedArgs a, const void *ids, int ids_type, const uint2 *from, int64_t entries, int span,
-                                                              int shift, int bits, uint32_t *counts, uint8_t *touched) {
+                                                              int shift, int bits, int blocks, uint32_t *counts, char *out, int64_t out_bytes) {
     __shared__ uint32_t count_s[MOST_BINS];
     const int bins = 1 << bits;
+    if (static_cast<int>(blockIdx.x) >= blocks) return clear(out, out_bytes, blockIdx.x - blocks, gridDim.x - blocks);
     for (int i = threadIdx.x; i < bins; i += THREADS) count_s[i] = 0;
-    if (touched)
-        for (int64_t r = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x; r < a.rows; r += static_cast<int64_t>(gridDim.x) * THREADS) touched[r] = 0;
     __syncthreads();
     const int64_t lo = static_cast<int64_t>(blockIdx.x) * span, hi = min(lo + span, entries);
     for (int64_t e = lo + threadIdx.x; e < hi; e += THREADS * 8) {
@@ -710,7 +806,7 @@ __global__ __launch_bounds__(THREADS) void embed_count_kernel(EmbedArgs a, const
             if (e + j * THREADS < hi) atomicAdd(&count_s[(entry[j].x >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < bins; i += THREADS) counts[static_cast<int64_t>(i) * gridDim.x + blockIdx.x] = count_s[i];
+    for (int i = threadIdx.x; i < bins; i += THREADS) counts[static_cast<int64_t>(i) * blocks + blockIdx.x] = count_s[i];
 }
 
 __global__ __launch_bounds__(SORT_THREADS) void embed_scan_kernel(uint32_t *counts, int n) {
@@ -737,7 +833,7 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scan_kernel(uint32_t *coun
 
 __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const void *ids, int ids_type, const uint2 *from, int64_t entries, int span,
                                                               int shift, int bits, const uint32_t *counts, uint2 *to, uint32_t *rows_out,
-                                                              uint32_t *tokens_out, uint8_t *touched) {
+                                                              uint32_t *tokens_out) {
     constexpr int WAVES = THREADS / 64, ROUNDS = SORT_TILE / THREADS;
     __shared__ uint32_t count_s[WAVES][MOST_BINS], base_s[MOST_BINS];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, bins = 1 << bits;
@@ -776,7 +872,6 @@ __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const
                 } else {
                     rows_out[p] = entry[j].x;
                     tokens_out[p] = entry[j].y;
-                    if (entry[j].x < static_cast<uint32_t>(a.rows)) touched[entry[j].x] = 1;
                 }
             }
         __syncthreads();
@@ -785,12 +880,10 @@ __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const
 
 struct Sorted {
     const uint32_t *rows, *tokens;  // [entries], by row; a.rows behind the last row
-    const uint8_t *touched;         // [a.rows]
     float *head, *tail;             // [chunks][dim]: what a chunk has of a run that an earlier chunk began / that goes on behind it
     int64_t entries;
     int32_t chunk, chunks;          // entries of a chunk, number of chunks
     int32_t lanes;                  // threads per chunk: a power of two, up to 64
-    int32_t sum_blocks;             // blocks that add up; those behind clear the rows that no token reads
 };
 
 template <class T>
@@ -799,13 +892,6 @@ __global__ __launch_bounds__(THREADS) void embed_runs_kernel(EmbedArgs a, Sorted
     const int lane = threadIdx.x % s.lanes, group = threadIdx.x / s.lanes, groups = THREADS / s.lanes;
     const int d0 = (blockIdx.y * s.lanes + lane) * V, left = a.dim - d0;
     if (left <= 0) return;
-    if (static_cast<int>(blockIdx.x) >= s.sum_blocks) {
-        const float zero[V] = {};
-        const int64_t step = static_cast<int64_t>(gridDim.x - s.sum_blocks) * groups;
-        for (int64_t r = static_cast<int64_t>(blockIdx.x - s.sum_blocks) * groups + group; r < a.rows; r += step)
-            if (!s.touched[r]) store_part<T, V>(out + r * a.dim + d0, left, zero);
-        return;
-    }
     const int64_t c = static_cast<int64_t>(blockIdx.x) * groups + group;
     if (c >= s.chunks) return;
     const int64_t e0 = c * s.chunk, e1 = min(e0 + s.chunk, s.entries);
@@ -855,22 +941,16 @@ template <class T>
 __global__ __launch_bounds__(THREADS) void embed_span_kernel(EmbedArgs a, Sorted s, T *out) {
     constexpr int SPAN = 64;  // columns of a block
     __shared__ float sum_s[THREADS / SPAN][SPAN];
-    const int64_t c = blockIdx.x, e0 = c * s.chunk, e1 = min(e0 + s.chunk, s.entries);
+    const int64_t c = blockIdx.x, e0 = c * s.chunk, e1 = e0 + s.chunk;
     if (e1 >= s.entries) return;
-    const uint32_t row = s.rows[e1 - 1];
-    if (row == static_cast<uint32_t>(a.rows) || s.rows[e1] != row) return;  // nothing goes on here
-    if (c > 0 && s.rows[e0] == row && s.rows[e0 - 1] == row) return;        // an earlier chunk began it
-    int64_t lo = c + 1, hi = s.chunks;  // chunks lo .. hi - 1 start with this row: rows are sorted, so the end is found by halving
-    {
-        int64_t a0 = lo, b0 = hi;
-        while (a0 < b0) {
-            const int64_t mid = (a0 + b0) / 2;
-            if (s.rows[mid * s.chunk] == row)
-                a0 = mid + 1;
-            else
-                b0 = mid;
-        }
-        hi = a0;
+    const uint32_t row = s.rows[e1 - 1], after = s.rows[e1], start = s.rows[e0], before = c > 0 ? s.rows[e0 - 1] : a.rows;
+    if (row == static_cast<uint32_t>(a.rows) || after != row) return;  // nothing goes on here
+    if (start == row && before == row) return;                         // an earlier chunk began it
+    const int64_t lo = c + 1;
+    int64_t hi = lo;  // chunks lo .. hi - 1 start with this row
+    for (int more = THREADS; more == THREADS; hi += more) {
+        const int64_t at = hi + threadIdx.x;
+        more = __syncthreads_count(at < s.chunks && s.rows[at * s.chunk] == row);
     }
     const int col = threadIdx.x % SPAN, share = threadIdx.x / SPAN;
     const int d = blockIdx.y * SPAN + col;
@@ -1971,7 +2051,7 @@ struct GradPlan {
     int64_t entries;
     int bits, passes, sort_blocks, span;
     Sorted s;
-    int64_t at_rows, at_tokens, at_touched, at_head, at_tail, at_pairs, at_counts;
+    int64_t at_rows, at_tokens, at_head, at_tail, at_pairs, at_counts;
     int64_t bytes;
 };
 
@@ -1988,7 +2068,8 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
         while (p.width > 1 && (16 * (p.width / 2) >= a.dim || p.width > a.dim)) p.width /= 2;
         p.tiles = a.rows <= 16 ? 1 : (a.rows <= 32 ? 2 : 4);
         const int64_t blocks = (a.n + THREADS - 1) / THREADS;
-        const int64_t slabs = (a.dim + 16 * p.width - 1) / (16 * p.width), most = slabs < FEW_BLOCKS / 64 ? FEW_BLOCKS / slabs : 64;
+        const int64_t slabs = (a.dim + 16 * p.width - 1) / (16 * p.width), all = p.width * 2 == wide ? FEW_BLOCKS * 2 / 3 : FEW_BLOCKS,
+                      most = slabs < all / 64 ? all / slabs : 64;
         p.blocks = static_cast<int>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
         if (p.blocks > 1) take(static_cast<int64_t>(p.blocks) * a.rows * a.dim * 4);
         return p;
@@ -2001,7 +2082,6 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
     p.one = p.entries <= SORT_ONE && a.rows <= SORT_ROWS;
     p.at_rows = take(p.entries * 4);
     p.at_tokens = take(p.entries * 4);
-    p.at_touched = take(a.rows);
     // chunks of 16 entries until there are 4096 of them, longer ones then
     int64_t chunk = (p.entries + 4095) / 4096;
     chunk = chunk < 16 ? 16 : (chunk + 7) / 8 * 8;
@@ -2012,8 +2092,6 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
     p.at_tail = take(static_cast<int64_t>(p.s.chunks) * a.dim * 4);
     p.s.lanes = 1;
     while (p.s.lanes < 64 && p.s.lanes * wide < a.dim) p.s.lanes *= 2;
-    const int groups = THREADS / p.s.lanes;
-    p.s.sum_blocks = (p.s.chunks + groups - 1) / groups;
     if (!p.one) {
         int64_t span = (p.entries + SORT_BLOCKS - 1) / SORT_BLOCKS;
         span = (span + SORT_TILE - 1) / SORT_TILE * SORT_TILE;
@@ -2054,32 +2132,34 @@ void launch_grad(const EmbedArgs &a, GradPlan p, const void *ids, int ids_type, 
         return;
     }
     uint32_t *rows = reinterpret_cast<uint32_t *>(ws + p.at_rows), *tokens = reinterpret_cast<uint32_t *>(ws + p.at_tokens);
-    uint8_t *touched = reinterpret_cast<uint8_t *>(ws + p.at_touched);
+    char *bytes = reinterpret_cast<char *>(out);
+    const int64_t out_bytes = static_cast<int64_t>(a.rows) * a.dim * sizeof(T);
     if (p.one) {
-        hipLaunchKernelGGL(embed_sort_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, a, ids, ids_type, static_cast<int>(p.entries), p.passes, p.bits, rows, tokens,
-                           touched);
+        const int64_t fill = (out_bytes + SORT_THREADS * 64 - 1) / (SORT_THREADS * 64);  // four stores a thread, or a block to each compute unit
+        hipLaunchKernelGGL(embed_sort_kernel, dim3(1 + static_cast<unsigned>(fill < 255 ? fill : 255)), dim3(SORT_THREADS), 0, stream, a, ids, ids_type,
+                           static_cast<int>(p.entries), p.passes, p.bits, rows, tokens, bytes, out_bytes);
     } else {
         uint2 *pairs = reinterpret_cast<uint2 *>(ws + p.at_pairs);
         uint32_t *counts = reinterpret_cast<uint32_t *>(ws + p.at_counts);
         const uint2 *from = nullptr;
         for (int pass = 0; pass < p.passes; ++pass) {
             uint2 *to = pass + 1 < p.passes ? pairs + (pass & 1) * p.entries : nullptr;
-            hipLaunchKernelGGL(embed_count_kernel, dim3(p.sort_blocks), dim3(THREADS), 0, stream, a, ids, ids_type, from, p.entries, p.span, pass * p.bits, p.bits,
-                               counts, pass == 0 ? touched : nullptr);
+            const int64_t fill = pass ? 0 : (out_bytes + THREADS * 64 - 1) / (THREADS * 64);
+            hipLaunchKernelGGL(embed_count_kernel, dim3(p.sort_blocks + static_cast<unsigned>(fill < 2048 ? fill : 2048)), dim3(THREADS), 0, stream, a, ids, ids_type,
+                               from, p.entries, p.span, pass * p.bits, p.bits, p.sort_blocks, counts, bytes, out_bytes);
             hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, counts, p.sort_blocks << p.bits);
             hipLaunchKernelGGL(embed_place_kernel, dim3(p.sort_blocks), dim3(THREADS), 0, stream, a, ids, ids_type, from, p.entries, p.span, pass * p.bits, p.bits,
-                               counts, to, rows, tokens, touched);
+                               counts, to, rows, tokens);
             from = to;
         }
     }
     p.s.rows = rows;
     p.s.tokens = tokens;
-    p.s.touched = touched;
     p.s.head = reinterpret_cast<float *>(ws + p.at_head);
     p.s.tail = reinterpret_cast<float *>(ws + p.at_tail);
+    if (p.s.chunks == 0) return;
     const int groups = THREADS / p.s.lanes;
-    const int64_t clear = (a.rows + groups - 1) / groups;
-    const dim3 grid(p.s.sum_blocks + static_cast<unsigned>(clear < 2048 ? clear : 2048), (a.dim + p.s.lanes * WIDE<T> - 1) / (p.s.lanes * WIDE<T>));
+    const dim3 grid((p.s.chunks + groups - 1) / groups, (a.dim + p.s.lanes * WIDE<T> - 1) / (p.s.lanes * WIDE<T>));
     hipLaunchKernelGGL((embed_runs_kernel<T>), grid, dim3(THREADS), 0, stream, a, p.s, grad, out);
     if (p.s.chunks > 1) hipLaunchKernelGGL((embed_span_kernel<T>), dim3(p.s.chunks, (a.dim + 63) / 64), dim3(THREADS), 0, stream, a, p.s, out);
 }
@@ -2201,7 +2281,16 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
         using I = decltype(i);
         const int vecs = (a.dim + WIDE<T> - 1) / WIDE<T>, per_block = THREADS / (vecs < THREADS ? vecs : THREADS);
         const int64_t held = static_cast<int64_t>(a.rows + 1) * vecs * 16;
-        // worth its copy from a few blocks' tokens on
+        // what a block prepares has to be little beside the tokens it then writes: sixteen times as many, and a few blocks' tokens
+        // for a table alone
+        int64_t combined = 1;
+        for (int f = 0; f < a.fields; ++f) combined = combined * (a.sizes[f] + 1) <= (1 << 15) ? combined * (a.sizes[f] + 1) : 1 << 15;
+        if (combined * vecs * 16 <= COMBINED_BYTES && a.n >= 16 * combined * 256) {
+            hipLaunchKernelGGL((embed_combined_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, COMBINED_BLOCKS)), dim3(COMBINED_THREADS),
+                               (combined + a.rows + 1) * vecs * 16 + FAR * 2, static_cast<hipStream_t>(stream), a, static_cast<int>(combined),
+                               static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
+            return;
+        }
         if (held <= TABLE_BYTES && a.n >= 4 * FAR) {
             hipLaunchKernelGGL((embed_table_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, TABLE_BLOCKS)), dim3(THREADS), held + a.fields * FAR * 2,
                                static_cast<hipStream_t>(stream), a, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
