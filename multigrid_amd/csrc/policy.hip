@@ -99,19 +99,23 @@ __device__ __forceinline__ void load_words(const T *p, int left, int length, uin
                 w[0] = static_cast<uint32_t>(to);
                 w[1] = static_cast<uint32_t>(to >> 32);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) w[i] = fills;
+        } else if constexpr (WORDS > 1) {  // a short row: its halves
             if (left > 0) {
+                uint32_t half[WORDS / 2], rest[WORDS / 2];
+                load_words<T, W / 2>(p, left, length, fill, half);
+                load_words<T, W / 2>(p + W / 2, left - W / 2, length, fill, rest);
 #pragma unroll
-                for (int i = 0; i < W; ++i)
-                    if (i < left) {
-                        if constexpr (BITS == 32)
-                            w[i] = reinterpret_cast<const uint32_t *>(p)[i];
-                        else
-                            w[i / 2] = (w[i / 2] & (i & 1 ? 0xFFFFu : 0xFFFF0000u)) | static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[i]) << (16 * (i & 1));
-                    }
+                for (int i = 0; i < WORDS / 2; ++i) {
+                    w[i] = half[i];
+                    w[WORDS / 2 + i] = rest[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) w[i] = fills;
             }
+        } else {  // one element of a word, or none
+            w[0] = fills;
+            if (left > 0) w[0] = BITS == 32 ? *reinterpret_cast<const uint32_t *>(p) : (fills & 0xFFFF0000u) | *reinterpret_cast<const uint16_t *>(p);
         }
     }
 }
@@ -126,7 +130,8 @@ __device__ __forceinline__ float element(const uint32_t *w, int i) {
 }
 
 // N vectors of a row, number j at first + (j * lanes + lane) * V; behind the row's k elements `fill`.  Only one thread's vector
-// can hold the row's end in part; it is loaded apart from the others, once.
+// can hold the row's end in part; it is loaded apart from the others, once.  V elements or more lie before that end (the row has more than
+// SHORT, and a piece of one begins behind others).
 template <class T, int N>
 __device__ __forceinline__ void load_vectors(const T *row, int k, int first, int lanes, int lane, uint32_t fill, uint32_t (&w)[N][4]) {
     constexpr int V = WIDE<T>;
@@ -146,7 +151,7 @@ __device__ __forceinline__ void load_vectors(const T *row, int k, int first, int
         const int v = (end - first) / V, j = v >> __builtin_ctz(lanes);  // (a power of two)
         if (j < N && v - j * lanes == lane) {
             uint32_t q[4];
-            load_words<T, V>(row + end, k - end, k, fill, q);
+            load_words<T, V>(row + end, k - end, V, fill, q);
 #pragma unroll
             for (int o = 0; o < N; ++o)
 #pragma unroll
@@ -174,14 +179,59 @@ __device__ __forceinline__ void load_part(const T *p, int left, int length, floa
     for (int i = 0; i < V; ++i) x[i] = element<T>(w, i);
 }
 
+// The first `left` of 16 bytes of elements: by halves, where they are not all of them.
+template <class T>
+__device__ __forceinline__ void store_words(T *p, int left, uint32_t (&w)[4]) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Four {
+        uint32_t w[4];
+    };
+    struct __attribute__((packed, aligned(sizeof(T)))) Two {
+        uint32_t w[2];
+    };
+    struct __attribute__((packed, aligned(sizeof(T)))) One {
+        uint32_t w;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("" : "+v"(w[i]));  // (else the elements that two ways have in common are stored by themselves)
+    constexpr int V = WIDE<T>;
+    char *to = reinterpret_cast<char *>(p);
+    if (left >= V) {
+        *reinterpret_cast<Four *>(to) = Four{{w[0], w[1], w[2], w[3]}};
+    } else if (left > 0) {
+        if (left & (V / 2)) {
+            *reinterpret_cast<Two *>(to) = Two{{w[0], w[1]}};
+            to += 8;
+            w[0] = w[2];
+            w[1] = w[3];
+        }
+        if (left & (V / 4)) {
+            reinterpret_cast<One *>(to)->w = w[0];
+            to += 4;
+            w[0] = w[1];
+        }
+        if (V == 8 && (left & 1)) *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(w[0]);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void pack(const float (&x)[WIDE<T>], uint32_t (&w)[4]) {
+    Vec<T, WIDE<T>> r;
+#pragma unroll
+    for (int i = 0; i < WIDE<T>; ++i) r.v[i] = static_cast<T>(x[i]);
+    __builtin_memcpy(w, &r, sizeof r);
+}
+
 template <class T, int V>
 __device__ __forceinline__ void store_part(T *p, int left, const float (&x)[V]) {
-    if (left >= V) {
-        store<T, V>(p, x);
-    } else {
+    static_assert(V % WIDE<T> == 0, "16 bytes, or several");
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < left) p[i] = static_cast<T>(x[i]);
+    for (int i = 0; i < V; i += WIDE<T>) {
+        float y[WIDE<T>];
+#pragma unroll
+        for (int j = 0; j < WIDE<T>; ++j) y[j] = x[i + j];
+        uint32_t w[4];
+        pack<T>(y, w);
+        store_words(p + i, left - i, w);
     }
 }
 
@@ -194,7 +244,8 @@ struct EmbedArgs {
     int32_t sizes[MG_MAX_FIELDS];
 };
 
-// One thread per 16 bytes of output; the threads of a token share its ids.
+// One thread per 16 bytes of output; the threads of a token share its ids.  (Four tokens to a thread at once: no faster where
+// there are many tokens, half as fast at 8190.)
 template <class T, class I>
 __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *ids, const T *table, T *out) {
     constexpr int V = WIDE<T>;
@@ -207,21 +258,28 @@ __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *id
         T *to = out + n * a.dim;
         for (int c = col; c < vecs; c += cols) {
             const int d0 = c * V;
-            float acc[V] = {};
-            int64_t base = 0;
-            for (int f = 0; f < a.fields; ++f) {
-                const int64_t id = static_cast<int64_t>(id_at[f * a.field_stride]);
-                if (id >= 0 && id < a.sizes[f]) {
-                    float x[V];
-                    load_part<T, V>(table + (base + id) * a.row_stride + d0, a.dim - d0, a.dim, x);
+            // get(one row's elements) for every row that the token reads
+            auto sum = [&](auto get) {
+                float acc[V] = {};
+                int64_t base = 0;
+                for (int f = 0; f < a.fields; ++f) {
+                    const int64_t id = static_cast<int64_t>(id_at[f * a.field_stride]);
+                    if (id >= 0 && id < a.sizes[f]) {
+                        float x[V];
+                        get(table + (base + id) * a.row_stride + d0, x);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) acc[i] += x[i];
+                        for (int i = 0; i < V; ++i) acc[i] += x[i];
+                    }
+                    base += a.sizes[f];
                 }
-                base += a.sizes[f];
-            }
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] *= a.scale;
-            store_part<T, V>(to + d0, a.dim - d0, acc);
+                for (int i = 0; i < V; ++i) acc[i] *= a.scale;
+                store_part<T, V>(to + d0, a.dim - d0, acc);
+            };
+            if (d0 + V <= a.dim)
+                sum([](const T *from, float (&x)[V]) { load<T, V>(from, x); });
+            else
+                sum([&](const T *from, float (&x)[V]) { load_part<T, V>(from, a.dim - d0, a.dim, x); });
         }
     }
 }
@@ -991,20 +1049,7 @@ __device__ __forceinline__ void load_row(const T *p, int k, float (&x)[K], uint3
 
 template <class T, int K>
 __device__ __forceinline__ void store_row(T *p, int k, const float (&x)[K]) {
-    constexpr int V = WIDE<T>;
-#pragma unroll
-    for (int i = 0; i < K; i += V) {
-        if (i + V <= k) {
-            float v[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = x[i + j];
-            store<T, V>(p + i, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (i + j < k) p[i + j] = static_cast<T>(x[i + j]);
-        }
-    }
+    store_part<T, K>(p, k, x);
 }
 
 // ---- longer rows ---------------------------------------------------------------------------------------------------
@@ -1142,7 +1187,7 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
         }
         float rep = 1.f, presence = 0.f, frequency = 0.f;
         if (live) {
-            rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
+            rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;  // (its reciprocal below: a division for a row, not for a token)
             presence = a.presence_dev ? a.presence_dev[row] : a.presence;
             frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
         }
@@ -1169,6 +1214,7 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
             __syncthreads();
         }
         if (live) {
+            const float inverse = 1.f / rep;
 #pragma unroll
             for (int j = 0; j < STRETCH; ++j) {
                 const int at = first + (j * lanes + lane) * V;
@@ -1202,9 +1248,9 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                     if (GRAD) {
                         const bool up = y[i] > 0.f;
                         y[i] = element<T>(g[j], i);
-                        if (c[i] > 0) y[i] = up ? y[i] / rep : y[i] * rep;
+                        if (c[i] > 0) y[i] = y[i] * (up ? inverse : rep);
                     } else {
-                        if (c[i] > 0) y[i] = (y[i] > 0.f ? y[i] / rep : y[i] * rep) - presence;
+                        if (c[i] > 0) y[i] = y[i] * (y[i] > 0.f ? inverse : rep) - presence;
                         y[i] = y[i] - frequency * static_cast<float>(c[i]);
                     }
                 }
@@ -1236,6 +1282,13 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
     }
 }
 
+__device__ __forceinline__ uint32_t four_bytes(const uint8_t *p) {
+    struct __attribute__((packed)) One {
+        uint32_t w;
+    };
+    return reinterpret_cast<const One *>(p)->w;
+}
+
 // Rows of few tokens: every thread counts its own row's history in its own LDS counters (an odd number of words apart, so that
 // lanes fall on different banks), which needs no barrier.
 template <class T, class H, bool GRAD, int K>
@@ -1250,15 +1303,39 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
     float x[K], g[K];
     load_row<T, K>(logits + row * a.logits_stride, a.k, x, 0);
     if (GRAD) load_row<T, K>(grad + row * a.grad_stride, a.k, g, 0);
+    const float rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
+    const float presence = a.presence_dev ? a.presence_dev[row] : a.presence;
+    const float frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
     uint32_t allow = ~0u;
     if (a.mask_kind == MG_MASK_BYTES) {
         const uint8_t *m = static_cast<const uint8_t *>(a.mask_dev) + row * a.mask_stride;
+        uint32_t w[K / 4];
+#pragma unroll
+        for (int j = 0; j < K; j += 4) {
+            w[j / 4] = 0;
+            if (j + 4 <= a.k)
+                w[j / 4] = four_bytes(m + j);
+            else if (j < a.k && a.k >= 4)
+                w[j / 4] = four_bytes(m + a.k - 4) >> (8 * (4 - (a.k - j)));
+            else
+                for (int i = j; i < a.k; ++i) w[j / 4] |= static_cast<uint32_t>(m[i]) << (8 * (i - j));
+        }
         allow = 0;
 #pragma unroll
         for (int j = 0; j < K; ++j)
-            if (j < a.k && m[j]) allow |= 1u << j;
+            if ((w[j / 4] >> (8 * (j % 4))) & 0xFF) allow |= 1u << j;
     } else if (a.mask_kind == MG_MASK_BITS) {
         allow = static_cast<const uint32_t *>(a.mask_dev)[row * a.mask_stride];
+    }
+    float bias[K];
+    if (!GRAD && a.bias_dev) {
+        if (a.bias_stride == 0) {  // the same for all rows: scalar loads
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+                if (j < a.k) bias[j] = a.bias_dev[j];
+        } else {
+            load_row<float, K>(a.bias_dev + row * a.bias_stride, a.k, bias, 0);
+        }
     }
     if (history) {
 #pragma unroll
@@ -1276,9 +1353,7 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
         for (; i < len; ++i)
             if (h[i] >= 0 && h[i] < static_cast<H>(a.k)) atomicAdd(&counts[h[i]], 1u);
     }
-    const float rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
-    const float presence = a.presence_dev ? a.presence_dev[row] : a.presence;
-    const float frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
+    const float inverse = 1.f / rep;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
         if (j >= a.k) continue;
@@ -1286,13 +1361,13 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
         const bool ok = (allow >> j) & 1;
         if (GRAD) {
             float v = g[j];
-            if (c > 0) v = x[j] > 0.f ? v / rep : v * rep;
+            if (c > 0) v = v * (x[j] > 0.f ? inverse : rep);
             x[j] = ok ? v : 0.f;
         } else {
             float v = x[j];
-            if (c > 0) v = (v > 0.f ? v / rep : v * rep) - presence;
+            if (c > 0) v = v * (v > 0.f ? inverse : rep) - presence;
             v = v - frequency * static_cast<float>(c);
-            if (a.bias_dev) v = v + a.bias_dev[row * a.bias_stride + j];
+            if (a.bias_dev) v = v + bias[j];
             x[j] = ok ? v : NEG_INF;
         }
     }

@@ -91,7 +91,8 @@ def per_row(v, n):
 
 
 def adjust(logits, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, mask=None):
-    """(values, bound, factor of the gradient): at most five operations, each off by half a step of what it gives."""
+    """(values, bound, factor of the gradient): at most six operations (1 / repetition, its product, presence, frequency times
+    c, that, bias), each off by half a step of what it gives."""
     x = np64(logits)
     n, k = x.shape
     c, r = history_counts(history, lengths, n, k), per_row(repetition, n)
@@ -102,7 +103,7 @@ def adjust(logits, history=None, lengths=None, repetition=1.0, presence=0.0, fre
         y = parts[0] + parts[1] + parts[2] + parts[3]
         size = sum(np.abs(p) for p in parts)
     ok = allowed(mask, n, k)
-    return np.where(ok, y, -np.inf), np.where(ok & np.isfinite(size), 5 * U32 * size, 0.0), np.where(ok, factor, 0.0)
+    return np.where(ok, y, -np.inf), np.where(ok & np.isfinite(size), 6 * U32 * size, 0.0), np.where(ok, factor, 0.0)
 
 
 def draw(logits, uniforms, temperature=1.0):
