@@ -466,7 +466,7 @@ __device__ __forceinline__ uint32_t row_of(Id id, uint32_t base, uint32_t size, 
 //
 // 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
 // again, one after the other, each added to its own rows only.
-constexpr int FEW = 64, FEW_BLOCKS = 768;  // three to a compute unit, two where a lane loads 8 bytes
+constexpr int FEW = 64, FEW_BLOCKS = 768;  // three to a compute unit, two where a lane takes four columns
 constexpr int64_t FAR_ROWS = 1 << 24;       // a stride up to which 64 tokens lie within 32-bit offsets, and dim's limit
 
 template <class T>
@@ -496,7 +496,7 @@ union Fragment {
 };
 
 template <class T, int W, int TILES>
-__global__ __launch_bounds__(THREADS, TILES > 2 || W * sizeof(T) > 4 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
+__global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
     constexpr int COLS = 16 * W, WORDS = (W * sizeof(T) + 3) / 4;
     __shared__ __align__(16) uint16_t rows_s[THREADS / 64][MG_MAX_FIELDS][64];  // 0xFFFF: none
     __shared__ float sum_s[TILES * 16][COLS];
@@ -1192,24 +1192,31 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
             frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
         }
         if (history) {
+            // the first entries before their number is known: they lie there whatever it is
+            constexpr int AHEAD = 8;
+            const H *h = static_cast<const H *>(a.history_dev) + (live ? row : 0) * a.history_stride;
+            H entry[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) entry[u] = h[min(lane + u * lanes, a.t - 1)];
             const int len = !live ? 0 : (a.lengths_dev ? min(max(a.lengths_dev[row], 0), a.t) : a.t);
-            const H *h = static_cast<const H *>(a.history_dev) + row * a.history_stride;
 #pragma unroll
             for (int j = 0; j < STRETCH; ++j)
 #pragma unroll
                 for (int i = 0; i < V; i += 4) *reinterpret_cast<uint4 *>(&counts[(j * lanes + lane) * V + i]) = make_uint4(0, 0, 0, 0);
             __syncthreads();
             const int end = min(width, a.k - first);
-            constexpr int AHEAD = 8;
-            for (int i = lane; i < len; i += AHEAD * lanes) {
-                H entry[AHEAD];
-#pragma unroll
-                for (int u = 0; u < AHEAD; ++u) entry[u] = h[min(i + u * lanes, len - 1)];
+            auto count = [&](int i, const H (&entry)[AHEAD]) {
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
                     const int64_t j = static_cast<int64_t>(entry[u]) - first;
                     if (i + u * lanes < len && j >= 0 && j < end) atomicAdd(&counts[j], 1u);
                 }
+            };
+            count(lane, entry);
+            for (int i = lane + AHEAD * lanes; i < len; i += AHEAD * lanes) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) entry[u] = h[min(i + u * lanes, len - 1)];
+                count(i, entry);
             }
             __syncthreads();
         }
@@ -1656,87 +1663,66 @@ __global__ __launch_bounds__(PIECE_LANES) void draw_pieces_kernel(MgLogits l, co
     }
 }
 
-// One block to a row: the pieces' totals, the piece in which the border lies, the token in that piece.
+// One block to a row: the pieces' totals, the piece in which the border lies, the token in that piece.  Every wave goes through
+// the pieces by itself, a run of adjacent ones to each lane, and comes to the same.
 template <class T>
 __global__ __launch_bounds__(PIECE_LANES) void draw_join_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type, const DrawPiece *pieces,
                                                                 int count, void *tokens, float *logprob) {
     __shared__ DrawShared sh;
-    __shared__ double upto_s[PIECE_LANES], before_s;
-    __shared__ int piece_s;
-    const int tid = threadIdx.x;
+    const int lane = threadIdx.x % 64, run = (count + 63) / 64, lo = min(lane * run, count), hi = min(lo + run, count);
     for (int64_t i = blockIdx.x; i < l.n; i += gridDim.x) {
         const DrawPiece *of = pieces + i * count;
+        const double u = uniforms ? uniform_at(uniforms, uniforms_type, i) : 0.0;
         float m = NEG_INF;
-        for (int p = tid; p < count; p += PIECE_LANES) m = larger(m, of[p].m);
-        m = over_row<PIECE_LANES>(m, sh.most, larger);
+        for (int p = lo; p < hi; ++p) m = larger(m, of[p].m);
+        m = over_row<64>(m, sh.most, larger);
         if (!(fabsf(m) < -NEG_INF)) {
-            if (tid == 0) put_drawn(l, i, -1, m, 0.f, tokens, logprob);
-            __syncthreads();
+            if (threadIdx.x == 0) put_drawn(l, i, -1, m, 0.f, tokens, logprob);
             continue;
         }
         const Spread s = spread(l, i, m);
         auto total_of = [&](int p) { return of[p].m == NEG_INF ? 0.0 : of[p].total * exp2_64((static_cast<double>(of[p].m) - s.m) * s.c); };
-        // a run of adjacent pieces to each thread
-        const int run = (count + PIECE_LANES - 1) / PIECE_LANES, lo = min(tid * run, count), hi = min(lo + run, count);
         double mine = 0.0;
         for (int p = lo; p < hi; ++p) mine += total_of(p);
-        upto_s[tid] = mine;
-        if (tid == 0) piece_s = uniforms ? -1 : 0x7FFFFFFF;
-        __syncthreads();
-        for (int by = 1; by < PIECE_LANES; by *= 2) {
-            const double o = tid >= by ? upto_s[tid - by] : 0.0;
-            __syncthreads();
-            upto_s[tid] += o;
-            __syncthreads();
+        double end = mine;
+#pragma unroll
+        for (int by = 1; by < 64; by *= 2) {
+            const double o = __shfl_up(end, by, 64);
+            if (lane >= by) end += o;
         }
-        const double total = upto_s[PIECE_LANES - 1];
-        double border = 0.0;
+        const double total = read_lane(end, 63), border = u * total;
+        // the lane whose pieces hold the border (rounding may leave none: the last one that has any), or the largest logit
+        int piece = -1;
+        double before = lane ? end - mine : 0.0;
+        uint64_t there;
         if (uniforms) {
-            border = uniform_at(uniforms, uniforms_type, i) * total;
-            // the first piece whose sum passes the border; where rounding leaves none, the last one that has any
-            double sum = tid ? upto_s[tid - 1] : 0.0;
-            int last = -1, found = -1;
-            double start = 0.0, start_last = 0.0;
-            for (int p = lo; p < hi && found < 0; ++p) {
+            const uint64_t above = __ballot(end > border && mine > 0.0), some = __ballot(mine > 0.0);
+            there = above ? above & -above : 1ull << (63 - __builtin_clzll(some));
+            double sum = before;
+            bool done = false;
+            for (int p = lo; p < hi && !done; ++p) {
                 const double t = total_of(p);
                 if (t > 0.0) {
-                    last = p;
-                    start_last = sum;
-                }
-                if (sum + t > border) {
-                    found = p;
-                    start = sum;
+                    piece = p;
+                    before = sum;
                 }
                 sum += t;
-            }
-            const bool has = found >= 0;
-            if (has) last = -1;
-            // sums grow from thread to thread, so the first thread that found one has the piece
-            if (tid == 0) sh.token = PIECE_LANES;
-            __syncthreads();
-            if (has) atomicMin(&sh.token, tid);
-            if (last >= 0) atomicMax(&piece_s, last);
-            __syncthreads();
-            const int from = sh.token;
-            const int of_last = piece_s;
-            __syncthreads();
-            if (from < PIECE_LANES ? tid == from : last == of_last) {
-                piece_s = from < PIECE_LANES ? found : last;
-                before_s = from < PIECE_LANES ? start : start_last;
+                done = sum > border;
             }
         } else {
-            for (int p = lo; p < hi; ++p)
-                if (of[p].m == m) {
-                    atomicMin(&piece_s, p);
-                    break;
-                }
+            for (int p = hi - 1; p >= lo; --p)
+                if (of[p].m == m) piece = p;
+            const uint64_t has = __ballot(piece >= 0);
+            there = has & -has;
         }
-        __syncthreads();
-        const int first = piece_s * PIECE<T>;
-        Row<T, PIECE_LANES, PIECE_HELD> row(logits + i * l.stride + first, min(PIECE<T>, l.k - first), tid);
+        const int from = __builtin_ctzll(there);
+        piece = __shfl(piece, from, 64);
+        before = __shfl(before, from, 64);
+        const int first = piece * PIECE<T>;
+        Row<T, PIECE_LANES, PIECE_HELD> row(logits + i * l.stride + first, min(PIECE<T>, l.k - first), threadIdx.x);
         double unused;
-        const int token = first + (uniforms ? find_border(row, sh, s, false, border, before_s, unused) : find_largest(row, sh, s, m, unused));
-        if (tid == 0) put_drawn(l, i, token, m, logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
+        const int token = first + (uniforms ? find_border(row, sh, s, false, border, before, unused) : find_largest(row, sh, s, m, unused));
+        if (threadIdx.x == 0) put_drawn(l, i, token, m, logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
         __syncthreads();
     }
 }
@@ -2143,7 +2129,7 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
         while (p.width > 1 && (16 * (p.width / 2) >= a.dim || p.width > a.dim)) p.width /= 2;
         p.tiles = a.rows <= 16 ? 1 : (a.rows <= 32 ? 2 : 4);
         const int64_t blocks = (a.n + THREADS - 1) / THREADS;
-        const int64_t slabs = (a.dim + 16 * p.width - 1) / (16 * p.width), all = p.width * 2 == wide ? FEW_BLOCKS * 2 / 3 : FEW_BLOCKS,
+        const int64_t slabs = (a.dim + 16 * p.width - 1) / (16 * p.width), all = p.width > 2 ? FEW_BLOCKS * 2 / 3 : FEW_BLOCKS,
                       most = slabs < all / 64 ? all / slabs : 64;
         p.blocks = static_cast<int>(blocks < 1 ? 1 : (blocks < most ? blocks : most));
         if (p.blocks > 1) take(static_cast<int64_t>(p.blocks) * a.rows * a.dim * 4);
