@@ -325,7 +325,7 @@ int mg_episode_stats(int32_t num_envs, int32_t num_agents, const float *reward_d
 typedef struct MgEmbed {
     int64_t n;                    /* tokens; n * fields 0 .. 2^31 - 1 */
     int32_t fields;               /* 1 .. MG_MAX_FIELDS */
-    int32_t dim;                  /* 1 .. 2^24 */
+    int32_t dim;                  /* 1 .. 2^20 */
     int32_t ids_type;             /* MG_U8, MG_I32, MG_I64 */
     int32_t dtype;                /* of table, output and gradients: MG_F32, MG_BF16, MG_F16 */
     int64_t ids_stride;           /* elements from one token's ids to the next one's; 0 allowed */
@@ -393,15 +393,16 @@ typedef struct MgLogits {
     int32_t k;                     /* tokens, 1 .. 2^24 */
     int32_t dtype;                 /* MG_F32, MG_BF16, MG_F16 */
     int64_t stride;                /* elements between rows */
-    const float *temperature_dev;  /* [n], NULL: the number below; positive and finite */
+    const float *temperature_dev;  /* [n], NULL: the number below; at least 2^-126 and finite */
     float temperature;
     int32_t tokens_type;           /* MG_U8 (k at most 255), MG_I32, MG_I64 */
 } MgLogits;
 
 /* Draws one token of every row: the lowest j whose p_0 + ... + p_j exceeds uniforms[i] (in [0, 1), `uniforms_type`
  * MG_F32 or MG_F64), decided in 64 bits; uniforms_dev NULL: the lowest j of the largest logit.  logprob[i] (may be NULL)
- * = log p of that token, as mg_token_logprobs gives it but for roundings.  A row that is no distribution (all -inf, or a NaN or +inf in it) gives token -1
- * (255 as MG_U8, which mg_step takes for no action at all) and log-probability -inf (all -inf) or NaN.
+ * = log p of that token, as mg_token_logprobs gives it but for roundings.  A row that is no distribution (all -inf, or a NaN
+ * or +inf in it, or a number of temperature_dev that is no temperature) gives token -1 (255 as MG_U8, which mg_step takes
+ * for no action at all) and log-probability -inf (all -inf) or NaN.
  * `workspace_dev`: mg_draw_workspace(l) bytes, 16-byte aligned (NULL where that is 0). */
 int64_t mg_draw_workspace(const MgLogits *l);
 int mg_draw(const MgLogits *l, const void *logits_dev, const void *uniforms_dev, int32_t uniforms_type, void *tokens_dev,

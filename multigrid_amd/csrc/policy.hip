@@ -25,6 +25,7 @@ using ushort2_t = unsigned short __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 256;
 constexpr float NEG_INF = -__builtin_inff();
+constexpr float LEAST_TEMPERATURE = 0x1p-126f;  // its reciprocal is finite
 
 // V elements at any element's alignment: global loads and stores of gfx950 take 16 bytes at any address
 template <class T, int V>
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, const
 
 // The same where LDS holds the finished output of every combination of a token's ids, none included (cells: 12 x 7 x 8): worked
 // out once a block, then each 16 bytes of output are one read of LDS and one store.
-constexpr int COMBINED_BYTES = 49152, COMBINED_THREADS = 512, COMBINED_BLOCKS = 768;  // three blocks to a compute unit
+constexpr int COMBINED_BYTES = 53248, COMBINED_THREADS = 512, COMBINED_BLOCKS = 768;  // three blocks to a compute unit
 static_assert(FAR == COMBINED_THREADS, "a token's ids to each thread");
 
 template <class T, class I>
@@ -467,7 +468,7 @@ __device__ __forceinline__ uint32_t row_of(Id id, uint32_t base, uint32_t size, 
 // 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
 // again, one after the other, each added to its own rows only.
 constexpr int FEW = 64, FEW_BLOCKS = 768;  // three to a compute unit, two where a lane takes four columns
-constexpr int64_t FAR_ROWS = 1 << 24;       // a stride up to which 64 tokens lie within 32-bit offsets, and dim's limit
+constexpr int64_t FAR_ROWS = 1 << 24;       // a stride up to which 64 tokens lie within 32-bit offsets
 
 template <class T>
 struct Operand {
@@ -1418,6 +1419,12 @@ __device__ __forceinline__ double exp2_64(double t) {
     return ldexp(p, static_cast<int>(n));
 }
 
+// Of a row: a number on the device cannot be refused, one that is no temperature makes the row none that can be drawn from.
+__device__ __forceinline__ float temperature_of(const MgLogits &l, int64_t row) {
+    const float t = l.temperature_dev ? l.temperature_dev[row] : l.temperature;
+    return t >= LEAST_TEMPERATURE && t < -NEG_INF ? t : __builtin_nanf("");
+}
+
 // A row as a distribution: its largest logit and log2(e) / temperature.
 struct Spread {
     double m, c;
@@ -1431,11 +1438,14 @@ struct Spread {
     }
 };
 __device__ __forceinline__ Spread spread(const MgLogits &l, int64_t row, float m) {
-    return Spread{m, 1.4426950408889634 / static_cast<double>(l.temperature_dev ? l.temperature_dev[row] : l.temperature)};
+    return Spread{m, 1.4426950408889634 / static_cast<double>(temperature_of(l, row))};
 }
+__device__ __forceinline__ bool drawable(float m, const Spread &s) { return fabsf(m) < -NEG_INF && s.c == s.c; }
 
+// (outside of [0, 1] it is the nearest end, NaN the lower one)
 __device__ __forceinline__ double uniform_at(const void *uniforms, int type, int64_t row) {
-    return type == MG_F64 ? static_cast<const double *>(uniforms)[row] : static_cast<double>(static_cast<const float *>(uniforms)[row]);
+    const double u = type == MG_F64 ? static_cast<const double *>(uniforms)[row] : static_cast<double>(static_cast<const float *>(uniforms)[row]);
+    return fmin(fmax(u, 0.0), 1.0);
 }
 
 // log p of a token from its logit; total - 1 is exact where little stands beside the maximum
@@ -1499,7 +1509,7 @@ __device__ __forceinline__ int find_border(Row<T, LANES, HELD> &row, DrawShared 
         int found = N;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            if (found == N && sum + own[i] > border && lane * EACH + i < N) {
+            if (found == N && own[i] > 0.0 && sum + own[i] > border) {  // (own: rounding may put the sum of one that has none above the last one's)
                 found = lane * EACH + i;
                 start = sum;
             }
@@ -1525,7 +1535,7 @@ __device__ __forceinline__ int find_border(Row<T, LANES, HELD> &row, DrawShared 
         double sum = before;
 #pragma unroll
         for (int j = 0; j < HELD; ++j) {
-            if (vec < 0 && sum + sums[j] > border) {
+            if (vec < 0 && sums[j] > 0.0 && sum + sums[j] > border) {
                 vec = j;
                 before = sum;
             }
@@ -1540,7 +1550,7 @@ __device__ __forceinline__ int find_border(Row<T, LANES, HELD> &row, DrawShared 
         const double here = s.of_vector<T>(v), end = before + upto(here);
         const int shift = (threadIdx.x % 64) / SPAN * SPAN;
         const uint64_t threads = (~0ull >> (64 - SPAN)) << shift;
-        const uint64_t above = __ballot(end > border) & threads, some = __ballot(here > 0.0) & threads;
+        const uint64_t above = __ballot(end > border && here > 0.0) & threads, some = __ballot(here > 0.0) & threads;
         // rounding may leave none above it: the last one that has any then
         const int at = (above ? __builtin_ctzll(above) : (some ? 63 - __builtin_clzll(some) : shift)) - shift;
         if ((lane & (SPAN - 1)) == at) {
@@ -1614,9 +1624,9 @@ __device__ __forceinline__ float largest(Row<T, LANES, HELD> &row, float *shared
     return over_row<LANES>(m, shared, larger);
 }
 
-__device__ __forceinline__ void put_drawn(const MgLogits &l, int64_t row, int token, float m, float lp, void *tokens, float *logprob) {
+__device__ __forceinline__ void put_drawn(const MgLogits &l, int64_t row, int token, float m, const Spread &s, float lp, void *tokens, float *logprob) {
     put_token(tokens, l.tokens_type, row, token);
-    if (logprob) logprob[row] = token >= 0 ? lp : (m == NEG_INF ? NEG_INF : __builtin_nanf(""));
+    if (logprob) logprob[row] = token >= 0 ? lp : (m == NEG_INF && s.c == s.c ? NEG_INF : __builtin_nanf(""));
 }
 
 template <class T, int LANES, int HELD>
@@ -1632,8 +1642,8 @@ __global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T 
         const Spread s = spread(l, i, m);
         int token = -1;
         double total = 0.0;
-        if (fabsf(m) < -NEG_INF) token = uniforms ? find_border(row, sh, s, true, u, 0.0, total) : find_largest(row, sh, s, m, total);
-        if (lane == 0) put_drawn(l, i, token, m, token >= 0 && logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
+        if (drawable(m, s)) token = uniforms ? find_border(row, sh, s, true, u, 0.0, total) : find_largest(row, sh, s, m, total);
+        if (lane == 0) put_drawn(l, i, token, m, s, token >= 0 && logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
         if (LANES > 64 && i + step < l.n) __syncthreads();  // the shared values are read
     }
 }
@@ -1676,11 +1686,11 @@ __global__ __launch_bounds__(PIECE_LANES) void draw_join_kernel(MgLogits l, cons
         float m = NEG_INF;
         for (int p = lo; p < hi; ++p) m = larger(m, of[p].m);
         m = over_row<64>(m, sh.most, larger);
-        if (!(fabsf(m) < -NEG_INF)) {
-            if (threadIdx.x == 0) put_drawn(l, i, -1, m, 0.f, tokens, logprob);
+        const Spread s = spread(l, i, m);
+        if (!drawable(m, s)) {
+            if (threadIdx.x == 0) put_drawn(l, i, -1, m, s, 0.f, tokens, logprob);
             continue;
         }
-        const Spread s = spread(l, i, m);
         auto total_of = [&](int p) { return of[p].m == NEG_INF ? 0.0 : of[p].total * exp2_64((static_cast<double>(of[p].m) - s.m) * s.c); };
         double mine = 0.0;
         for (int p = lo; p < hi; ++p) mine += total_of(p);
@@ -1722,7 +1732,7 @@ __global__ __launch_bounds__(PIECE_LANES) void draw_join_kernel(MgLogits l, cons
         Row<T, PIECE_LANES, PIECE_HELD> row(logits + i * l.stride + first, min(PIECE<T>, l.k - first), threadIdx.x);
         double unused;
         const int token = first + (uniforms ? find_border(row, sh, s, false, border, before, unused) : find_largest(row, sh, s, m, unused));
-        if (threadIdx.x == 0) put_drawn(l, i, token, m, logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
+        if (threadIdx.x == 0) put_drawn(l, i, token, m, s, logprob ? drawn_logprob(static_cast<float>(logits[i * l.stride + token]), s, total) : 0.f, tokens, logprob);
         __syncthreads();
     }
 }
@@ -1742,7 +1752,7 @@ __global__ __launch_bounds__(THREADS) void draw_short_kernel(MgLogits l, const T
     const Spread s = spread(l, row, m);
     int token = -1;
     float lp = 0.f;
-    if (fabsf(m) < -NEG_INF) {
+    if (drawable(m, s)) {
         // what is filled up behind the last token is -inf, so 0
         constexpr bool KEEP = K <= 16;
         double p[KEEP ? K : 1], total = 0.0;
@@ -1776,7 +1786,7 @@ __global__ __launch_bounds__(THREADS) void draw_short_kernel(MgLogits l, const T
         }
         if (logprob) lp = drawn_logprob(at, s, total);
     }
-    put_drawn(l, row, token, m, lp, tokens, logprob);
+    put_drawn(l, row, token, m, s, lp, tokens, logprob);
 }
 
 // ---- log-probabilities and entropies -------------------------------------------------------------------------------
@@ -1858,6 +1868,7 @@ __device__ __forceinline__ Soft soft_of(Row<T, LANES, HELD> &row, SoftShared &sh
     const auto both = [](float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); };
     const float c = inv_t * HALF_LOG2E;
     Soft s{largest(row, sh.most), -1.f, 0.f};
+    if (inv_t != inv_t) s.m = inv_t;  // no temperature: NaN throughout
     if (s.m > NEG_INF && s.m < -NEG_INF) {
         float sum = 0.f, slant = 0.f;
         row.each([&](int, const uint32_t *v) {
@@ -1900,7 +1911,7 @@ __global__ __launch_bounds__(BLOCK<LANES>) void logprob_kernel(MgLogits l, const
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * ROWS + sub; i < l.n; i += step) {
         Row<T, LANES, HELD> row(logits + i * l.stride, l.k, lane);
         const Taken t = taken(l, logits + i * l.stride, i, tokens, logprob != nullptr);
-        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature);
+        const float inv_t = 1.f / temperature_of(l, i);
         const Soft s = soft_of(row, sh, inv_t);
         if (lane == 0) row_result(i, s, inv_t, t, logprob, entropy, stats);
         if (LANES > 64 && i + step < l.n) __syncthreads();  // the shared values are read
@@ -1914,7 +1925,7 @@ __global__ __launch_bounds__(PIECE_LANES) void logprob_pieces_kernel(MgLogits l,
     const int first = blockIdx.x * PIECE<T>;
     for (int64_t i = blockIdx.y; i < l.n; i += gridDim.y) {
         Row<T, PIECE_LANES, PIECE_HELD> row(logits + i * l.stride + first, min(PIECE<T>, l.k - first), threadIdx.x);
-        const Soft s = soft_of(row, sh, 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature));
+        const Soft s = soft_of(row, sh, 1.f / temperature_of(l, i));
         if (threadIdx.x == 0) pieces[i * gridDim.x + blockIdx.x] = make_float4(s.m, s.r, s.t, 0.f);
         __syncthreads();
     }
@@ -1925,7 +1936,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(MgLogits l, const T *l
                                                           float *entropy, float *stats) {
     for (int64_t i = blockIdx.x; i < l.n; i += gridDim.x) {
         const Taken t = taken(l, logits + i * l.stride, i, tokens, logprob != nullptr);
-        const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[i] : l.temperature);
+        const float inv_t = 1.f / temperature_of(l, i);
         Soft s{NEG_INF, -1.f, 0.f};
         for (int p = threadIdx.x; p < count; p += 64) {
             const float4 q = pieces[i * count + p];
@@ -1957,7 +1968,7 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int l
         uint32_t w[TAKES][4];
         load_vectors<T, TAKES>(x, l.k, first, lanes, lane, NEG_INF_BITS<T>, w);
         // (none of these waits for another)
-        const float temperature = l.temperature_dev ? l.temperature_dev[row] : l.temperature;
+        const float temperature = temperature_of(l, row);
         const float4 st = reinterpret_cast<const float4 *>(stats)[row];
         const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
         const float grad_of_lp = grad_lp ? grad_lp[row * lp_stride] : 0.f, grad_of_h = grad_h ? grad_h[row * h_stride] : 0.f;
@@ -1971,8 +1982,8 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int l
             float v[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float lp = fmaxf((element<T>(w[j], i) - st.x) * inv_t - st.y, 2.f * DEEP), p = exp_twice(lp * HALF_LOG2E);
-                v[i] = -p * fmaf(h, lp, whole);
+                const float at_i = element<T>(w[j], i), lp = fmaxf((at_i - st.x) * inv_t - st.y, 2.f * DEEP), p = exp_twice(lp * HALF_LOG2E);
+                v[i] = at_i == NEG_INF ? 0.f : -p * fmaf(h, lp, whole);
             }
             if (token >= at && token < at + V) {
                 const float own = logprob_slope(static_cast<float>(x[token]), true, st, inv_t, g, h);
@@ -1992,6 +2003,7 @@ __device__ __forceinline__ Soft soft_short(const float (&x)[K], int k, float inv
     float m = x[0];
 #pragma unroll
     for (int j = 1; j < K; ++j) m = __builtin_elementwise_maximum(m, x[j]);  // NaN if one is there
+    if (inv_t != inv_t) m = inv_t;  // no temperature: NaN throughout
     Soft s{m, m == NEG_INF ? -1.f : 0.f, 0.f};
     bool passed = m == NEG_INF;
 #pragma unroll
@@ -2016,7 +2028,7 @@ __global__ __launch_bounds__(THREADS) void logprob_short_kernel(MgLogits l, cons
     float x[K];
     load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF_BITS<T>);
     const Taken t = taken(l, logits + row * l.stride, row, tokens, logprob != nullptr);
-    const float inv_t = 1.f / (l.temperature_dev ? l.temperature_dev[row] : l.temperature);
+    const float inv_t = 1.f / temperature_of(l, row);
     row_result(row, soft_short<K>(x, l.k, inv_t), inv_t, t, logprob, entropy, stats);
 }
 
@@ -2027,7 +2039,7 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_short_kernel(MgLogits l,
     if (row >= l.n) return;
     float x[K];
     load_row<T, K>(logits + row * l.stride, l.k, x, NEG_INF_BITS<T>);
-    const float temperature = l.temperature_dev ? l.temperature_dev[row] : l.temperature;
+    const float temperature = temperature_of(l, row);
     const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
     const float grad_of_lp = grad_lp ? grad_lp[row * lp_stride] : 0.f, grad_of_h = grad_h ? grad_h[row * h_stride] : 0.f;
     const float inv_t = 1.f / temperature, g = token >= 0 && token < l.k ? grad_of_lp * inv_t : 0.f, h = grad_of_h * inv_t;
@@ -2050,7 +2062,7 @@ int launched(const char *who) {
 unsigned blocks_for(int64_t items, int64_t most = 1 << 20) { return static_cast<unsigned>(items < most ? items : most); }
 
 constexpr int64_t MOST_ROWS = (1ll << 31) - 1;
-constexpr int32_t MOST_TOKENS = 1 << 24;
+constexpr int32_t MOST_TOKENS = 1 << 24, MOST_COLUMNS = 1 << 20;  // (a grid's second dimension ends at 65535: 2^20 columns in blocks of 32)
 
 bool workspace_ok(const char *who, const void *workspace, int64_t bytes, int64_t need) {
     if (need == 0 || (workspace && bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0)) return true;
@@ -2065,7 +2077,7 @@ int embed_args(const char *who, const MgEmbed *e, EmbedArgs *a) {
     if (!e) return refuse(MG_EINVAL, "%s: null argument", who);
     if (e->n < 0 || e->n > MOST_ROWS) return refuse(MG_EINVAL, "%s: n %lld not supported (0..2^31 - 1)", who, static_cast<long long>(e->n));
     if (e->fields < 1 || e->fields > MG_MAX_FIELDS) return refuse(MG_EINVAL, "%s: %d fields not supported (1..%d)", who, e->fields, MG_MAX_FIELDS);
-    if (e->dim < 1 || e->dim > MOST_TOKENS) return refuse(MG_EINVAL, "%s: dim %d not supported (1..2^24)", who, e->dim);
+    if (e->dim < 1 || e->dim > MOST_COLUMNS) return refuse(MG_EINVAL, "%s: dim %d not supported (1..2^20)", who, e->dim);
     if (!int_ok(e->ids_type)) return refuse(MG_EINVAL, "%s: unknown type %d of the ids", who, e->ids_type);
     if (!dtype_ok(e->dtype)) return refuse(MG_EINVAL, "%s: unknown element type %d", who, e->dtype);
     if (e->ids_stride < 0 || e->field_stride < 0 || e->row_stride < 0) return refuse(MG_EINVAL, "%s: negative stride", who);
@@ -2323,8 +2335,8 @@ int logits_args(const char *who, const MgLogits *l) {
     if (!int_ok(l->tokens_type) || (l->tokens_type == MG_U8 && l->k > 255))
         return refuse(MG_EINVAL, "%s: tokens of type %d not supported for k = %d", who, l->tokens_type, l->k);
     if (l->stride < 0) return refuse(MG_EINVAL, "%s: negative stride", who);
-    if (!l->temperature_dev && !(l->temperature > 0.f && l->temperature < __builtin_inff()))
-        return refuse(MG_EINVAL, "%s: temperature must be positive and finite", who);
+    if (!l->temperature_dev && !(l->temperature >= LEAST_TEMPERATURE && l->temperature < __builtin_inff()))
+        return refuse(MG_EINVAL, "%s: temperature must be at least 2^-126 and finite", who);
     return MG_OK;
 }
 
@@ -2346,9 +2358,10 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
         // for a table alone
         int64_t combined = 1;
         for (int f = 0; f < a.fields; ++f) combined = combined * (a.sizes[f] + 1) <= (1 << 15) ? combined * (a.sizes[f] + 1) : 1 << 15;
-        if (combined * vecs * 16 <= COMBINED_BYTES && a.n >= 16 * combined * 256) {
+        const int64_t combined_bytes = (combined + a.rows + 1) * vecs * 16 + FAR * 2;
+        if (combined_bytes <= COMBINED_BYTES && a.n >= 16 * combined * 256) {
             hipLaunchKernelGGL((embed_combined_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, COMBINED_BLOCKS)), dim3(COMBINED_THREADS),
-                               (combined + a.rows + 1) * vecs * 16 + FAR * 2, static_cast<hipStream_t>(stream), a, static_cast<int>(combined),
+                               combined_bytes, static_cast<hipStream_t>(stream), a, static_cast<int>(combined),
                                static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
             return;
         }

@@ -9,10 +9,12 @@
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
 #include <variant>
 #include <vector>
 
@@ -90,6 +92,32 @@ int whole(const char *name, at::ScalarType t) {
 
 bool wants_grad(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+void no_gradient(const char *name, const Maybe &t, const char *instead) { TORCH_CHECK_VALUE(!t || !wants_grad(*t), name, " passes no gradient: ", instead); }
+void no_gradient(const char *name, const Number &v) {
+    if (const Tensor *t = std::get_if<Tensor>(&v)) no_gradient(name, Maybe(*t), "detach it");
+}
+
+// Before a differentiable call of `t`, while a stream is captured: a leaf's gradient is accumulated on the stream that was
+// current when the first graph that holds the leaf was built.  Where that is the default stream, the captured backward pass
+// would order work behind it, which no capture allows and no one catches.
+void no_leaf_of_the_default_stream(const Tensor &t) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(t.device().index()).stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    std::vector<std::shared_ptr<torch::autograd::Node>> rest;
+    std::unordered_set<torch::autograd::Node *> seen;
+    if (auto first = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t)) rest.push_back(std::move(first));
+    while (!rest.empty()) {
+        const auto node = std::move(rest.back());
+        rest.pop_back();
+        if (!seen.insert(node.get()).second) continue;
+        const auto stream = node->stream();
+        TORCH_CHECK(!stream || stream->id() != 0, "a differentiable call is captured, but what it depends on belongs to an eager graph of the default stream as well (", node->name(),
+                    "): let that graph go first (del its outputs), or build it on another stream");
+        for (const auto &edge : node->next_edges())
+            if (edge.function) rest.push_back(edge.function);
+    }
+}
+
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the operators of multigrid_amd.policy are differentiable once (create_graph is not supported)"); }
 
 // [..., k] as [n, k] with adjacent elements in a row; a view wherever there is one
@@ -124,7 +152,7 @@ Lookup lookup(const Tensor &ids, const Fields &fields, int64_t rows, int64_t dim
     Lookup l;
     MgEmbed &e = l.e;
     int64_t count = 1;
-    TORCH_CHECK_VALUE(rows <= (1 << 30) && dim <= (1 << 24), "a table of ", rows, " x ", dim, " is not supported");
+    TORCH_CHECK_VALUE(rows <= (1 << 30) && dim <= (1 << 20), "a table of ", rows, " x ", dim, " is not supported");
     if (!fields) {
         l.shape = ids.sizes().vec();
         e.sizes[0] = static_cast<int32_t>(rows);
@@ -204,7 +232,9 @@ Tensor embed(const Tensor &ids, const Tensor &table, const Fields &fields, doubl
     on_gpu("table", table);
     beside("ids", ids, table);
     TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) && table.size(1), "table must be [rows, dim] and hold something, got ", table.sizes());
-    return wants_grad(table) ? Embed::apply(ids, table, fields, scale) : embed_forward(ids, table, fields, scale);
+    if (!wants_grad(table)) return embed_forward(ids, table, fields, scale);
+    no_leaf_of_the_default_stream(table);
+    return Embed::apply(ids, table, fields, scale);
 }
 
 // ---- adjustment of logits
@@ -220,7 +250,6 @@ std::pair<Tensor, float> per_row(const char *name, const Number &v, const Tensor
     if (const double *d = std::get_if<double>(&v)) return {Tensor(), static_cast<float>(*d)};
     Tensor t = std::get<Tensor>(v);
     beside(name, t, logits);
-    TORCH_CHECK_VALUE(!wants_grad(t), name, " passes no gradient: detach it");
     const auto lead = lead_of(logits);
     if (t.dim() == 0) t = t.expand(lead);
     TORCH_CHECK_VALUE(t.sizes() == lead, name, " must be a number or of shape ", lead, ", got ", t.sizes());
@@ -237,6 +266,17 @@ Tensor table_of(const char *name, const Tensor &t, const Tensor &logits, int64_t
     return width ? rows_of(t) : t;
 }
 int64_t table_stride(const Tensor &t) { return t.dim() == 1 || t.size(0) <= 1 ? 0 : t.stride(0); }
+
+// whether two tensors may share memory, by their first and last element
+bool overlap(const Tensor &a, const Tensor &b) {
+    if (!a.numel() || !b.numel()) return false;
+    auto end = [](const Tensor &t) {
+        int64_t last = 1;
+        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+        return static_cast<const char *>(t.data_ptr()) + last * t.element_size();
+    };
+    return static_cast<const char *>(a.data_ptr()) < end(b) && static_cast<const char *>(b.data_ptr()) < end(a);
+}
 
 struct Adjustment {
     MgAdjust a{};
@@ -286,7 +326,6 @@ Adjustment adjustment(const Tensor &logits, const Maybe &history, const Maybe &l
     row("presence", presence, a.presence_dev, a.presence);
     row("frequency", frequency, a.frequency_dev, a.frequency);
     if (bias) {
-        TORCH_CHECK_VALUE(!wants_grad(*bias), "bias passes no gradient: add one that is trained to the logits");
         Tensor b = table_of("bias", *bias, logits, k);
         if (b.scalar_type() != at::kFloat) b = b.to(at::kFloat);
         a.bias_dev = static_cast<const float *>(address(b));
@@ -311,6 +350,8 @@ Tensor adjust_forward(const Tensor &logits, const Maybe &into, const Maybe &hist
     const Tensor x = rows_of(logits), out = into ? *into : at::empty(logits.sizes(), logits.options());
     d.a.logits_stride = row_stride(x);
     d.a.out_stride = d.a.k;
+    if (into)
+        for (const Tensor &t : d.keep) TORCH_CHECK_VALUE(!overlap(out, t), "out must not lie across history, lengths, penalties, bias or mask");
     if (d.a.n) {
         On on(logits);
         check(entry.adjust(&d.a, address(x), address(out), on.stream));
@@ -345,20 +386,13 @@ struct Adjust : torch::autograd::Function<Adjust> {
     }
 };
 
-// whether two tensors may share memory, by their first and last element
-bool overlap(const Tensor &a, const Tensor &b) {
-    if (!a.numel() || !b.numel()) return false;
-    auto end = [](const Tensor &t) {
-        int64_t last = 1;
-        for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-        return static_cast<const char *>(t.data_ptr()) + last * t.element_size();
-    };
-    return static_cast<const char *>(a.data_ptr()) < end(b) && static_cast<const char *>(b.data_ptr()) < end(a);
-}
-
 Tensor adjust_logits(const Tensor &logits, const Maybe &history, const Maybe &lengths, const Number &repetition, const Number &presence, const Number &frequency,
                      const Maybe &bias, const Maybe &mask, const Maybe &out) {
     on_gpu("logits", logits);
+    no_gradient("repetition", repetition);
+    no_gradient("presence", presence);
+    no_gradient("frequency", frequency);
+    no_gradient("bias", bias, "add one that is trained to the logits");
     if (out) {
         TORCH_CHECK_VALUE(!wants_grad(logits) && !wants_grad(*out), "out is not differentiable: leave it out, or call under torch.no_grad()");
         beside("out", *out, logits);
@@ -366,6 +400,7 @@ Tensor adjust_logits(const Tensor &logits, const Maybe &history, const Maybe &le
                           " and of shape ", logits.sizes());
         TORCH_CHECK_VALUE(!overlap(*out, logits) || (out->data_ptr() == logits.data_ptr() && logits.is_contiguous()), "out may be the logits or lie beside them, not across them");
     } else if (wants_grad(logits)) {
+        no_leaf_of_the_default_stream(logits);
         return Adjust::apply(logits, history, lengths, repetition, presence, frequency, bias, mask);
     }
     return adjust_forward(logits, out, history, lengths, repetition, presence, frequency, bias, mask);
@@ -398,6 +433,7 @@ Rows rows(const Tensor &logits, const Number &temperature, int tokens_type) {
 std::pair<Tensor, Tensor> draw(const Tensor &logits, const Maybe &uniforms, const Number &temperature, at::ScalarType dtype) {
     Rows r = rows(logits, temperature, whole("dtype", dtype));
     const auto lead = lead_of(logits);
+    no_gradient("temperature", temperature);
     TORCH_CHECK_VALUE(dtype != at::kByte || logits.size(-1) <= 255, "tokens as uint8 take rows of at most 255, got ", logits.size(-1));
     Tensor u;
     if (uniforms) {
@@ -463,6 +499,8 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
 
 std::pair<Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &tokens, const Number &temperature) {
     on_gpu("logits", logits);
+    no_gradient("temperature", temperature);
+    if (wants_grad(logits)) no_leaf_of_the_default_stream(logits);
     const auto out = wants_grad(logits) ? Logprobs::apply(logits, tokens, temperature) : logprobs_forward(logits, tokens, temperature, false);
     return {out[0], out[1]};
 }

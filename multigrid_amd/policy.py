@@ -15,8 +15,9 @@ last dimension that is not adjacent in memory is copied.  What a backward pass r
 simulator writes its images in place).  float32, bfloat16 and float16; sums are held in 32 bits or more and rounded
 once.
 
-A backward pass that is captured must not meet a leaf that an eager graph still holds (torch's own rule: the leaf's
-gradient would be accumulated on that graph's stream); ``embed_grad`` is the table's gradient without autograd.
+A backward pass that is captured must not meet a leaf that an eager graph of the default stream still holds: the leaf's
+gradient would be accumulated on that stream, which ends the process.  A differentiable call under capture looks for such
+a leaf and raises RuntimeError; ``embed_grad`` is the table's gradient without autograd.
 """
 from __future__ import annotations
 
@@ -73,7 +74,7 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
 
     ``history`` ``[..., t]`` (or ``[t]`` for all rows): what was answered before, whole numbers; of row i the first
     ``lengths[i]`` count (all without ``lengths``), entries outside 0 .. k - 1 do not.  A token that stands there c > 0 times
-    has its logit x made ``x / repetition`` where positive and ``x * repetition`` elsewhere, less ``presence``, less
+    has its logit x made ``x * (1 / repetition)`` where positive and ``x * repetition`` elsewhere, less ``presence``, less
     ``frequency * c``; each of the three is a number or a tensor of one per row.  ``bias`` ``[k]`` or ``[..., k]`` is added.
     ``mask`` says what may be answered - ``bool`` / ``uint8`` ``[k]`` or ``[..., k]``, or one bit per token in ``int32``
     ``[ceil(k / 32)]`` or ``[..., ceil(k / 32)]``, lowest bit first; everything else becomes -inf, also all of a row.
@@ -89,8 +90,8 @@ def draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *, tempe
 
     ``uniforms`` ``[...]`` in [0, 1), float32 or float64: the lowest token up to which the probabilities add up to more
     than it, worked out in 64 bits.  Without: the lowest token of the largest logit.  ``temperature`` is a number or a
-    tensor of one per row.  A row that is no distribution - everything -inf, a NaN, +inf - gives token -1 (255 in uint8)
-    and log-probability -inf or NaN.  ``dtype`` of the tokens: int64, int32, or uint8 for up to 255 tokens, which is what
+    tensor of one per row.  A row that is no distribution - everything -inf, a NaN, +inf, no positive temperature - gives
+    token -1 (255 in uint8) and log-probability -inf or NaN.  ``dtype`` of the tokens: int64, int32, or uint8 for up to 255 tokens, which is what
     ``step`` takes as actions (255 is no action).  Not differentiable: ``token_logprobs`` is."""
     return (_bound or _native()).draw(logits, uniforms, temperature, dtype)
 

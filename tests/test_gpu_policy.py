@@ -724,3 +724,151 @@ def test_calls_on_two_streams_at_once(policy):
     for i in range(2):
         for outs in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+
+
+# ---- what no argument check can see, and what one refuses --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("k", [7, 33, 64, 600, 2000, 9000, 70000])
+def test_temperatures_and_uniforms_out_of_range(policy, k):
+    g = gen(k)
+    inf, nan = math.inf, math.nan
+    x = randn(g, 7, k)
+    x[:, : k // 3] = -inf
+    x[:, -(k // 3):] = -inf
+    temperature = torch.tensor([0.0, -1.0, nan, inf, 1e-40, 1.0, 2.0 ** -126])
+    x, t = x.to(DEV), temperature.to(DEV)
+    for u in (torch.full((7,), 0.5, device=DEV), None):
+        tokens, lp = policy.draw(x, u, temperature=t)
+        assert (tokens[:5] == -1).all() and lp[:5].isnan().all()
+        assert (tokens[5:] >= k // 3).all() and (tokens[5:] < k - k // 3).all() and lp[5:].isfinite().all()
+        assert tokens[6] == x[6].argmax()  # next to nothing beside it
+    leaf = x.clone().requires_grad_()
+    lp, h = policy.token_logprobs(leaf, torch.full((7,), k // 2, device=DEV), temperature=t)
+    assert lp[:5].isnan().all() and h[:5].isnan().all() and lp[5].isfinite() and not lp[6].isnan() and h[5:].isfinite().all()
+    grad, = torch.autograd.grad(lp[:6].sum() + h[:6].sum(), leaf)
+    barred = x.isinf()
+    assert (grad[barred] == 0).all() and grad[:5][~barred[:5]].isnan().all() and grad[5].isfinite().all()
+    # uniform numbers below, above and none at all: the first and the last token that has a probability
+    low, _ = policy.draw(x, torch.tensor([-1.0, nan, -inf, 0.0, -1e-30, -0.0, -5.0], device=DEV))
+    high, _ = policy.draw(x, torch.tensor([1.0, 2.0, inf, 1e30, 1.0, 1.0, 1.5], device=DEV))
+    assert (low == k // 3).all() and (high == k - k // 3 - 1).all()
+
+
+@pytest.mark.parametrize("k", [7, 300, 70000])
+def test_token_logprobs_of_infinite_gradients(policy, k):
+    x = randn(gen(k), 4, k)
+    x[:, ::2] = -math.inf
+    x = x.to(DEV).requires_grad_()
+    lp, h = policy.token_logprobs(x, torch.ones(4, dtype=torch.int64, device=DEV))
+    up = torch.tensor([math.inf, -math.inf, math.nan, 1.0], device=DEV)
+    grad, = torch.autograd.grad((lp, h), x, (up, torch.zeros_like(up)))
+    assert (grad[:, ::2] == 0).all() and grad[3].isfinite().all()
+
+
+def test_embed_of_many_tokens_from_one_field(policy):
+    # finished rows and the table itself, side by side, would pass the LDS that a launch may ask for
+    n, rows, dim = 16 * 256 * 1001 + 3, 1000, 12
+    g = gen(3)
+    ids = torch.randint(0, rows + 1, (n,), generator=g, dtype=torch.int32).to(DEV)
+    table = randn(g, rows, dim).to(DEV)
+    got = policy.embed(ids, table, scale=2.0)
+    want = torch.where((ids < rows)[:, None], 2.0 * table[ids.clamp(max=rows - 1).long()], 0.0)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [24, 100])
+def test_embed_of_the_widest_rows(policy, rows):
+    dim, n = 1 << 20, 40
+    g = gen(rows)
+    ids = torch.randint(0, rows, (n,), generator=g)
+    table = torch.arange(rows * dim, device=DEV, dtype=torch.float32).reshape(rows, dim) % 1021
+    up = torch.arange(n * dim, device=DEV, dtype=torch.float32).reshape(n, dim) % 1019
+    assert torch.equal(policy.embed(ids.to(DEV), table), table[ids.to(DEV)])
+    want = torch.zeros(rows, dim, device=DEV)  # whole numbers: every order gives the same sum
+    for i, r in enumerate(ids.tolist()):
+        want[r] += up[i]
+    assert torch.equal(policy.embed_grad(up, ids.to(DEV), rows), want)
+    with pytest.raises(ValueError, match="not supported"):
+        policy.embed_grad(torch.empty(1, dim + 1, device=DEV), ids[:1].to(DEV), rows)
+
+
+def test_refusals(policy):
+    f = lambda *shape, dtype=torch.float32: torch.zeros(shape, device=DEV, dtype=dtype)
+    x, table, ids = f(4, 9), f(24, 8), f(5, dtype=torch.int64)
+    asks = lambda t: t.clone().requires_grad_()
+    refused = [
+        (lambda: policy.embed(ids.cpu(), table), "GPU"), (lambda: policy.embed(ids, table.cpu()), "GPU"), (lambda: policy.embed(ids.float(), table), "ids must be"),
+        (lambda: policy.embed(ids, table.double()), "table must be"), (lambda: policy.embed(ids, f(8)), "table must be"), (lambda: policy.embed(ids, f(0, 8)), "hold something"),
+        (lambda: policy.embed(f(5, 3, dtype=torch.uint8), table, fields=(11, 6, 8)), "add up"), (lambda: policy.embed(f(5, 2, dtype=torch.uint8), table, fields=(11, 6, 7)), "fields"),
+        (lambda: policy.embed(f(5, 9, dtype=torch.uint8), table, fields=(1,) * 8 + (16,)), "fields"), (lambda: policy.embed(f(5, 2, dtype=torch.uint8), table, fields=(24, 0)), "positive"),
+        (lambda: policy.embed_grad(f(6, 8), ids, 24), "shape"), (lambda: policy.embed_grad(f(5, 8), ids, 0), "hold something"),
+        (lambda: policy.adjust_logits(x.double()), "logits must be"), (lambda: policy.adjust_logits(x, history=f(3, 2, dtype=torch.int64)), "history must be"),
+        (lambda: policy.adjust_logits(x, history=f(4, 2)), "history must be"), (lambda: policy.adjust_logits(x, lengths=f(4, dtype=torch.int32)), "without a history"),
+        (lambda: policy.adjust_logits(x, history=f(4, 2, dtype=torch.int32), lengths=f(3, dtype=torch.int32)), "lengths must be"),
+        (lambda: policy.adjust_logits(x, mask=f(4, 8, dtype=torch.bool)), "mask must be"), (lambda: policy.adjust_logits(x, mask=f(4, 9)), "mask must be"),
+        (lambda: policy.adjust_logits(x, mask=f(4, 2, dtype=torch.int32)), "mask must be"), (lambda: policy.adjust_logits(x, bias=f(8)), "bias must be"),
+        (lambda: policy.adjust_logits(x, presence=f(3)), "presence must be"), (lambda: policy.adjust_logits(x, out=f(4, 8)), "out must be"),
+        (lambda: policy.adjust_logits(x, out=f(9, 4).t()), "out must be"), (lambda: policy.adjust_logits(x, out=x.half()), "out must be"),
+        (lambda: policy.adjust_logits(asks(x), out=f(4, 9)), "not differentiable"), (lambda: policy.adjust_logits(f(5, 9)[:4], out=f(4, 9).cpu()), "GPU"),
+        (lambda: policy.draw(x, f(3)), "uniforms must be"), (lambda: policy.draw(x, f(4, dtype=torch.float16)), "uniforms must be"),
+        (lambda: policy.draw(x, dtype=torch.int16), "dtype must be"), (lambda: policy.draw(f(2, 256), dtype=torch.uint8), "uint8"), (lambda: policy.draw(x, temperature=f(2)), "temperature must be"),
+        (lambda: policy.token_logprobs(x, f(3, dtype=torch.int64)), "tokens must be"), (lambda: policy.token_logprobs(x, f(4)), "tokens must be"), (lambda: policy.token_logprobs(x[0, 0], ids), "logits must be"),
+        # gradients that would be lost without a word
+        (lambda: policy.adjust_logits(asks(x), bias=asks(f(9))), "bias passes no"), (lambda: policy.adjust_logits(x, bias=asks(f(9))), "bias passes no"),
+        (lambda: policy.adjust_logits(asks(x), repetition=asks(f(4))), "repetition passes no"), (lambda: policy.adjust_logits(asks(x), presence=asks(f(4))), "presence passes no"),
+        (lambda: policy.adjust_logits(x, frequency=asks(f(4))), "frequency passes no"), (lambda: policy.draw(x, temperature=asks(f(4))), "temperature passes no"),
+        (lambda: policy.token_logprobs(asks(x), f(4, dtype=torch.int64), temperature=asks(f(4))), "temperature passes no"),
+    ]
+    for call, text in refused:
+        with pytest.raises(ValueError, match=text):
+            call()
+    # out across what the call reads
+    whole = f(10, 9)
+    for more in (dict(out=whole[1:5]), dict(out=whole[4:8], bias=whole[7]), dict(out=whole[4:8], presence=whole.view(-1)[36:40])):
+        with pytest.raises(ValueError, match="across"):
+            policy.adjust_logits(whole[:4], **more)
+    from multigrid_amd._lib import MgError
+    for call in (lambda: policy.draw(x, temperature=0.0), lambda: policy.draw(x, temperature=1e-40), lambda: policy.token_logprobs(x, f(4, dtype=torch.int64), temperature=math.nan),
+                 lambda: policy.adjust_logits(x, repetition=0.0)):
+        with pytest.raises(MgError, match="temperature must be|repetition must be"):
+            call()
+    # differentiable once
+    for out, leaf in ((lambda t: policy.embed(ids, t), table), (lambda t: policy.adjust_logits(t, presence=1.0), x), (lambda t: policy.token_logprobs(t, ids[:4])[0], x)):
+        leaf = asks(leaf)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(out(leaf).sum(), leaf, create_graph=True)
+
+
+def test_capture_beside_an_eager_graph_of_the_same_leaf(policy):
+    table = randn(gen(1), 24, 8).to(DEV).requires_grad_()
+    w = randn(gen(2), 6, 9).to(DEV).requires_grad_()
+    ids, tokens, x = torch.arange(24, device=DEV), torch.arange(4, device=DEV), randn(gen(3), 4, 6).to(DEV)
+    calls = [lambda: policy.embed(ids, table), lambda: policy.adjust_logits(x @ w, presence=1.0), lambda: policy.token_logprobs(x @ w, tokens)[0]]
+    with torch.no_grad():
+        x @ w  # the library's own first call
+    held = [call().sum() for call in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mark = x + 1  # (a graph of nothing is reported)
+        for call in calls:
+            with pytest.raises(RuntimeError, match="eager graph"):
+                call()
+    graph.replay()
+    del held, graph
+    # with that graph gone the same is captured
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want, = torch.autograd.grad(calls[0]().square().sum(), table)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(calls[0]().square().sum(), table)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    assert torch.equal(mark, x + 1)

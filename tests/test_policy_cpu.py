@@ -28,7 +28,7 @@ def embed_spec(**more):
 @needs_lib
 @pytest.mark.parametrize("more,word", [
     (dict(n=-1), "n -1"), (dict(n=1 << 31), "n 2147483648"), (dict(fields=0), "fields"), (dict(fields=9), "fields"), (dict(dim=0), "dim"),
-    (dict(dim=(1 << 24) + 1), "dim"), (dict(ids_type=3), "type"), (dict(dtype=3), "type"), (dict(ids_stride=-1), "stride"), (dict(row_stride=-1), "stride"),
+    (dict(dim=(1 << 20) + 1), "dim"), (dict(ids_type=3), "type"), (dict(dtype=3), "type"), (dict(ids_stride=-1), "stride"), (dict(row_stride=-1), "stride"),
     (dict(field_stride=-1), "stride"), (dict(size0=0), "field 0"), (dict(size0=-5), "field 0"), (dict(size0=(1 << 30)), "rows"), (dict(reserved0=1), "reserved0")])
 def test_embed_refuses(more, word):
     L = _lib.lib()
@@ -99,7 +99,7 @@ def logits_spec(**more):
 @needs_lib
 @pytest.mark.parametrize("more,word", [
     (dict(n=-1), "n -1"), (dict(n=1 << 31), "n "), (dict(k=0), "k 0"), (dict(k=(1 << 24) + 1), "k "), (dict(dtype=3), "type"), (dict(tokens_type=3), "tokens"),
-    (dict(tokens_type=_lib.U8, k=256), "tokens"), (dict(stride=-1), "stride"), (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
+    (dict(tokens_type=_lib.U8, k=256), "tokens"), (dict(stride=-1), "stride"), (dict(temperature=0.0), "temperature"), (dict(temperature=1e-40), "temperature"), (dict(temperature=-1.0), "temperature"),
     (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature")])
 def test_draw_and_logprobs_refuse(more, word):
     L = _lib.lib()
