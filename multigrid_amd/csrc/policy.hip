@@ -285,13 +285,13 @@ __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *id
     }
 }
 
-// A table that LDS holds (cells: 24 rows): a block copies it there once, then takes FAR tokens' ids at a time into LDS as row
-// numbers, and writes those tokens' outputs 16 bytes a thread, four tokens to a thread at once.  Bound by the writes; from memory
+// A table that LDS holds (cells: 24 rows): a block copies it there once, then takes `far` (up to FAR) tokens' ids at a time into LDS
+// as row numbers, and writes those tokens' outputs 16 bytes a thread, four tokens to a thread at once.  Bound by the writes; from memory
 // or L1 each output waited for a chain of id, row and store.
-constexpr int TABLE_BYTES = 32768, FAR = 512, TABLE_BLOCKS = 2048;
+constexpr int TABLE_BYTES = 32768, FAR = 512, TABLE_BLOCKS = 2048, UNITS = 256;
 
 template <class T, class I>
-__global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, const I *ids, const T *table, T *out) {
+__global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, int far, const I *ids, const T *table, T *out) {
     constexpr int V = WIDE<T>, TOGETHER = 4;
     extern __shared__ __align__(16) char lds[];
     const int vecs = (a.dim + V - 1) / V, pitch = vecs * V;
@@ -303,8 +303,8 @@ __global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, const
     }
     const int cols = min(vecs, THREADS), per_block = THREADS / cols;
     const int sub = threadIdx.x / cols, col = threadIdx.x - sub * cols;
-    for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * FAR; n0 < a.n; n0 += static_cast<int64_t>(gridDim.x) * FAR) {
-        const int tokens = static_cast<int>(min(static_cast<int64_t>(FAR), a.n - n0));
+    for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * far; n0 < a.n; n0 += static_cast<int64_t>(gridDim.x) * far) {
+        const int tokens = static_cast<int>(min(static_cast<int64_t>(far), a.n - n0));
         __syncthreads();
         int base = 0;
         for (int f = 0; f < a.fields; ++f) {
@@ -385,16 +385,20 @@ __global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedA
     }
     const int cols = min(vecs, COMBINED_THREADS), per_block = COMBINED_THREADS / cols;
     const int sub = threadIdx.x / cols, col = threadIdx.x - sub * cols;
-    for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * FAR; n0 < a.n; n0 += static_cast<int64_t>(gridDim.x) * FAR) {
+    I id[MG_MAX_FIELDS];
+    auto fetch = [&](int64_t n0) {  // FAR is COMBINED_THREADS
+        const I *from = ids + min(n0 + threadIdx.x, a.n - 1) * a.ids_stride;
+#pragma unroll
+        for (int f = 0; f < MG_MAX_FIELDS; ++f)
+            if (f < a.fields) id[f] = from[f * a.field_stride];
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * FAR;
+    int64_t n0 = static_cast<int64_t>(blockIdx.x) * FAR;
+    if (n0 < a.n) fetch(n0);
+    for (; n0 < a.n; n0 += step) {
         const int tokens = static_cast<int>(min(static_cast<int64_t>(FAR), a.n - n0));
         __syncthreads();
         {
-            const int t = min(static_cast<int>(threadIdx.x), tokens - 1);  // FAR is COMBINED_THREADS
-            const I *from = ids + (n0 + t) * a.ids_stride;
-            I id[MG_MAX_FIELDS];
-#pragma unroll
-            for (int f = 0; f < MG_MAX_FIELDS; ++f)
-                if (f < a.fields) id[f] = from[f * a.field_stride];
             int which = 0;
 #pragma unroll
             for (int f = 0; f < MG_MAX_FIELDS; ++f)
@@ -404,6 +408,7 @@ __global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedA
                 }
             which_s[threadIdx.x] = static_cast<uint16_t>(which);
         }
+        if (n0 + step < a.n) fetch(n0 + step);  // on their way while this one's outputs are written
         __syncthreads();
         if (sub < per_block)
             for (int c = col; c < vecs; c += cols)
@@ -729,24 +734,34 @@ __device__ __forceinline__ void load_entries(const EmbedArgs &a, const void *ids
     }
 }
 
-// Lanes with the same digit as this one.
-__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool live) {
-    uint64_t same = __ballot(live);
-    for (int b = 0; b < bits; ++b) {
-        const uint64_t ones = __ballot((digit >> b) & 1);
-        same &= (digit >> b) & 1 ? ones : ~ones;
+// Places among the wave's earlier entries of the same digit, counted in `count`: N digits of a lane, one after the other.  What
+// waits (the counters) is under way for all of them at once.
+template <int N>
+__device__ __forceinline__ void places(uint32_t *count, const uint32_t (&digit)[N], const bool (&live)[N], int bits, uint32_t (&at)[N]) {
+    uint32_t low[N], high[N];  // lanes with the same digit as this one
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint64_t all = __ballot(live[j]);
+        low[j] = static_cast<uint32_t>(all);
+        high[j] = static_cast<uint32_t>(all >> 32);
     }
-    return same;
-}
-
-// Place among the wave's earlier entries of the same digit, counted in `count`.
-__device__ __forceinline__ uint32_t place(uint32_t *count, uint32_t digit, int bits, bool live, int lane) {
-    const uint64_t same = same_digit(digit, bits, live);
-    const int leader = same ? __builtin_ctzll(same) : 0;
-    uint32_t before = 0;
-    if (live && lane == leader) before = atomicAdd(&count[digit], static_cast<uint32_t>(__popcll(same)));
-    before = __shfl(before, leader, 64);
-    return before + __popcll(same & ((1ull << lane) - 1));
+    for (int b = 0; b < bits; ++b)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t one = __builtin_amdgcn_sbfe(digit[j], b, 1);  // no bit, or all
+            const uint64_t ones = __ballot(one != 0);
+            low[j] &= ~(static_cast<uint32_t>(ones) ^ one);
+            high[j] &= ~(static_cast<uint32_t>(ones >> 32) ^ one);
+        }
+    uint32_t before[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        at[j] = __builtin_amdgcn_mbcnt_hi(high[j], __builtin_amdgcn_mbcnt_lo(low[j], 0));
+        before[j] = 0;
+        if (live[j] && at[j] == 0) before[j] = atomicAdd(&count[digit[j]], static_cast<uint32_t>(__popc(low[j]) + __popc(high[j])));
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) at[j] += __shfl(before[j], low[j] ? __builtin_ctz(low[j]) : (high[j] ? 32 + __builtin_ctz(high[j]) : 0), 64);
 }
 
 // exclusive sums of v over the threads of a block
@@ -790,10 +805,10 @@ constexpr int SORT_THREADS = 1024, SORT_ONE = 1 << 14, SORT_ROWS = (1 << 18) - 1
 
 __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, const void *ids, int ids_type, int entries, int passes, int bits,
                                                                   uint32_t *rows_out, uint32_t *tokens_out, char *out, int64_t out_bytes) {
-    constexpr int WAVES = SORT_THREADS / 64, ROUNDS = SORT_ONE / SORT_THREADS;
+    constexpr int WAVES = SORT_THREADS / 64, ROUNDS = SORT_ONE / SORT_THREADS, TOGETHER = 4;
     if (blockIdx.x > 0) return clear(out, out_bytes, blockIdx.x - 1, gridDim.x - 1);
     __shared__ uint32_t word_s[SORT_ONE];
-    __shared__ uint32_t count_s[WAVES][MOST_BINS];
+    __shared__ uint32_t count_s[WAVES][MOST_BINS], base_s[MOST_BINS];
     __shared__ uint32_t wave_sums[WAVES];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     const int rounds = (entries + SORT_THREADS - 1) / SORT_THREADS, first = wave * rounds * 64 + lane;
@@ -806,32 +821,46 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, c
     }
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = 14 + pass * bits, bins = 1 << bits;
-        for (int i = tid; i < WAVES * MOST_BINS; i += SORT_THREADS) (&count_s[0][0])[i] = 0;
+        for (int i = tid; i < WAVES << bits; i += SORT_THREADS) count_s[i >> bits][i & (bins - 1)] = 0;
         __syncthreads();
-        uint32_t word[ROUNDS], at[ROUNDS];
+        uint32_t word[ROUNDS / TOGETHER][TOGETHER], at[ROUNDS / TOGETHER][TOGETHER];
 #pragma unroll
-        for (int j = 0; j < ROUNDS; ++j) {
-            if (j >= rounds) break;
-            const int e = first + j * 64;
-            const bool live = e < entries;
-            word[j] = live ? word_s[e] : 0;
-            at[j] = place(count_s[wave], (word[j] >> shift) & (bins - 1), bits, live, lane);
+        for (int j = 0; j < ROUNDS / TOGETHER; ++j) {
+            if (j * TOGETHER >= rounds) break;
+            uint32_t digit[TOGETHER];
+            bool live[TOGETHER];
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u) {
+                const int e = first + (j * TOGETHER + u) * 64;
+                live[u] = j * TOGETHER + u < rounds && e < entries;
+                word[j][u] = live[u] ? word_s[e] : 0;
+                digit[u] = (word[j][u] >> shift) & (bins - 1);
+            }
+            places(count_s[wave], digit, live, bits, at[j]);
         }
         __syncthreads();
         uint32_t mine = 0;
-        if (tid < bins)
+        if (tid < bins) {
+            uint32_t c[WAVES];
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) c[w] = count_s[w][tid];
+#pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const uint32_t c = count_s[w][tid];
                 count_s[w][tid] = mine;
-                mine += c;
+                mine += c[w];
             }
+        }
         const uint32_t before = sum_before<SORT_THREADS>(mine, wave_sums, nullptr);
-        if (tid < bins)
-            for (int w = 0; w < WAVES; ++w) count_s[w][tid] += before;
+        if (tid < bins) base_s[tid] = before;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < ROUNDS; ++j)
-            if (j < rounds && first + j * 64 < entries) word_s[count_s[wave][(word[j] >> shift) & (bins - 1)] + at[j]] = word[j];
+        for (int j = 0; j < ROUNDS / TOGETHER; ++j)
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u)
+                if (j * TOGETHER + u < rounds && first + (j * TOGETHER + u) * 64 < entries) {
+                    const uint32_t digit = (word[j][u] >> shift) & (bins - 1);
+                    word_s[base_s[digit] + count_s[wave][digit] + at[j][u]] = word[j][u];
+                }
         __syncthreads();
     }
     for (int i = tid; i < entries; i += SORT_THREADS) {
@@ -893,7 +922,7 @@ __global__ __launch_bounds__(SORT_THREADS) void embed_scan_kernel(uint32_t *coun
 __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const void *ids, int ids_type, const uint2 *from, int64_t entries, int span,
                                                               int shift, int bits, const uint32_t *counts, uint2 *to, uint32_t *rows_out,
                                                               uint32_t *tokens_out) {
-    constexpr int WAVES = THREADS / 64, ROUNDS = SORT_TILE / THREADS;
+    constexpr int WAVES = THREADS / 64, ROUNDS = SORT_TILE / THREADS, TOGETHER = 4;
     __shared__ uint32_t count_s[WAVES][MOST_BINS], base_s[MOST_BINS];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, bins = 1 << bits;
     for (int i = tid; i < bins; i += THREADS) base_s[i] = counts[static_cast<int64_t>(i) * gridDim.x + blockIdx.x];
@@ -903,14 +932,23 @@ __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const
         __syncthreads();
         const int64_t first = e0 + wave * (SORT_TILE / WAVES) + lane;
         uint2 entry[ROUNDS];
-        uint32_t at[ROUNDS];
+        uint32_t at[ROUNDS / TOGETHER][TOGETHER];
         if (from)
 #pragma unroll
             for (int j = 0; j < ROUNDS; ++j) entry[j] = from[min(first + j * 64, hi - 1)];
         else
             load_entries(a, ids, ids_type, first, 64, hi, entry);
 #pragma unroll
-        for (int j = 0; j < ROUNDS; ++j) at[j] = place(count_s[wave], (entry[j].x >> shift) & (bins - 1), bits, first + j * 64 < hi, lane);
+        for (int j = 0; j < ROUNDS / TOGETHER; ++j) {
+            uint32_t digit[TOGETHER];
+            bool live[TOGETHER];
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u) {
+                digit[u] = (entry[j * TOGETHER + u].x >> shift) & (bins - 1);
+                live[u] = first + (j * TOGETHER + u) * 64 < hi;
+            }
+            places(count_s[wave], digit, live, bits, at[j]);
+        }
         __syncthreads();
         for (int i = tid; i < bins; i += THREADS) {
             uint32_t s = base_s[i];
@@ -925,7 +963,7 @@ __global__ __launch_bounds__(THREADS) void embed_place_kernel(EmbedArgs a, const
 #pragma unroll
         for (int j = 0; j < ROUNDS; ++j)
             if (first + j * 64 < hi) {
-                const uint32_t p = count_s[wave][(entry[j].x >> shift) & (bins - 1)] + at[j];
+                const uint32_t p = count_s[wave][(entry[j].x >> shift) & (bins - 1)] + at[j / TOGETHER][j % TOGETHER];
                 if (to) {
                     to[p] = entry[j];
                 } else {
@@ -1012,8 +1050,8 @@ __global__ __launch_bounds__(THREADS) void embed_span_kernel(EmbedArgs a, Sorted
         more = __syncthreads_count(at < s.chunks && s.rows[at * s.chunk] == row);
     }
     const int col = threadIdx.x % SPAN, share = threadIdx.x / SPAN;
-    const int d = blockIdx.y * SPAN + col;
     const int64_t per = (hi - lo + THREADS / SPAN - 1) / (THREADS / SPAN);
+    const int d = blockIdx.y * SPAN + col;
     float sum = 0.f;
     if (d < a.dim) {
         if (share == 0) sum = s.tail[c * a.dim + d];
@@ -2366,8 +2404,11 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
             return;
         }
         if (held <= TABLE_BYTES && a.n >= 4 * FAR) {
-            hipLaunchKernelGGL((embed_table_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, TABLE_BLOCKS)), dim3(THREADS), held + a.fields * FAR * 2,
-                               static_cast<hipStream_t>(stream), a, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
+            // as many tokens to a block as give every compute unit the same number of blocks
+            const int64_t rounds = (a.n + UNITS * FAR - 1) / (UNITS * FAR), share = (a.n + UNITS * rounds - 1) / (UNITS * rounds);
+            const int far = static_cast<int>(share + per_block - 1 < FAR ? (share + per_block - 1) / per_block * per_block : FAR);
+            hipLaunchKernelGGL((embed_table_kernel<T, I>), dim3(blocks_for((a.n + far - 1) / far, TABLE_BLOCKS)), dim3(THREADS), held + a.fields * FAR * 2,
+                               static_cast<hipStream_t>(stream), a, far, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
             return;
         }
         hipLaunchKernelGGL((embed_kernel<T, I>), dim3(blocks_for((a.n + per_block - 1) / per_block)), dim3(THREADS), 0,
