@@ -57,6 +57,23 @@ __device__ __forceinline__ void store(T *p, const float (&x)[V]) {
 template <class T>
 constexpr int WIDE = 16 / static_cast<int>(sizeof(T));
 
+// 16 bytes moved down by `bits` (1 .. 128), `fills` behind them
+__device__ __forceinline__ void move_down(uint32_t (&w)[4], int bits, uint32_t fills) {
+    const uint64_t all = static_cast<uint64_t>(fills) << 32 | fills, lo = static_cast<uint64_t>(w[1]) << 32 | w[0], hi = static_cast<uint64_t>(w[3]) << 32 | w[2];
+    uint64_t to, top;
+    if (bits < 64) {
+        to = lo >> bits | hi << (64 - bits);
+        top = hi >> bits | all << (64 - bits);
+    } else {
+        to = bits == 64 ? hi : (bits == 128 ? all : hi >> (bits - 64) | all << (128 - bits));
+        top = all;
+    }
+    w[0] = static_cast<uint32_t>(to);
+    w[1] = static_cast<uint32_t>(to >> 32);
+    w[2] = static_cast<uint32_t>(top);
+    w[3] = static_cast<uint32_t>(top >> 32);
+}
+
 // Words of W adjacent elements at p, which stay packed until they are used.  `left` elements are the row's, the others become
 // `fill` (an element's bits).  A row of at least W elements is never read element by element (each would be waited for): the W
 // elements that end where the row does are read and moved down.
@@ -80,25 +97,14 @@ __device__ __forceinline__ void load_words(const T *p, int left, int length, uin
             const int down = (W - left) * BITS;
             if constexpr (WORDS == 1) {
                 w[0] = r.w[0] >> 16 | fills << 16;
-            } else {
-                const uint64_t all = static_cast<uint64_t>(fills) << 32 | fills, lo = static_cast<uint64_t>(r.w[1]) << 32 | r.w[0];
-                uint64_t to = 0, top = 0;
-                if constexpr (WORDS == 2) {
-                    to = lo >> down | all << (64 - down);
-                } else {
-                    const uint64_t hi = static_cast<uint64_t>(r.w[3]) << 32 | r.w[2];
-                    if (down < 64) {
-                        to = lo >> down | hi << (64 - down);
-                        top = hi >> down | all << (64 - down);
-                    } else {
-                        to = down == 64 ? hi : hi >> (down - 64) | all << (128 - down);
-                        top = all;
-                    }
-                    w[2] = static_cast<uint32_t>(top);
-                    w[3] = static_cast<uint32_t>(top >> 32);
-                }
+            } else if constexpr (WORDS == 2) {
+                const uint64_t to = (static_cast<uint64_t>(r.w[1]) << 32 | r.w[0]) >> down | (static_cast<uint64_t>(fills) << 32 | fills) << (64 - down);
                 w[0] = static_cast<uint32_t>(to);
                 w[1] = static_cast<uint32_t>(to >> 32);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = r.w[i];
+                move_down(w, down, fills);
             }
         } else if constexpr (WORDS > 1) {  // a short row: its halves
             if (left > 0) {
@@ -130,34 +136,28 @@ __device__ __forceinline__ float element(const uint32_t *w, int i) {
         return static_cast<float>(__builtin_bit_cast(T, static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)))));
 }
 
-// N vectors of a row, number j at first + (j * lanes + lane) * V; behind the row's k elements `fill`.  Only one thread's vector
-// can hold the row's end in part; it is loaded apart from the others, once.  V elements or more lie before that end (the row has more than
+// N vectors of a row, number j at first + (j * lanes + lane) * V; behind the row's k elements `fill`.  All loads are under way
+// before the first is looked at, so none stands behind a test (which would be waited for): a vector that passes the row's end is
+// read where the row's last V elements lie, and moved down.  V elements or more lie before that end (the row has more than
 // SHORT, and a piece of one begins behind others).
 template <class T, int N>
 __device__ __forceinline__ void load_vectors(const T *row, int k, int first, int lanes, int lane, uint32_t fill, uint32_t (&w)[N][4]) {
     constexpr int V = WIDE<T>;
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {
+        uint32_t w[4];
+    };
     const uint32_t fills = sizeof(T) == 4 ? fill : fill * 0x10001u;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const int at = first + (j * lanes + lane) * V;
-        if (at + V <= k) {
-            load_words<T, V>(row + at, V, V, fill, w[j]);
-        } else {
+        const Words r = *reinterpret_cast<const Words *>(row + min(first + (j * lanes + lane) * V, k - V));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[j][i] = fills;
-        }
+        for (int i = 0; i < 4; ++i) w[j][i] = r.w[i];
     }
-    const int end = k / V * V;
-    if (end < k && end >= first) {
-        const int v = (end - first) / V, j = v >> __builtin_ctz(lanes);  // (a power of two)
-        if (j < N && v - j * lanes == lane) {
-            uint32_t q[4];
-            load_words<T, V>(row + end, k - end, V, fill, q);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int o = 0; o < N; ++o)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[o][i] = o == j ? q[i] : w[o][i];
-        }
+    for (int j = 0; j < N; ++j) {
+        const int past = first + (j * lanes + lane) * V - (k - V);
+        if (past > 0) move_down(w[j], min(past, V) * 8 * static_cast<int>(sizeof(T)), fills);
     }
 }
 
@@ -1112,6 +1112,7 @@ struct Row {
     uint32_t held[HELD][4];
 
     __device__ __forceinline__ Row(const T *row, int tokens, int thread) : x(row), k(tokens), lane(thread) {
+        asm volatile("" : "+v"(lane));  // (else every token's number would wait in a register while rows go by)
         load_vectors<T, HELD>(x, k, 0, LANES, lane, NEG_INF_BITS<T>, held);
     }
     // f(number of the vector, its words) for all of this thread's vectors.  The empty statements keep a pass from sharing its
@@ -1504,7 +1505,10 @@ __device__ __forceinline__ int find_border(Row<T, LANES, HELD> &row, DrawShared 
     constexpr int V = WIDE<T>, SPAN = LANES < 64 ? LANES : 64, WAVES = LANES > 64 ? LANES / 64 : 1;
     const int wave = LANES > 64 ? threadIdx.x / 64 : 0, lane = row.lane % 64;
     double part[HELD];
-    row.each([&](int j, const uint32_t *v) { part[j] = s.of_vector<T>(v); });
+    row.each([&](int j, const uint32_t *v) {
+        part[j] = s.of_vector<T>(v);
+        asm volatile("" : "+v"(part[j]));  // now, not where it is used
+    });
     // inclusive sums over the threads of a wave (or of a shorter row)
     auto upto = [&](double v) {
 #pragma unroll
