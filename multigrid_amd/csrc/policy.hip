@@ -127,6 +127,25 @@ __device__ __forceinline__ void load_words(const T *p, int left, int length, uin
     }
 }
 
+// 2, 4 or 8 bytes of elements of ALIGN bytes from an address that was a number: a pointer made of one is no pointer to global memory
+// to the compiler, and its loads would be waited for together with everything else.
+template <int BYTES, int ALIGN>
+__device__ __forceinline__ void load_global(uint64_t at, uint32_t (&w)[(BYTES + 3) / 4]) {
+    using one_t = uint32_t __attribute__((aligned(ALIGN)));
+    using two_t = uint32_t __attribute__((ext_vector_type(2), aligned(ALIGN)));
+#define GLOBAL_AT(type) *reinterpret_cast<const __attribute__((address_space(1))) type *>(at)
+    if constexpr (BYTES == 2) {
+        w[0] = GLOBAL_AT(uint16_t);
+    } else if constexpr (BYTES == 4) {
+        w[0] = GLOBAL_AT(one_t);
+    } else {
+        const two_t v = GLOBAL_AT(two_t);
+        w[0] = v.x;
+        w[1] = v.y;
+    }
+#undef GLOBAL_AT
+}
+
 // element i of words
 template <class T>
 __device__ __forceinline__ float element(const uint32_t *w, int i) {
@@ -501,10 +520,10 @@ union Fragment {
     }
 };
 
-template <class T, int W, int TILES>
-__global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
+template <class T, int W, int TILES, int FIELDS>
+__global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 || FIELDS > 3 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
     constexpr int COLS = 16 * W, WORDS = (W * sizeof(T) + 3) / 4;
-    __shared__ __align__(16) uint16_t rows_s[THREADS / 64][MG_MAX_FIELDS][64];  // 0xFFFF: none
+    __shared__ __align__(16) uint16_t rows_s[THREADS / 64][FIELDS][64];  // 0xFFFF: none
     __shared__ float sum_s[TILES * 16][COLS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, l16 = lane % 16, quad = lane / 16;
     const int d0 = blockIdx.y * COLS, col = l16 * W;
@@ -528,49 +547,59 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
     const int64_t step = static_cast<int64_t>(gridDim.x) * THREADS;
     // a lane at the row's end, or behind it, takes the last W columns and keeps of them those that are its own
     const int from_col = min(col, a.dim - d0 - W);
-    const uint32_t stride = static_cast<uint32_t>(a.row_stride) * sizeof(T), at_col = (d0 + from_col) * sizeof(T), own = quad * stride + at_col;  // bytes, see FAR_ROWS
-    auto fetch_ids = [&](int64_t t0, Id (&id)[MG_MAX_FIELDS]) {
-        int64_t at = min(t0 + lane, a.n - 1) * a.ids_stride;
-        asm volatile("" : "+v"(at));  // one running address, not one for each field and type
-        with_ids(ids, ids_type, [&](auto load_id) {
+    const uint32_t stride = static_cast<uint32_t>(a.row_stride) * sizeof(T), own = quad * stride + (d0 + from_col) * sizeof(T);  // bytes, see FAR_ROWS
+    // No load stands behind a branch: it would be waited for at the branch's end, and with it all that were on their way before.
+    // So the last 64 tokens stand for a wave that passes the end (tokens of another wave's are given no row), the last field for
+    // those that are not there, and of an id the aligned word that holds it, or its lower half, is read, and an upper half, which
+    // only int64 has.
+    const int id_shift = ids_type == MG_U8 ? 0 : (ids_type == MG_I32 ? 2 : 3);
+    const uint32_t id_mask = ids_type == MG_U8 ? 0xFF : ~0u, high_mask = ids_type == MG_I64 ? ~0u : 0;
+    auto id_at = [&](int64_t t0, int f) {
+        return reinterpret_cast<uint64_t>(ids) + (((min(t0, a.n - 64) + lane) * a.ids_stride + min(f, a.fields - 1) * a.field_stride) << id_shift);
+    };
+    auto fetch_ids = [&](int64_t t0, Id (&id)[FIELDS]) {
 #pragma unroll
-            for (int f = 0; f < MG_MAX_FIELDS; ++f)
-                if (f < a.fields) id[f] = load_id(at + f * a.field_stride);
-        });
+        for (int f = 0; f < FIELDS; ++f) {
+            const uint64_t at = id_at(t0, f) & ~3ull;
+            uint32_t low[1], high[1];
+            load_global<4, 4>(at, low);
+            load_global<4, 4>(at + (high_mask & 4), high);
+            id[f] = Id{low[0], high[0]};
+        }
     };
     auto fetch = [&](int64_t t0, uint32_t (&x)[2][8][WORDS]) {
         // an address that is the same for the wave, and this lane's offset
-        uint64_t from = reinterpret_cast<uint64_t>(grad + t0 * a.row_stride);
+        uint64_t from = reinterpret_cast<uint64_t>(grad + min(t0, a.n - 64) * a.row_stride);
         asm volatile("" : "+s"(from));
-        auto at = [&](int token, uint32_t offset) { return reinterpret_cast<const T *>(from + static_cast<uint64_t>(token) * stride + offset); };
-        if (t0 + 64 <= a.n) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) load_words<T, W>(at(s * 32 + j * 4, own), W, W, 0, x[s][j]);
-        } else {  // tokens behind the last one read that one; no row takes them
-            const int last = static_cast<int>(a.n - 1 - t0);
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) load_words<T, W>(at(0, min(s * 32 + j * 4 + quad, last) * stride + at_col), W, W, 0, x[s][j]);
-        }
+            for (int j = 0; j < 8; ++j) load_global<W * sizeof(T), sizeof(T)>(from + static_cast<uint64_t>(s * 32 + j * 4) * stride + own, x[s][j]);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    auto put_rows = [&](int64_t t0, const Id (&id)[MG_MAX_FIELDS]) {
+    auto put_rows = [&](int64_t t0, const Id (&id)[FIELDS]) {
         __builtin_amdgcn_wave_barrier();  // the last tokens' rows are read
         const int place = (lane & 32) + (lane & 3) * 8 + (lane & 31) / 4;  // token j * 4 + quad is number j of the quad
+        const bool live = min(t0, a.n - 64) + lane >= t0;
         uint32_t base = 0;
 #pragma unroll
-        for (int f = 0; f < MG_MAX_FIELDS; ++f)
-            if (f < a.fields) {
-                rows_s[wave][f][place] = static_cast<uint16_t>(t0 + lane < a.n ? row_of(id[f], base, a.sizes[f], 0xFFFF) : 0xFFFF);
-                base += a.sizes[f];
-            }
+        for (int f = 0; f < FIELDS; ++f) {
+            const uint32_t shift = ids_type == MG_U8 ? static_cast<uint32_t>(id_at(t0, f)) % 4 * 8 : 0, size = f < a.fields ? a.sizes[f] : 0;
+            const Id own_id{(id[f].low >> shift) & id_mask, id[f].high & high_mask};
+            rows_s[wave][f][place] = static_cast<uint16_t>(live ? row_of(own_id, base, size, 0xFFFF) : 0xFFFF);
+            base += size;
+        }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
     auto add = [&](uint32_t (&x)[2][8][WORDS]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(x[s][j][i]));  // not before the next loads are on their way
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             Fragment hot[TILES];
@@ -614,16 +643,15 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
             }
         }
     };
-    // three sets of registers in turn: while one is multiplied, the loads of the next two are under way (one ahead leaves the
-    // memory idle whenever a wave waits: 3.6 TB/s).  Ids are loaded one set ahead, before the loads of the set behind that.
-    uint32_t x0[2][8][WORDS], x1[2][8][WORDS], x2[2][8][WORDS];
-    Id id[MG_MAX_FIELDS];
+    // two sets of registers in turn: while one is multiplied, the loads of the other are under way
+    uint32_t x0[2][8][WORDS], x1[2][8][WORDS];
+    Id id[FIELDS];
     int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (THREADS / 64) + wave) * 64;
-    auto turn = [&](uint32_t (&now)[2][8][WORDS], uint32_t (&far)[2][8][WORDS]) {
+    auto turn = [&](uint32_t (&now)[2][8][WORDS], uint32_t (&next)[2][8][WORDS]) {
         if (t0 >= a.n) return false;
         put_rows(t0, id);
-        if (t0 + step < a.n) fetch_ids(t0 + step, id);
-        if (t0 + 2 * step < a.n) fetch(t0 + 2 * step, far);
+        fetch_ids(t0 + step, id);
+        fetch(t0 + step, next);
         add(now);
         t0 += step;
         return true;
@@ -631,8 +659,7 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 ? 2 : 3) void embed_gra
     if (t0 < a.n) {
         fetch_ids(t0, id);
         fetch(t0, x0);
-        if (t0 + step < a.n) fetch(t0 + step, x1);
-        while (turn(x0, x2) && turn(x1, x0) && turn(x2, x1)) {
+        while (turn(x0, x1) && turn(x1, x0)) {
         }
     }
 
@@ -987,7 +1014,7 @@ template <class T>
 __global__ __launch_bounds__(THREADS) void embed_runs_kernel(EmbedArgs a, Sorted s, const T *grad, T *out) {
     constexpr int V = WIDE<T>, AHEAD = 8;
     const int lane = threadIdx.x % s.lanes, group = threadIdx.x / s.lanes, groups = THREADS / s.lanes;
-    const int d0 = (blockIdx.y * s.lanes + lane) * V, left = a.dim - d0;
+    const int d0 = (blockIdx.y * s.lanes + lane) * V, left = a.dim - d0, back = max(V - left, 0);
     if (left <= 0) return;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * groups + group;
     if (c >= s.chunks) return;
@@ -1007,15 +1034,23 @@ __global__ __launch_bounds__(THREADS) void embed_runs_kernel(EmbedArgs a, Sorted
         }
     };
     for (int64_t e = e0; e < e1; e += AHEAD) {
-        uint32_t r[AHEAD], t[AHEAD];
-        float x[AHEAD][V];
+        uint32_t r[AHEAD], t[AHEAD], w[AHEAD][4];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            r[j] = e + j < e1 ? s.rows[e + j] : none;
-            t[j] = e + j < e1 ? s.tokens[e + j] : 0;
+        for (int j = 0; j < AHEAD; ++j) {  // (behind the chunk its last entry again)
+            const int64_t at = min(e + j, e1 - 1);
+            r[j] = s.rows[at];
+            t[j] = s.tokens[at];
         }
+        if (a.dim >= V) {  // all of them under way, none behind a test; a column group that passes the row's end as in load_vectors
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) load_part<T, V>(grad + static_cast<int64_t>(t[j]) * a.row_stride + d0, r[j] == none ? 0 : left, a.dim, x[j]);
+            for (int j = 0; j < AHEAD; ++j) load_words<T, V>(grad + static_cast<int64_t>(t[j]) * a.row_stride + d0 - back, V, V, 0, w[j]);
+            if (back > 0)
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) move_down(w[j], back * 8 * static_cast<int>(sizeof(T)), 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) load_words<T, V>(grad + static_cast<int64_t>(t[j]) * a.row_stride + d0, left, a.dim, 0, w[j]);
+        }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             if (e + j >= e1) break;
@@ -1027,7 +1062,7 @@ __global__ __launch_bounds__(THREADS) void embed_runs_kernel(EmbedArgs a, Sorted
                 for (int i = 0; i < V; ++i) acc[i] = 0.f;
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] += x[j][i];
+            for (int i = 0; i < V; ++i) acc[i] += element<T>(w[j], i);
         }
     }
     finish(e1 < s.entries && s.rows[e1] == row);
@@ -1213,13 +1248,15 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
 #pragma clang fp contract(off)
     constexpr int V = WIDE<T>, PIECE = THREADS * STRETCH * V;
     __shared__ __align__(16) uint32_t counts_s[PIECE];
-    const int lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * STRETCH * V;
+    int lane = threadIdx.x & (lanes - 1);
+    const int sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * STRETCH * V;
     const int first = blockIdx.y * width;  // 0 where rows share a block
     const bool history = a.history_dev != nullptr && a.t > 0;
     uint32_t *counts = counts_s + sub * width;
     for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * per_block; row0 < a.n; row0 += static_cast<int64_t>(gridDim.x) * per_block) {
         const int64_t row = row0 + sub;
         const bool live = row < a.n;
+        asm volatile("" : "+v"(lane));  // (else every token's number would wait in a register while rows go by)
         uint32_t x[STRETCH][4], g[STRETCH][4];
         if (live) {
             load_vectors<T, STRETCH>(logits + row * a.logits_stride, a.k, first, lanes, lane, 0, x);
@@ -1323,6 +1360,7 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                 for (int i = 0; i < V; ++i)
                     if (!((allow >> i) & 1)) y[i] = GRAD ? 0.f : NEG_INF;
                 store_part<T, V>(out + row * a.out_stride + at, a.k - at, y);
+                __builtin_amdgcn_sched_barrier(0);  // one vector after the other: fewer registers
             }
         }
         if (history) __syncthreads();  // the counters are read
@@ -2002,11 +2040,13 @@ template <class T>
 __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int lanes, const T *logits, const void *tokens, const float *stats,
                                                                const float *grad_lp, int64_t lp_stride, const float *grad_h, int64_t h_stride, T *out) {
     constexpr int V = WIDE<T>, TAKES = 4;
-    const int lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * TAKES * V;
+    int lane = threadIdx.x & (lanes - 1);
+    const int sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * TAKES * V;
     const int first = blockIdx.y * width;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * per_block + sub; row < l.n; row += static_cast<int64_t>(gridDim.x) * per_block) {
         const T *x = logits + row * l.stride;
         T *to = out + row * l.k;
+        asm volatile("" : "+v"(lane));  // (else every token's number would wait in a register while rows go by)
         uint32_t w[TAKES][4];
         load_vectors<T, TAKES>(x, l.k, first, lanes, lane, NEG_INF_BITS<T>, w);
         // (none of these waits for another)
@@ -2034,6 +2074,7 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int l
                     if (at + i == token) v[i] = own;
             }
             store_part<T, V>(to + at, l.k - at, v);
+            __builtin_amdgcn_sched_barrier(0);  // one vector after the other: fewer registers
         }
     }
 }
@@ -2177,11 +2218,12 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
         p.bytes += (bytes + 15) / 16 * 16;
         return at;
     };
-    p.few = a.rows <= FEW && a.row_stride <= FAR_ROWS;
+    p.few = a.rows <= FEW && a.row_stride <= FAR_ROWS && a.n >= 64;
     if (p.few) {
         p.width = wide / 2;  // the narrowest that holds a token's columns at once, or 8 bytes: two sets of 16 loads are held
         while (p.width > 1 && (16 * (p.width / 2) >= a.dim || p.width > a.dim)) p.width /= 2;
-        p.tiles = a.rows <= 16 ? 1 : (a.rows <= 32 ? 2 : 4);
+        p.tiles = a.rows <= 32 ? 2 : 4;
+        if (p.tiles > 2 && p.width > 2) p.width = 2;  // (the sums of four tiles and four columns leave no registers for the loads)
         const int64_t blocks = (a.n + THREADS - 1) / THREADS;
         const int64_t slabs = (a.dim + 16 * p.width - 1) / (16 * p.width), all = p.width > 2 ? FEW_BLOCKS * 2 / 3 : FEW_BLOCKS,
                       most = slabs < all / 64 ? all / slabs : 64;
@@ -2218,15 +2260,21 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
     return p;
 }
 
-template <class T, int W>
+template <class T, int W, int TILES>
 void launch_few(const EmbedArgs &a, const GradPlan &p, const void *ids, int ids_type, const T *grad, T *out, float *parts, hipStream_t stream) {
     const dim3 grid(p.blocks, (a.dim + 16 * W - 1) / (16 * W));
-    if (p.tiles == 1)
-        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, 1>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
-    else if (p.tiles == 2)
-        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, 2>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
+    if (a.fields == 1)
+        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, TILES, 1>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
+    else if (a.fields <= 3)
+        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, TILES, 3>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
     else
-        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, 4>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
+        hipLaunchKernelGGL((embed_grad_few_kernel<T, W, TILES, MG_MAX_FIELDS>), grid, dim3(THREADS), 0, stream, a, ids, ids_type, grad, out, parts);
+}
+template <class T, int W>
+void launch_few(const EmbedArgs &a, const GradPlan &p, const void *ids, int ids_type, const T *grad, T *out, float *parts, hipStream_t stream) {
+    if constexpr (W <= 2)
+        if (p.tiles > 2) return launch_few<T, W, 4>(a, p, ids, ids_type, grad, out, parts, stream);
+    launch_few<T, W, 2>(a, p, ids, ids_type, grad, out, parts, stream);
 }
 
 template <class T>
