@@ -1243,16 +1243,16 @@ constexpr float DEEP = -200.f;  // exp_twice of it is 0
 // whole history (a few KB that the cache holds).
 constexpr int STRETCH = 4;
 
-template <class T, class H, bool GRAD>
+template <class T, class H, bool GRAD, class C>
 __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, const T *logits, const T *grad, T *out) {
 #pragma clang fp contract(off)
-    constexpr int V = WIDE<T>, PIECE = THREADS * STRETCH * V;
-    __shared__ __align__(16) uint32_t counts_s[PIECE];
+    constexpr int V = WIDE<T>, PIECE = THREADS * STRETCH * V, PER_WORD = 4 / static_cast<int>(sizeof(C)), WORDS = V / PER_WORD;
+    __shared__ __align__(16) uint32_t counts_s[PIECE / PER_WORD];
     int lane = threadIdx.x & (lanes - 1);
     const int sub = threadIdx.x / lanes, per_block = THREADS / lanes, width = lanes * STRETCH * V;
     const int first = blockIdx.y * width;  // 0 where rows share a block
     const bool history = a.history_dev != nullptr && a.t > 0;
-    uint32_t *counts = counts_s + sub * width;
+    uint32_t *counts = counts_s + sub * (width / PER_WORD);
     for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * per_block; row0 < a.n; row0 += static_cast<int64_t>(gridDim.x) * per_block) {
         const int64_t row = row0 + sub;
         const bool live = row < a.n;
@@ -1279,14 +1279,17 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
 #pragma unroll
             for (int j = 0; j < STRETCH; ++j)
 #pragma unroll
-                for (int i = 0; i < V; i += 4) *reinterpret_cast<uint4 *>(&counts[(j * lanes + lane) * V + i]) = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < WORDS; i += 2) *reinterpret_cast<uint2 *>(&counts[(j * lanes + lane) * WORDS + i]) = make_uint2(0, 0);
             __syncthreads();
             const int end = min(width, a.k - first);
             auto count = [&](int i, const H (&entry)[AHEAD]) {
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
                     const int64_t j = static_cast<int64_t>(entry[u]) - first;
-                    if (i + u * lanes < len && j >= 0 && j < end) atomicAdd(&counts[j], 1u);
+                    if (i + u * lanes < len && j >= 0 && j < end) {
+                        const uint32_t at = static_cast<uint32_t>(j);
+                        atomicAdd(&counts[at / PER_WORD], PER_WORD == 1 ? 1u : 1u << (at % PER_WORD * 16));
+                    }
                 }
             };
             count(lane, entry);
@@ -1321,9 +1324,11 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                 uint32_t c[V] = {};
                 if (history)
 #pragma unroll
-                    for (int i = 0; i < V; i += 4) {
-                        const uint4 q = *reinterpret_cast<const uint4 *>(&counts[(j * lanes + lane) * V + i]);
-                        c[i] = q.x, c[i + 1] = q.y, c[i + 2] = q.z, c[i + 3] = q.w;
+                    for (int i = 0; i < WORDS; i += 2) {
+                        const uint2 q = *reinterpret_cast<const uint2 *>(&counts[(j * lanes + lane) * WORDS + i]);
+                        const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+                        for (int o = 0; o < 2 * PER_WORD; ++o) c[i * PER_WORD + o] = PER_WORD == 1 ? w[o] : (w[o / PER_WORD] >> (16 * (o % PER_WORD))) & 0xFFFF;
                     }
                 float y[V];
 #pragma unroll
@@ -2412,7 +2417,11 @@ void launch_adjust(const MgAdjust &a, const void *logits, const void *grad, void
             int lanes = 8;  // the fewest that take a row at once
             while (lanes < THREADS && lanes * TAKES < a.k) lanes *= 2;
             const int64_t per_block = THREADS / lanes, pieces = (a.k + lanes * TAKES - 1) / (lanes * TAKES);
-            hipLaunchKernelGGL((adjust_kernel<T, H, GRAD>), dim3(blocks_for((a.n + per_block - 1) / per_block), pieces), dim3(THREADS), 0, stream, a, lanes, x, g, y);
+            const dim3 grid(blocks_for((a.n + per_block - 1) / per_block), pieces);
+            if (a.history_dev && a.t > 0xFFFF)
+                hipLaunchKernelGGL((adjust_kernel<T, H, GRAD, uint32_t>), grid, dim3(THREADS), 0, stream, a, lanes, x, g, y);
+            else
+                hipLaunchKernelGGL((adjust_kernel<T, H, GRAD, uint16_t>), grid, dim3(THREADS), 0, stream, a, lanes, x, g, y);
         }
     });
 }
