@@ -131,8 +131,8 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
 
     The build keeps its intermediate files in a scratch directory and looks at the device assembly before the
     library is put in place: every kernel's register and spill counts are listed (``kernel_registers.json`` beside
-    the library; printed with ``verbose``), a step kernel that spills vector registers to scratch memory fails the
-    build, and so does a code pattern this compiler was seen to get wrong (see _isa_lint.py)."""
+    the library; printed with ``verbose``), a step or policy kernel that spills vector registers to scratch memory fails
+    the build, and so does a code pattern this compiler was seen to get wrong (see _isa_lint.py)."""
     target = out_path or LIB_PATH
     sources = [SRC_PATH, POLICY_PATH, os.path.join(PKG_DIR, "csrc", "mgrid_experiment.h"),
                os.path.join(PKG_DIR, "csrc", "mgrid_error.h"), os.path.join(INCLUDE_DIR, "mgrid.h")]
@@ -182,7 +182,7 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
         listings = glob.glob(os.path.join(tmp, "*gfx950*.s"))
         if not listings:
             raise RuntimeError("the build left no device assembly to check")
-        report = {}
+        report, spilling = {}, []
         for path in listings:
             hits = find_masked_copies(path)
             if hits:
@@ -195,19 +195,20 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), out_path: 
                 raise RuntimeError(f"{os.path.basename(path)} holds {packed.group(0)}")
             res = kernel_resources(path)
             for mangled, plain in zip(res, _demangle(list(res))):
-                report[plain.replace("(anonymous namespace)::", "")] = res[mangled]
-        # template arguments of mg_tile_kernel: view, see-through, MODE (0 = step), ...
-        # (a private segment without spilled vector registers is a frame object the compiler reserved and then never
-        # touched - the listing has no scratch instruction for it; it is reported, not refused)
-        spilling = [k for k, r in report.items() if "mg_tile_kernel" in k and r["vgpr_spill_count"]]
+                name = plain.replace("(anonymous namespace)::", "")
+                report[name] = res[mangled]  # template arguments of mg_tile_kernel: view, see-through, MODE (0 = step), ...
+                # (a private segment without spilled vector registers is a frame object the compiler reserved and then
+                # never touched - the listing has no scratch instruction for it; it is reported, not refused)
+                if res[mangled]["vgpr_spill_count"] and ("mg_tile_kernel" in name or "policy" in os.path.basename(path)):
+                    spilling.append((name, res[mangled]))
         if verbose:
             for k in sorted(report):
                 r = report[k]
                 print(f"  {r['vgpr_count']:3d} vgpr {r['sgpr_count']:3d} sgpr  spills {r['sgpr_spill_count']:3d} s / "
                       f"{r['vgpr_spill_count']:3d} v  scratch {r['private_segment_fixed_size']:4d} B  {k}")
         if spilling and os.environ.get("MGRID_ALLOW_SPILLS") != "1":  # (the switch is for work in progress only)
-            raise RuntimeError(f"{len(spilling)} instantiation(s) of the tile kernel spill vector registers to scratch "
-                               f"memory, e.g. {spilling[0]}: {report[spilling[0]]}")
+            raise RuntimeError(f"{len(spilling)} instantiation(s) of the tile or policy kernels spill vector registers to "
+                               f"scratch memory, e.g. {spilling[0][0]}: {spilling[0][1]}")
         # a new inode, renamed into place: processes that have the old library mapped keep the old file
         for built, place in ((out, target), (torch_out, TORCH_LIB_PATH)) if with_torch else ((out, target),):
             staged = f"{place}.tmp.{os.getpid()}"

@@ -1546,7 +1546,7 @@ struct DrawShared {
 template <class T, int LANES, int HELD>
 __device__ __forceinline__ int find_border(Row<T, LANES, HELD> &row, DrawShared &sh, const Spread &s, bool share, double border, double before, double &total) {
     constexpr int V = WIDE<T>, SPAN = LANES < 64 ? LANES : 64, WAVES = LANES > 64 ? LANES / 64 : 1;
-    const int wave = LANES > 64 ? threadIdx.x / 64 : 0, lane = row.lane % 64;
+    const int wave = LANES > 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0, lane = row.lane % 64;
     double part[HELD];
     row.each([&](int j, const uint32_t *v) {
         part[j] = s.of_vector<T>(v);
@@ -1715,7 +1715,7 @@ __device__ __forceinline__ void put_drawn(const MgLogits &l, int64_t row, int to
 }
 
 template <class T, int LANES, int HELD>
-__global__ __launch_bounds__(BLOCK<LANES>) void draw_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type, void *tokens, float *logprob) {
+__global__ __launch_bounds__(BLOCK<LANES>, HELD == 8 ? 4 : 1) void draw_kernel(MgLogits l, const T *logits, const void *uniforms, int uniforms_type, void *tokens, float *logprob) {
     __shared__ DrawShared sh;
     constexpr int ROWS = BLOCK<LANES> / LANES;
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
