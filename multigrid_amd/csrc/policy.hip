@@ -7,6 +7,9 @@
 //
 // Sums, maxima and probabilities are held in 32 bits (64 in the draw, where a token's borders decide); a value is
 // rounded to its type once, when it is stored.
+//
+// All of it is bound by memory or by launches.  On this card a copy of 1 GiB moves 5.1 TB/s (read and written together), a fill
+// 6.9, a sum reads 3.7 to 4.0; the smallest launch takes 3.5 us.  The times beside the kernels are theirs alone, without the host.
 
 #include <hip/hip_runtime.h>
 
@@ -265,7 +268,8 @@ struct EmbedArgs {
 };
 
 // One thread per 16 bytes of output; the threads of a token share its ids.  (Four tokens to a thread at once: no faster where
-// there are many tokens, half as fast at 8190.)
+// there are many tokens, half as fast at 8190.)  Bound by the writes and by the rows that the cache does not hold: 16384 tokens x
+// 2048 bfloat16 of 32000 rows 22 us (134 MB), 98 cells x 32 2.6 us.
 template <class T, class I>
 __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *ids, const T *table, T *out) {
     constexpr int V = WIDE<T>;
@@ -305,8 +309,9 @@ __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *id
 }
 
 // A table that LDS holds (cells: 24 rows): a block copies it there once, then takes `far` (up to FAR) tokens' ids at a time into LDS
-// as row numbers, and writes those tokens' outputs 16 bytes a thread, four tokens to a thread at once.  Bound by the writes; from memory
-// or L1 each output waited for a chain of id, row and store.
+// as row numbers, and writes those tokens' outputs 16 bytes a thread, four tokens to a thread at once.  Bound by the writes; with the
+// table in memory or L1 each output waits for a chain of id, row and store.  401408 cells x 64 float32: 22.6 us (103 MB, 4.6 TB/s),
+// 31.5 by embed_kernel.
 constexpr int TABLE_BYTES = 32768, FAR = 512, TABLE_BLOCKS = 2048, UNITS = 256;
 
 template <class T, class I>
@@ -368,7 +373,8 @@ __global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, int f
 }
 
 // The same where LDS holds the finished output of every combination of a token's ids, none included (cells: 12 x 7 x 8): worked
-// out once a block, then each 16 bytes of output are one read of LDS and one store.
+// out once a block, then each 16 bytes of output are one read of LDS and one store.  6422528 cells x 32 bfloat16: 86 us (430 MB, 5.0
+// TB/s), 110 by embed_table_kernel, 185 by embed_kernel.
 constexpr int COMBINED_BYTES = 53248, COMBINED_THREADS = 512, COMBINED_BLOCKS = 768;  // three blocks to a compute unit
 static_assert(FAR == COMBINED_THREADS, "a token's ids to each thread");
 
@@ -486,8 +492,12 @@ __device__ __forceinline__ uint32_t row_of(Id id, uint32_t base, uint32_t size, 
 // columns.  The indicator's fragment (row l % 16, tokens 8 (l / 16) ...) is made from eight row numbers by three packed 16-bit
 // instructions per pair; the gradient's fragment (column l % 16, the same tokens) comes straight from memory, W adjacent
 // columns of a token to a lane, so that product i of W covers columns W * (0 .. 15) + i and pairs of tokens meet by one byte
-// permutation each.  The order of the tokens within 32 is free: a load takes four adjacent tokens, whole lines of memory.  Waves and blocks stride over the tokens, a block adds its four waves, embed_join_kernel the blocks, all
-// in a fixed order.
+// permutation each.  The order of the tokens within 32 is free: a load takes four adjacent tokens, whole lines of memory.
+// Waves and blocks stride over the tokens, a block adds its four waves, embed_join_kernel the blocks, all in a fixed order.
+//
+// Bound by the reads: 6422528 cells x 32 bfloat16 122 us (430 MB with the ids, 3.5 TB/s), 401408 x 64 float32 36 us (104 MB, 2.9
+// TB/s: four or five turns of a wave, and their beginning and end).  By sorting the tokens these take 3250 and 172 us; with 64
+// rows and 8190 tokens x 1024 the two are equal (28 and 26 us), with 2000 tokens x 64 it is 10 against 20.
 //
 // 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
 // again, one after the other, each added to its own rows only.
@@ -736,6 +746,7 @@ __global__ __launch_bounds__(JOIN_COLS *JOIN_SHARES) void embed_join_kernel(cons
 // More rows: the entries (token n, field f) are sorted by row, order kept (a radix sort of up to 9 bits a pass), and the sorted
 // list is cut into chunks of equal length whatever the rows' frequencies are.  A chunk adds up its runs of equal rows; a run
 // that lies inside one chunk is finished there, one that passes a border leaves float32 parts for embed_span_kernel.
+// 8190 tokens, 30011 rows x 1024 bfloat16: sort 19 us, runs 10, spans 7.4.
 constexpr int MOST_BINS = 512, DIGIT = 9;
 
 // The entries e0, e0 + step, ... (N of them, those below `end`): row (a.rows where the id reads none) and token.
@@ -827,7 +838,9 @@ __device__ __forceinline__ void clear(char *out, int64_t bytes, int64_t block, i
     }
 }
 
-// Up to SORT_ONE entries and 2^18 - 1 rows: one workgroup sorts words of row << 14 | entry in LDS.
+// Up to SORT_ONE entries and 2^18 - 1 rows: one workgroup sorts words of row << 14 | entry in LDS, while others clear the output.
+// Bound by the one compute unit's instructions (the digits' comparison bit by bit); still the whole gradient of 8190 tokens x 64
+// takes 30 us so and 45 with the three kernels below for each digit, of 16384 tokens 42 and 47.
 constexpr int SORT_THREADS = 1024, SORT_ONE = 1 << 14, SORT_ROWS = (1 << 18) - 1;
 
 __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(EmbedArgs a, const void *ids, int ids_type, int entries, int passes, int bits,
@@ -1106,7 +1119,9 @@ __global__ __launch_bounds__(THREADS) void embed_span_kernel(EmbedArgs a, Sorted
 
 // Up to SHORT tokens (actions, not words) a thread has a row to itself, in registers: a wave's rows are adjacent in memory, so
 // its unaligned 16-byte loads use every line they touch, and no lane waits for another.  K is 8, 16 or SHORT; the tests
-// against the real number of tokens are the same for all lanes.
+// against the real number of tokens are the same for all lanes.  2^20 rows of 7 float32: draw 15 us, log-probabilities 14 and their
+// gradient 22, adjustment with a history of 16 entries and a mask 26 (40 to 60 MB each); with eight threads to a row, as for
+// longer ones, draw 100, log-probabilities 48, adjustment 101, and of 32 tokens still 90 against 55, 47 against 42, 99 against 87.
 constexpr int SHORT = 32;
 
 template <class T, int K>
@@ -1132,7 +1147,8 @@ __device__ __forceinline__ void store_row(T *p, int k, const float (&x)[K]) {
 // 16-byte vectors in registers, vector j * LANES + lane with each: one pass over memory, whose loads are all under way at
 // once; the maximum is known before the first exponential.  A row that no block holds is cut into pieces of
 // PIECE_LANES * PIECE_HELD vectors, each taken as a row, and a second kernel joins what they give: many blocks to a row also
-// where there are few rows.
+// where there are few rows.  At the border, 30011 bfloat16, one block to a row is faster still: one row 5.9 us against 9.4 in
+// pieces (log-probabilities), 11.3 against 12 (draw); 4095 rows 55 against 60 and 136 against 170.
 template <int LANES>
 constexpr int BLOCK = LANES > THREADS ? LANES : THREADS;
 constexpr int HELD_MOST = 4096, PIECE_LANES = 256, PIECE_HELD = 4;  // vectors of a row in one piece; a piece
@@ -1240,7 +1256,9 @@ constexpr float DEEP = -200.f;  // exp_twice of it is 0
 // A block counts a stretch of tokens' occurrences in their rows' histories in LDS, then the stretch streams through once: of
 // `lanes` threads to a row (a power of two) each takes up to STRETCH 16-byte vectors, whose loads are under way while the
 // history is counted.  Short rows share a block, a row longer than a block's stretch is cut, and each piece looks through the
-// whole history (a few KB that the cache holds).
+// whole history (a few KB that the cache holds).  The counters have 16 bits where the history has no more entries than that, so
+// that LDS holds eight blocks.  256 rows x 128000 bfloat16, 2048 entries, bits: 37.5 us (135 MB, 3.6 TB/s; 41 with 32-bit counters).
+// What keeps it from a copy's 5.1 TB/s is the chain in each block: history, barrier, counting, barrier, output.
 constexpr int STRETCH = 4;
 
 template <class T, class H, bool GRAD, class C>
@@ -1541,6 +1559,9 @@ struct DrawShared {
     int token;
 };
 
+// Bound by the exponentials in 64 bits where there are many long rows (4095 x 30011 bfloat16: 136 us; reading them 60), by
+// latency where there are few: 64 rows x 128003 float16 in pieces 11 us and their join 7.5.
+//
 // The token of a row (or of a piece of one) at whose sum of probabilities the border lies, known to all of its threads, and
 // the total.  `share`: the border is that share of the total; otherwise `border` is it, `before` what stands before the row.
 template <class T, int LANES, int HELD>
@@ -2003,6 +2024,8 @@ __global__ __launch_bounds__(BLOCK<LANES>) void logprob_kernel(MgLogits l, const
     }
 }
 
+// 4095 x 30011 bfloat16: 82 us (246 MB from memory, 3.0 TB/s; 55 us where the cache holds half of it).
+//
 // A long row's pieces, and their join by one wave.
 template <class T>
 __global__ __launch_bounds__(PIECE_LANES) void logprob_pieces_kernel(MgLogits l, const T *logits, float4 *pieces) {
@@ -2040,7 +2063,8 @@ __device__ __forceinline__ float logprob_slope(float x, bool is_token, float4 st
     return is_token ? -g * expm1f(lp) - p * hs : -p * (g + hs);
 }
 
-// One pass over the logits, `lanes` threads (a power of two) to a row or to a piece of one.
+// One pass over the logits, `lanes` threads (a power of two) to a row or to a piece of one.  Bound by memory: 4095 x 30011 bfloat16
+// 87 us (492 MB, 5.6 TB/s: part of the logits is still in the cache).
 template <class T>
 __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int lanes, const T *logits, const void *tokens, const float *stats,
                                                                const float *grad_lp, int64_t lp_stride, const float *grad_h, int64_t h_stride, T *out) {
@@ -2223,7 +2247,7 @@ GradPlan plan_grad(const EmbedArgs &a, int wide) {
         p.bytes += (bytes + 15) / 16 * 16;
         return at;
     };
-    p.few = a.rows <= FEW && a.row_stride <= FAR_ROWS && a.n >= 64;
+    p.few = a.rows <= FEW && a.row_stride <= FAR_ROWS && a.n >= 64;  // (a wave takes 64 tokens at a time)
     if (p.few) {
         p.width = wide / 2;  // the narrowest that holds a token's columns at once, or 8 bytes: two sets of 16 loads are held
         while (p.width > 1 && (16 * (p.width / 2) >= a.dim || p.width > a.dim)) p.width /= 2;
@@ -2453,18 +2477,20 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
         using I = decltype(i);
         const int vecs = (a.dim + WIDE<T> - 1) / WIDE<T>, per_block = THREADS / (vecs < THREADS ? vecs : THREADS);
         const int64_t held = static_cast<int64_t>(a.rows + 1) * vecs * 16;
-        // what a block prepares has to be little beside the tokens it then writes: sixteen times as many, and a few blocks' tokens
-        // for a table alone
+        // What a block prepares has to be little beside the tokens that it then writes.  Combinations: sixteen tokens for each, at a
+        // block to a compute unit (401408 cells x 32, a tenth of that: 17.5 us by embed_combined_kernel, 11.1 by
+        // embed_table_kernel).  A table: a full share of tokens for every compute unit (100352 cells x 32: 6.3 us with it, 5.9 by
+        // embed_kernel; 401408: 11.1 and 12.6).
         int64_t combined = 1;
         for (int f = 0; f < a.fields; ++f) combined = combined * (a.sizes[f] + 1) <= (1 << 15) ? combined * (a.sizes[f] + 1) : 1 << 15;
         const int64_t combined_bytes = (combined + a.rows + 1) * vecs * 16 + FAR * 2;
-        if (combined_bytes <= COMBINED_BYTES && a.n >= 16 * combined * 256) {
+        if (combined_bytes <= COMBINED_BYTES && a.n >= 16 * combined * UNITS) {
             hipLaunchKernelGGL((embed_combined_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, COMBINED_BLOCKS)), dim3(COMBINED_THREADS),
                                combined_bytes, static_cast<hipStream_t>(stream), a, static_cast<int>(combined),
                                static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
             return;
         }
-        if (held <= TABLE_BYTES && a.n >= 4 * FAR) {
+        if (held <= TABLE_BYTES && a.n >= UNITS * FAR) {
             // as many tokens to a block as give every compute unit the same number of blocks
             const int64_t rounds = (a.n + UNITS * FAR - 1) / (UNITS * FAR), share = (a.n + UNITS * rounds - 1) / (UNITS * rounds);
             const int far = static_cast<int>(share + per_block - 1 < FAR ? (share + per_block - 1) / per_block * per_block : FAR);

@@ -43,7 +43,7 @@ def some_ids(g, n, sizes, dtype, outside=True):
 
 EMBED = [  # tokens, sizes of the fields, dim
     (1, (1,), 1), (1, (24,), 5), (98, (11, 6, 7), 32), (63, (11, 6, 7), 16), (257, (11, 6, 7), 7), (1000, (11, 6, 7), 130),
-    (150001, (700,), 8), (70000, (11, 6, 7), 16), (40000, (2, 3), 8), (70000, (7,), 9), (30000, (300, 2, 5000), 20), (5, (300,), 1), (64, (2, 3), 8), (65, (1, 1, 1, 1, 1, 1, 1, 1), 3), (333, (64,), 40), (333, (65,), 33), (1025, (997,), 264),
+    (150001, (700,), 8), (70000, (11, 6, 7), 16), (140000, (11, 6, 7), 7), (131072, (30, 3), 24), (60000, (2, 3), 8), (63, (24,), 16), (64, (24,), 17), (127, (11, 6, 7), 40), (40000, (2, 3), 8), (70000, (7,), 9), (30000, (300, 2, 5000), 20), (5, (300,), 1), (64, (2, 3), 8), (65, (1, 1, 1, 1, 1, 1, 1, 1), 3), (333, (64,), 40), (333, (65,), 33), (1025, (997,), 264),
     (2049, (33, 200, 70), 24), (6000, (5000,), 9), (40, (131072,), 64), (3, (7,), 5000), (5000, (17,), 64), (20000, (11, 6, 7), 64),
 ]
 
