@@ -560,8 +560,8 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 || FIELDS > 3 ? 2 : 3) 
     const uint32_t stride = static_cast<uint32_t>(a.row_stride) * sizeof(T), own = quad * stride + (d0 + from_col) * sizeof(T);  // bytes, see FAR_ROWS
     // No load stands behind a branch: it would be waited for at the branch's end, and with it all that were on their way before.
     // So the last 64 tokens stand for a wave that passes the end (tokens of another wave's are given no row), the last field for
-    // those that are not there, and of an id the aligned word that holds it, or its lower half, is read, and an upper half, which
-    // only int64 has.
+    // those that are not there, and of an id the aligned word that holds it (its other bytes, the tensor's or not, are in the same
+    // page), or its lower half, is read, and an upper half, which only int64 has.
     const int id_shift = ids_type == MG_U8 ? 0 : (ids_type == MG_I32 ? 2 : 3);
     const uint32_t id_mask = ids_type == MG_U8 ? 0xFF : ~0u, high_mask = ids_type == MG_I64 ? ~0u : 0;
     auto id_at = [&](int64_t t0, int f) {

@@ -872,3 +872,46 @@ def test_capture_beside_an_eager_graph_of_the_same_leaf(policy):
         torch.cuda.synchronize()
         assert torch.equal(got, want)
     assert torch.equal(mark, x + 1)
+
+
+@pytest.mark.parametrize("t", [65535, 65536, 70001])
+@pytest.mark.parametrize("k", [20, 40])
+def test_adjust_counts_beyond_16_bits(policy, t, k):
+    # one token throughout, in one row; its neighbours' counts must not see it
+    x = randn(gen(t), 2, k)
+    history = torch.full((2, t), 3)
+    history[1] = torch.arange(t) % k
+    y = policy.adjust_logits(x.to(DEV), history=history.to(DEV), repetition=1.25, presence=0.5, frequency=2.0 ** -12)
+    want, err, _ = ref.adjust(x, history, None, 1.25, 0.5, 2.0 ** -12)
+    ref.close(y, want, err, torch.float32)
+
+
+def test_the_longest_rows(policy):
+    k = 1 << 24
+    x = torch.zeros((1, k), dtype=torch.bfloat16)
+    x[0, 5], x[0, k - 1] = 3.0, 17.0
+    total = (k - 2) + math.exp(3.0) + math.exp(17.0)
+    d = x.to(DEV).requires_grad_()
+    # a border in the middle of the equal ones, and one behind them
+    for u, token in ((0.25 * (k - 2) / total, None), (0.9, k - 1), (None, k - 1)):
+        got, lp = policy.draw(d.detach(), None if u is None else torch.tensor([u], dtype=torch.float64, device=DEV))
+        if token is None:  # tokens 0 .. j hold j plus the sixth's surplus
+            token = math.floor(u * total - (math.exp(3.0) - 1.0))
+            assert abs(int(got) - token) <= 1  # (one step where the product above is rounded the other way)
+            assert abs(float(lp) + math.log(total)) < 1e-5
+        else:
+            assert int(got) == token
+    lp, h = policy.token_logprobs(d, torch.tensor([k - 1], device=DEV))
+    # relative to the sum: 32 additions in a thread, 8 levels of a block, 38 merges of four roundings, which make 192; an exponent of
+    # up to 17 log2(e), rounded twice, 50 more: 256 half steps; the entropy is a mean of exponents of up to 17 on top of it
+    off = 256 * 2.0 ** -24
+    assert abs(float(lp.detach()) - (17.0 - math.log(total))) < off
+    p = (math.exp(17.0) / total, math.exp(3.0) / total, 1.0 / total)
+    entropy = -(p[0] * math.log(p[0]) + p[1] * math.log(p[1]) + (k - 2) * p[2] * math.log(p[2]))
+    assert abs(float(h.detach()) - entropy) < off * (1.0 + 2 * 17.0)
+    grad, = torch.autograd.grad(lp, d)
+    assert grad.shape == d.shape and abs(float(grad[0, k - 1]) - (1.0 - p[0])) < 2.0 ** -8 and abs(float(grad[0, 7]) + p[2]) < p[2] * 2.0 ** -7
+    y = policy.adjust_logits(d.detach(), history=torch.tensor([[5, k - 1, k, -1]], device=DEV), presence=2.0)
+    assert float(y[0, 5]) == 1.0 and float(y[0, k - 1]) == 15.0 and float(y.float().sum()) == 16.0
+    with pytest.raises(ValueError, match="not supported"):
+        policy.draw(torch.empty((1, k + 1), dtype=torch.bfloat16, device=DEV))
