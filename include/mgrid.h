@@ -335,6 +335,8 @@ typedef struct MgEmbed {
     int32_t sizes[MG_MAX_FIELDS]; /* every one positive, their sum at most 2^30 */
     float scale;
     int32_t reserved0;            /* must be 0 */
+    void *ids_copy_dev;           /* [n][fields], contiguous, in the ids' type: mg_embed writes the ids there as well (for a
+                                     backward pass after the ids were overwritten); NULL: it does not.  mg_embed_grad ignores it */
 } MgEmbed;
 
 /* out [n][dim], contiguous. */

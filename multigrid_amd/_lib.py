@@ -61,7 +61,7 @@ class MgLayoutSpec(ctypes.Structure):
 class MgEmbed(ctypes.Structure):
     _fields_ = [("n", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("fields", "dim", "ids_type", "dtype")] + [
         (n, ctypes.c_int64) for n in ("ids_stride", "field_stride", "row_stride")] + [
-        ("sizes", ctypes.c_int32 * MAX_FIELDS), ("scale", ctypes.c_float), ("reserved0", ctypes.c_int32)]
+        ("sizes", ctypes.c_int32 * MAX_FIELDS), ("scale", ctypes.c_float), ("reserved0", ctypes.c_int32), ("ids_copy_dev", ctypes.c_void_p)]
 
 
 class MgAdjust(ctypes.Structure):

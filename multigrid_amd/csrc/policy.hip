@@ -271,7 +271,7 @@ struct EmbedArgs {
 // there are many tokens, half as fast at 8190.)  Bound by the writes and by the rows that the cache does not hold: 16384 tokens x
 // 2048 bfloat16 of 32000 rows 22 us (134 MB), 98 cells x 32 2.6 us.
 template <class T, class I>
-__global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *ids, const T *table, T *out) {
+__global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *ids, const T *table, T *out, I *ids_copy) {
     constexpr int V = WIDE<T>;
     const int vecs = (a.dim + V - 1) / V;
     const int cols = min(vecs, THREADS), per_block = THREADS / cols;
@@ -305,6 +305,8 @@ __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *id
             else
                 sum([&](const T *from, float (&x)[V]) { load_part<T, V>(from, a.dim - d0, a.dim, x); });
         }
+        if (ids_copy && col == 0)
+            for (int f = 0; f < a.fields; ++f) ids_copy[n * a.fields + f] = id_at[f * a.field_stride];
     }
 }
 
@@ -315,7 +317,7 @@ __global__ __launch_bounds__(THREADS) void embed_kernel(EmbedArgs a, const I *id
 constexpr int TABLE_BYTES = 32768, FAR = 512, TABLE_BLOCKS = 2048, UNITS = 256;
 
 template <class T, class I>
-__global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, int far, const I *ids, const T *table, T *out) {
+__global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, int far, const I *ids, const T *table, T *out, I *ids_copy) {
     constexpr int V = WIDE<T>, TOGETHER = 4;
     extern __shared__ __align__(16) char lds[];
     const int vecs = (a.dim + V - 1) / V, pitch = vecs * V;
@@ -343,6 +345,7 @@ __global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, int f
             for (int j = 0; j < FAR / THREADS; ++j) {
                 const int64_t v = static_cast<int64_t>(id[j]);
                 rows_s[f * FAR + j * THREADS + threadIdx.x] = static_cast<uint16_t>(v >= 0 && v < a.sizes[f] ? base + v : a.rows);
+                if (ids_copy && j * THREADS + static_cast<int>(threadIdx.x) < tokens) ids_copy[(n0 + j * THREADS + threadIdx.x) * a.fields + f] = id[j];
             }
             base += a.sizes[f];
         }
@@ -372,18 +375,35 @@ __global__ __launch_bounds__(THREADS) void embed_table_kernel(EmbedArgs a, int f
     }
 }
 
+// the ids to a contiguous copy, by all blocks of a launch
+template <class I>
+__device__ __forceinline__ void copy_ids(const EmbedArgs &a, const I *ids, I *to) {
+    constexpr int V = 16 / static_cast<int>(sizeof(I));
+    const int64_t all = a.n * a.fields, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (a.ids_stride == a.fields && a.field_stride == 1) {
+        for (int64_t i = e * V; i + V <= all; i += step * V) *reinterpret_cast<Vec<I, V> *>(to + i) = *reinterpret_cast<const Vec<I, V> *>(ids + i);
+        e += all / V * V;
+    }
+    for (; e < all; e += step) {
+        const int64_t n = e / a.fields;
+        to[e] = ids[n * a.ids_stride + (e - n * a.fields) * a.field_stride];
+    }
+}
+
 // The same where LDS holds the finished output of every combination of a token's ids, none included (cells: 12 x 7 x 8): worked
-// out once a block, then each 16 bytes of output are one read of LDS and one store.  6422528 cells x 32 bfloat16: 86 us (430 MB, 5.0
+// out once a block, then each 16 bytes of output are one read of LDS and one store.  6422528 cells x 32 bfloat16: 84 us (430 MB, 5.1
 // TB/s), 110 by embed_table_kernel, 185 by embed_kernel.
 constexpr int COMBINED_BYTES = 53248, COMBINED_THREADS = 512, COMBINED_BLOCKS = 768;  // three blocks to a compute unit
 static_assert(FAR == COMBINED_THREADS, "a token's ids to each thread");
 
 template <class T, class I>
-__global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedArgs a, int combined, const I *ids, const T *table, T *out) {
+__global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedArgs a, int combined, const I *ids, const T *table, T *out, I *ids_copy) {
     constexpr int V = WIDE<T>, TOGETHER = 4;
     extern __shared__ __align__(16) char lds[];
     const int vecs = (a.dim + V - 1) / V, pitch = vecs * V;
     T *done_s = reinterpret_cast<T *>(lds), *table_s = done_s + combined * pitch;  // [combined][pitch], [rows + 1][pitch]
+    if (ids_copy) copy_ids(a, ids, ids_copy);  // (a stream of its own, before the others: 4 us; a launch of its own 10, beside each token's output 17)
     uint16_t *which_s = reinterpret_cast<uint16_t *>(table_s + (a.rows + 1) * pitch);
     for (int i = threadIdx.x; i < (a.rows + 1) * pitch; i += COMBINED_THREADS) {
         const int r = i / pitch, d = i - r * pitch;
@@ -2475,6 +2495,7 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
     with_types(e->dtype, e->ids_type, [&](auto t, auto i) {
         using T = decltype(t);
         using I = decltype(i);
+        I *ids_copy = static_cast<I *>(e->ids_copy_dev);
         const int vecs = (a.dim + WIDE<T> - 1) / WIDE<T>, per_block = THREADS / (vecs < THREADS ? vecs : THREADS);
         const int64_t held = static_cast<int64_t>(a.rows + 1) * vecs * 16;
         // What a block prepares has to be little beside the tokens that it then writes.  Combinations: sixteen tokens for each, at a
@@ -2487,7 +2508,7 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
         if (combined_bytes <= COMBINED_BYTES && a.n >= 16 * combined * UNITS) {
             hipLaunchKernelGGL((embed_combined_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, COMBINED_BLOCKS)), dim3(COMBINED_THREADS),
                                combined_bytes, static_cast<hipStream_t>(stream), a, static_cast<int>(combined),
-                               static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
+                               static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev), ids_copy);
             return;
         }
         if (held <= TABLE_BYTES && a.n >= UNITS * FAR) {
@@ -2495,12 +2516,12 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
             const int64_t rounds = (a.n + UNITS * FAR - 1) / (UNITS * FAR), share = (a.n + UNITS * rounds - 1) / (UNITS * rounds);
             const int far = static_cast<int>(share + per_block - 1 < FAR ? (share + per_block - 1) / per_block * per_block : FAR);
             hipLaunchKernelGGL((embed_table_kernel<T, I>), dim3(blocks_for((a.n + far - 1) / far, TABLE_BLOCKS)), dim3(THREADS), held + a.fields * FAR * 2,
-                               static_cast<hipStream_t>(stream), a, far, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev));
+                               static_cast<hipStream_t>(stream), a, far, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev), ids_copy);
             return;
         }
         hipLaunchKernelGGL((embed_kernel<T, I>), dim3(blocks_for((a.n + per_block - 1) / per_block)), dim3(THREADS), 0,
                            static_cast<hipStream_t>(stream), a, static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev),
-                           static_cast<T *>(out_dev));
+                           static_cast<T *>(out_dev), ids_copy);
     });
     return launched("mg_embed");
 }

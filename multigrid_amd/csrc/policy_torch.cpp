@@ -183,12 +183,17 @@ Lookup lookup(const Tensor &ids, const Fields &fields, int64_t rows, int64_t dim
     return l;
 }
 
-Tensor embed_forward(const Tensor &ids, const Tensor &given, const Fields &fields, double scale) {
+// `copy`: set to a copy of the ids, written by the same launch
+Tensor embed_forward(const Tensor &ids, const Tensor &given, const Fields &fields, double scale, Tensor *copy = nullptr) {
     const Tensor table = given.stride(1) == 1 || given.size(1) == 1 ? given : given.contiguous();
     Lookup l = lookup(ids, fields, table.size(0), table.size(1), floating("table", table), scale);
     l.e.row_stride = row_stride(table);
     l.shape.push_back(table.size(1));
     Tensor out = at::empty(l.shape, table.options());
+    if (copy) {
+        *copy = at::empty(ids.sizes(), ids.options());
+        l.e.ids_copy_dev = address(*copy);
+    }
     if (out.numel()) {
         On on(table);
         check(entry.embed(&l.e, address(l.ids), address(table), address(out), on.stream));
@@ -213,12 +218,14 @@ Tensor embed_grad(const Tensor &grad, const Tensor &ids, int64_t rows, const Fie
 
 struct Embed : torch::autograd::Function<Embed> {
     static Tensor forward(AutogradContext *ctx, const Tensor &ids, const Tensor &table, const Fields &fields, double scale) {
-        // a copy: the simulator writes its images in place, where no version is counted
-        ctx->save_for_backward({ids.clone()});
+        // a copy of the ids is kept: the simulator writes its images in place, where no version is counted
+        Tensor copy;
+        Tensor out = embed_forward(ids, table, fields, scale, &copy);
+        ctx->save_for_backward({copy});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["rows"] = table.size(0);
         ctx->saved_data["fields"] = fields ? c10::IValue(*fields) : c10::IValue();
-        return embed_forward(ids, table, fields, scale);
+        return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         once();

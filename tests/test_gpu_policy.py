@@ -915,3 +915,21 @@ def test_the_longest_rows(policy):
     assert float(y[0, 5]) == 1.0 and float(y[0, k - 1]) == 15.0 and float(y.float().sum()) == 16.0
     with pytest.raises(ValueError, match="not supported"):
         policy.draw(torch.empty((1, k + 1), dtype=torch.bfloat16, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int64])
+@pytest.mark.parametrize("n,sizes", [(1, (5,)), (101, (11, 6, 7)), (140003, (11, 6, 7)), (60005, (2, 3)), (60007, (7,)), (501, (200, 30))])
+def test_the_backward_pass_has_the_ids_of_the_forward_pass(policy, n, sizes, dtype):
+    # every way of embedding writes the copy itself: ids side by side, apart, and the same for all tokens
+    g = gen(n)
+    wide = torch.stack([torch.randint(0, r + 1, (n, 2), generator=g) for r in sizes], -1).to(dtype).to(DEV)  # [n, 2, fields]
+    w, up = randn(g, sum(sizes), 16).to(DEV).requires_grad_(), randn(g, n, 16).to(DEV)
+    for ids in (wide[:, 0].contiguous(), wide[:, 1], wide[:1, 0].expand(n, -1)):
+        want = policy.embed_grad(up, ids.clone(), sum(sizes), fields=sizes)
+        y = policy.embed(ids, w, fields=sizes)
+        with torch.no_grad():
+            assert torch.equal(policy.embed(ids, w, fields=sizes), y)
+        kept = wide.clone()
+        ids[:1].fill_(0) if ids.stride(0) == 0 else ids.fill_(0)
+        assert torch.equal(torch.autograd.grad(y, w, up)[0], want)
+        wide.copy_(kept)
