@@ -101,8 +101,9 @@ void no_gradient(const char *name, const Number &v) {
 // current when the first graph that holds the leaf was built.  Where that is the default stream, the captured backward pass
 // would order work behind it, which no capture allows and no one catches.
 void no_leaf_of_the_default_stream(const Tensor &t) {
+    const auto current = c10::hip::getCurrentHIPStream(t.device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(t.device().index()).stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (current.id() == 0 || hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;  // (the default stream is never captured)
     std::vector<std::shared_ptr<torch::autograd::Node>> rest;
     std::unordered_set<torch::autograd::Node *> seen;
     if (auto first = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t)) rest.push_back(std::move(first));
@@ -112,7 +113,7 @@ void no_leaf_of_the_default_stream(const Tensor &t) {
         if (!seen.insert(node.get()).second) continue;
         const auto stream = node->stream();
         TORCH_CHECK(!stream || stream->id() != 0, "a differentiable call is captured, but what it depends on belongs to an eager graph of the default stream as well (", node->name(),
-                    "): let that graph go first (del its outputs), or build it on another stream");
+                    "): let that graph go first (del its outputs)");
         for (const auto &edge : node->next_edges())
             if (edge.function) rest.push_back(edge.function);
     }
