@@ -2077,12 +2077,27 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(MgLogits l, const T *l
     }
 }
 
-// g, h: the row's gradients divided by its temperature.  One product with p, the smallest factor, and that last: a p below
-// 2^-126 has few bits left, which a second rounding would halve.
-__device__ __forceinline__ float logprob_slope(float x, bool is_token, float4 st, float inv_t, float g, float h) {
+// A row's incoming gradients g (of the log-probability) and h (of the entropy), divided by its temperature.  Where that could pass the
+// largest float (a temperature below 1, and a gradient above 4 at the least one) they stay as they are and `after` is 1 / T: infinity
+// times a probability of 0 would be NaN.  512 is more than |log p + entropy| comes to, see LEAST_LOGPROB.
+struct Incoming {
+    float g, h, after;
+};
+__device__ __forceinline__ Incoming incoming(float g, float h, float inv_t) {
+    const bool fits = (fabsf(g) + 512.f * fabsf(h)) * inv_t < -NEG_INF;
+    return fits ? Incoming{g * inv_t, h * inv_t, 1.f} : Incoming{g, h, inv_t};
+}
+// A log-probability where it multiplies: from here on p is 0, and 0 times -infinity (a logit of the type's lowest value at a temperature
+// below 1) would be NaN.
+constexpr float LEAST_LOGPROB = 2.f * DEEP;
+
+// One product with p, the smallest factor, and that last: a p below 2^-126 has few bits left, which a second rounding would halve.
+// (Where `after` is not 1, g or 512 h is above 4: their product with p has no fewer bits than p.)  A row that is NaN has it in st.z,
+// which nothing clamps.
+__device__ __forceinline__ float logprob_slope(float x, bool is_token, float4 st, float inv_t, const Incoming &in) {
     if (x == NEG_INF) return 0.f;
-    const float lp = (x - st.x) * inv_t - st.y, p = expf(lp), hs = h * (lp + st.z);
-    return is_token ? -g * expm1f(lp) - p * hs : -p * (g + hs);
+    const float lp = (x - st.x) * inv_t - st.y, p = expf(lp), hs = in.h * (fmaxf(lp, LEAST_LOGPROB) + st.z);
+    return (is_token ? -in.g * expm1f(lp) - p * hs : -p * (in.g + hs)) * in.after;
 }
 
 // One pass over the logits, `lanes` threads (a power of two) to a row or to a piece of one.  Bound by memory: 4095 x 30011 bfloat16
@@ -2105,9 +2120,10 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int l
         const float4 st = reinterpret_cast<const float4 *>(stats)[row];
         const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
         const float grad_of_lp = grad_lp ? grad_lp[row * lp_stride] : 0.f, grad_of_h = grad_h ? grad_h[row * h_stride] : 0.f;
-        const float inv_t = 1.f / temperature, g = token >= 0 && token < l.k ? grad_of_lp * inv_t : 0.f, h = grad_of_h * inv_t;
+        const float inv_t = 1.f / temperature;
+        const Incoming in = incoming(token >= 0 && token < l.k ? grad_of_lp : 0.f, grad_of_h, inv_t);
         // what a p of 0 must not hide: NaN where the row has one
-        const float whole = fmaf(h, st.z, g);
+        const float whole = fmaf(in.h, st.z, in.g);
 #pragma unroll
         for (int j = 0; j < TAKES; ++j) {
             const int at = first + (j * lanes + lane) * V;
@@ -2115,11 +2131,11 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int l
             float v[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float at_i = element<T>(w[j], i), lp = fmaxf((at_i - st.x) * inv_t - st.y, 2.f * DEEP), p = exp_twice(lp * HALF_LOG2E);
-                v[i] = at_i == NEG_INF ? 0.f : -p * fmaf(h, lp, whole);
+                const float at_i = element<T>(w[j], i), lp = fmaxf((at_i - st.x) * inv_t - st.y, LEAST_LOGPROB), p = exp_twice(lp * HALF_LOG2E);
+                v[i] = at_i == NEG_INF ? 0.f : -p * fmaf(in.h, lp, whole) * in.after;
             }
             if (token >= at && token < at + V) {
-                const float own = logprob_slope(static_cast<float>(x[token]), true, st, inv_t, g, h);
+                const float own = logprob_slope(static_cast<float>(x[token]), true, st, inv_t, in);
 #pragma unroll
                 for (int i = 0; i < V; ++i)
                     if (at + i == token) v[i] = own;
@@ -2176,11 +2192,12 @@ __global__ __launch_bounds__(THREADS) void logprob_grad_short_kernel(MgLogits l,
     const float temperature = temperature_of(l, row);
     const int64_t token = grad_lp ? get_token(tokens, l.tokens_type, row) : -1;
     const float grad_of_lp = grad_lp ? grad_lp[row * lp_stride] : 0.f, grad_of_h = grad_h ? grad_h[row * h_stride] : 0.f;
-    const float inv_t = 1.f / temperature, g = token >= 0 && token < l.k ? grad_of_lp * inv_t : 0.f, h = grad_of_h * inv_t;
+    const float inv_t = 1.f / temperature;
+    const Incoming in = incoming(token >= 0 && token < l.k ? grad_of_lp : 0.f, grad_of_h, inv_t);
     const float4 st = row_stats(soft_short<K>(x, l.k, inv_t));
 #pragma unroll
     for (int j = 0; j < K; ++j)
-        if (j < l.k) x[j] = logprob_slope(x[j], j == token, st, inv_t, g, h);
+        if (j < l.k) x[j] = logprob_slope(x[j], j == token, st, inv_t, in);
     store_row<T, K>(out + row * l.k, l.k, x);
 }
 

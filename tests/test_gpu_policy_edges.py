@@ -1,0 +1,120 @@
+"""The policy operators at the edges of their arguments: lowest values as a mask, the smallest temperatures and repetitions,
+infinite penalties, tensors that autograd watches, batches that another kernel takes."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import policy_util as ref  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def policy():
+    from multigrid_amd import policy
+    return policy
+
+
+def gen(seed):
+    return torch.Generator(device="cpu").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g)
+
+
+def held(want, dtype):
+    """Numbers of 64 bits, infinite where `dtype` holds none so large."""
+    most = torch.finfo(dtype).max * (1 + ref.HALF_STEP[dtype] / 2)
+    return np.where(np.abs(want) > most, np.copysign(np.inf, want), want)
+
+
+def close_held(got, want, err, dtype):
+    want = held(want, dtype)
+    ref.close(got, want, np.where(np.isfinite(want) & np.isfinite(err), err, 0.0), dtype)
+
+
+def number(t):
+    return t if isinstance(t, torch.Tensor) else float(np.float32(t))
+
+
+def to_gpu(t):
+    return t.to(DEV) if isinstance(t, torch.Tensor) else t
+
+
+# ---- gradient of the log-probabilities -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(12, 2), (300, 7), (40, 16), (40, 32), (40, 33), (12, 1000), (12, 9001), (3, 70000)])
+def test_logprob_gradient_of_rows_masked_by_the_lowest_value(policy, n, k, dtype):
+    """Barred places hold the type's lowest finite value beside ordinary logits, as masks of many programs write them: their
+    probability is 0 and so is their gradient, whatever the entropy's share and also where the answer itself is barred."""
+    g = gen(n * 3 + k)
+    x = randn(g, n, k).to(dtype)
+    barred = torch.rand((n, k), generator=g) < 0.4
+    barred[torch.arange(n), torch.randint(0, k, (n,), generator=g)] = False
+    x[barred] = torch.finfo(dtype).min
+    tokens = torch.randint(0, k, (n,), generator=g)
+    for i in range(n):  # every other answer is an allowed one, the others as often barred as not
+        if i % 2:
+            tokens[i] = int(torch.nonzero(~barred[i])[0])
+    up, up_h = randn(g, n), randn(g, n) * 8
+    for temperature in (1.0, 0.75, 0.5 + torch.rand(n, generator=g)):
+        leaf = x.to(DEV).requires_grad_()
+        lp, h = policy.token_logprobs(leaf, tokens.to(DEV), temperature=to_gpu(temperature))
+        want = ref.logprobs(x, tokens, number(temperature), up, up_h)
+        close_held(lp, *want[0], torch.float32)
+        ref.close(h, *want[1], torch.float32)
+        gone = barred.clone()
+        gone[torch.arange(n), tokens] = False
+        for outs, ups, (a, b) in (((lp, h), (up, up_h), (up, up_h)), ((lp,), (up,), (up, 0 * up_h)), ((h,), (up_h,), (0 * up, up_h))):
+            dx, = torch.autograd.grad(outs, leaf, tuple(u.to(DEV) for u in ups), retain_graph=True)
+            d, err = ref.logprobs(x, tokens, number(temperature), a, b)[2]
+            assert bool((dx.cpu()[gone] == 0).all())
+            seen = ~gone.numpy()
+            # (the bound of a probability that is 0 in 64 bits too, times a logarithm of 1e38, would be no bound)
+            close_held(dx.cpu()[~gone], d[seen], np.where(barred.numpy(), np.abs(d) * 4 * ref.U32, err)[seen], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [2, 7, 32, 33, 1000, 70000])
+def test_logprob_gradient_at_the_smallest_temperatures(policy, k, dtype):
+    """A temperature that the operator takes gives the gradient of its formula: 0 where a probability is 0, also where the
+    incoming gradient divided by the temperature passes the largest float32, and infinite only where the gradient itself does."""
+    n = 8
+    g = gen(k)
+    x = randn(g, n, k)
+    x[1], x[1, 0], x[1, k - 1] = -1.0, 2.0, 2.0  # two equal maxima
+    x[2] = 0.5
+    t = torch.tensor([2.0 ** -126, 2.0 ** -126, 2.0 ** -126, 2.0 ** -126, 1e-30, 1e-30, 1e-20, 2.0 ** -126])
+    x = x.to(dtype)
+    if dtype != torch.float16:  # logits as near to each other as the temperature is small
+        x[4:6] = (randn(g, 2, k) * 1e-30).to(dtype)
+        x[6] = (randn(g, k) * 1e-20).to(dtype)
+    tokens = torch.tensor([0, 0, k - 1, 0, 0, 0, 0, 0])
+    tokens[0], tokens[3] = int(x[0].float().argmax()), int(x[3].float().argmin())
+    tokens[7] = int(x[7].float().argmax())
+    up = torch.tensor([1.0, 1.0, -2.0, 0.5, 1e10, 1e10, 3.0, 100.0])
+    up_h = torch.tensor([1.0, 0.0, 2.0, -0.01, 0.0, 1e9, 5.0, -100.0])
+    leaf = x.to(DEV).requires_grad_()
+    lp, h = policy.token_logprobs(leaf, tokens.to(DEV), temperature=t.to(DEV))
+    want = ref.logprobs(x, tokens, t, up, up_h)
+    close_held(lp, *want[0], torch.float32)
+    ref.close(h, *want[1], torch.float32)
+    for a, b in ((up, up_h), (up, 0 * up_h), (0 * up, up_h)):
+        dx, = torch.autograd.grad((lp, h), leaf, (a.to(DEV), b.to(DEV)), retain_graph=True)
+        assert not torch.isnan(dx).any()
+        with np.errstate(invalid="ignore", over="ignore"):
+            d, err = ref.logprobs(x, tokens, t, a, b)[2]
+            p = np.exp((ref.np64(x) - ref.np64(x).max(1, keepdims=True)) / t.double().numpy()[:, None])
+        none = (p == 0) & (np.arange(k)[None] != tokens.numpy()[:, None])
+        assert bool((dx.cpu().double().numpy()[none] == 0).all())
+        # (a probability of 0 times a logarithm of 1e38 bounds nothing)
+        close_held(dx.cpu()[torch.from_numpy(~none)], d[~none], np.where(p == 0, np.abs(d) * 4 * ref.U32, err)[~none], dtype)
