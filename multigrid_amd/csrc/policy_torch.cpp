@@ -364,6 +364,8 @@ Tensor adjust_forward(const Tensor &logits, const Maybe &into, const Maybe &hist
         On on(logits);
         check(entry.adjust(&d.a, address(x), address(out), on.stream));
     }
+    // a write that autograd counts: a graph that has kept the tensor raises instead of using the new values (inference tensors count none)
+    if (into && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 

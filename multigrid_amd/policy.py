@@ -80,7 +80,8 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     ``[ceil(k / 32)]`` or ``[..., ceil(k / 32)]``, lowest bit first; everything else becomes -inf, also all of a row.
 
     Differentiable with respect to the logits.  ``out`` (contiguous, may be the logits) is written instead of a new
-    tensor, then nothing is differentiable."""
+    tensor, then nothing is differentiable; a backward pass that has kept ``out``'s old values raises RuntimeError, as after
+    torch's own operations in place (the replay of a captured graph writes uncounted)."""
     return (_bound or _native()).adjust_logits(logits, history, lengths, repetition, presence, frequency, bias, mask, out)
 
 

@@ -118,3 +118,46 @@ def test_logprob_gradient_at_the_smallest_temperatures(policy, k, dtype):
         assert bool((dx.cpu().double().numpy()[none] == 0).all())
         # (a probability of 0 times a logarithm of 1e38 bounds nothing)
         close_held(dx.cpu()[torch.from_numpy(~none)], d[~none], np.where(p == 0, np.abs(d) * 4 * ref.U32, err)[~none], dtype)
+
+
+# ---- tensors that autograd watches -----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("k", [7, 33, 9001])
+def test_out_counts_as_a_write(policy, k):
+    """A tensor that a graph has kept and that ``out`` overwrites makes the graph's backward pass raise, as torch's own
+    operations in place do: a gradient from the new values would be wrong."""
+    g = gen(k)
+    tokens, mask = torch.randint(0, k, (5,), generator=g).to(DEV), torch.rand((5, k), generator=g).to(DEV) < 0.6
+    for keeps in (lambda z: policy.token_logprobs(z, tokens)[0], lambda z: policy.token_logprobs(z, tokens)[1],
+                  lambda z: policy.adjust_logits(z, history=tokens[:, None], repetition=1.5), torch.square):
+        leaf = randn(g, 5, k).to(DEV).requires_grad_()
+        z = leaf * 2
+        y = keeps(z)
+        with torch.no_grad():
+            assert policy.adjust_logits(z, mask=mask, out=z) is z
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        # through a view, and where out is not the logits
+        z = leaf * 2
+        y = keeps(z)
+        with torch.no_grad():
+            policy.adjust_logits(randn(g, 2, k).to(DEV), out=z[1:3])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        # what is read only stays usable
+        z = leaf * 2
+        y = keeps(z)
+        with torch.no_grad():
+            policy.adjust_logits(z, mask=mask)
+            policy.adjust_logits(z, mask=mask, out=torch.empty_like(z))
+        y.sum().backward()
+    plain = torch.zeros((5, k), device=DEV)
+    before = plain._version
+    policy.adjust_logits(plain, bias=torch.ones(k, device=DEV), out=plain)
+    assert plain._version == before + 1 and (plain == 1).all()
+    with torch.inference_mode():  # such tensors count no writes
+        kept = torch.zeros((5, k), device=DEV)
+        policy.adjust_logits(kept, bias=torch.ones(k, device=DEV), out=kept)
+    policy.adjust_logits(kept, bias=torch.ones(k, device=DEV), out=kept)
+    assert (kept == 2).all()
