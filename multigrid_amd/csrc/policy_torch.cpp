@@ -92,7 +92,15 @@ int whole(const char *name, at::ScalarType t) {
 
 bool wants_grad(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
-void no_gradient(const char *name, const Maybe &t, const char *instead) { TORCH_CHECK_VALUE(!t || !wants_grad(*t), name, " passes no gradient: ", instead); }
+// Forward-mode differentiation (which torch.no_grad() does not switch off): a tangent is refused, as its loss would read as a derivative of 0.
+bool has_tangent(const Tensor &t) { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined(); }
+void no_tangent(const char *name, const Tensor &t) { TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), name, " has a tangent: forward-mode derivatives are not supported"); }
+
+void no_gradient(const char *name, const Maybe &t, const char *instead) {
+    if (!t) return;
+    TORCH_CHECK_VALUE(!wants_grad(*t), name, " passes no gradient: ", instead);
+    no_tangent(name, *t);
+}
 void no_gradient(const char *name, const Number &v) {
     if (const Tensor *t = std::get_if<Tensor>(&v)) no_gradient(name, Maybe(*t), "detach it");
 }
@@ -119,7 +127,11 @@ void no_leaf_of_the_default_stream(const Tensor &t) {
     }
 }
 
-void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the operators of multigrid_amd.policy are differentiable once (create_graph is not supported)"); }
+// of a backward pass, with the gradients that come in
+void once(const variable_list &grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the operators of multigrid_amd.policy are differentiable once (create_graph is not supported)");
+    for (const Tensor &g : grads) TORCH_CHECK_NOT_IMPLEMENTED(!g.defined() || !has_tangent(g), "the operators of multigrid_amd.policy are differentiable once (the gradient has a tangent)");
+}
 
 // [..., k] as [n, k] with adjacent elements in a row; a view wherever there is one
 Tensor rows_of(const Tensor &t) {
@@ -229,7 +241,7 @@ struct Embed : torch::autograd::Function<Embed> {
         return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        once();
+        once(grads);
         const auto &f = ctx->saved_data["fields"];
         const Fields fields = f.isNone() ? Fields() : Fields(f.toIntVector());
         return {Tensor(), embed_grad(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(), fields, ctx->saved_data["scale"].toDouble()), Tensor(), Tensor()};
@@ -240,6 +252,7 @@ Tensor embed(const Tensor &ids, const Tensor &table, const Fields &fields, doubl
     on_gpu("table", table);
     beside("ids", ids, table);
     TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) && table.size(1), "table must be [rows, dim] and hold something, got ", table.sizes());
+    no_tangent("table", table);
     if (!wants_grad(table)) return embed_forward(ids, table, fields, scale);
     no_leaf_of_the_default_stream(table);
     return Embed::apply(ids, table, fields, scale);
@@ -378,7 +391,7 @@ struct Adjust : torch::autograd::Function<Adjust> {
         return adjust_forward(logits, Maybe(), history, lengths, repetition, presence, frequency, bias, mask);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        once();
+        once(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0];
         auto maybe = [](const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
@@ -399,6 +412,7 @@ struct Adjust : torch::autograd::Function<Adjust> {
 Tensor adjust_logits(const Tensor &logits, const Maybe &history, const Maybe &lengths, const Number &repetition, const Number &presence, const Number &frequency,
                      const Maybe &bias, const Maybe &mask, const Maybe &out) {
     on_gpu("logits", logits);
+    no_tangent("logits", logits);
     no_gradient("repetition", repetition);
     no_gradient("presence", presence);
     no_gradient("frequency", frequency);
@@ -406,6 +420,7 @@ Tensor adjust_logits(const Tensor &logits, const Maybe &history, const Maybe &le
     if (out) {
         TORCH_CHECK_VALUE(!wants_grad(logits) && !wants_grad(*out), "out is not differentiable: leave it out, or call under torch.no_grad()");
         beside("out", *out, logits);
+        no_tangent("out", *out);
         TORCH_CHECK_VALUE(out->sizes() == logits.sizes() && out->scalar_type() == logits.scalar_type() && out->is_contiguous(), "out must be contiguous, ", logits.scalar_type(),
                           " and of shape ", logits.sizes());
         TORCH_CHECK_VALUE(!overlap(*out, logits) || (out->data_ptr() == logits.data_ptr() && logits.is_contiguous()), "out may be the logits or lie beside them, not across them");
@@ -487,7 +502,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
         return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        once();
+        once(grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0];
         Rows r = rows(logits, saved[2].defined() ? Number(saved[2]) : Number(ctx->saved_data["temperature"].toDouble()), whole("tokens", saved[1].scalar_type()));
@@ -509,6 +524,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
 
 std::pair<Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &tokens, const Number &temperature) {
     on_gpu("logits", logits);
+    no_tangent("logits", logits);
     no_gradient("temperature", temperature);
     if (wants_grad(logits)) no_leaf_of_the_default_stream(logits);
     const auto out = wants_grad(logits) ? Logprobs::apply(logits, tokens, temperature) : logprobs_forward(logits, tokens, temperature, false);

@@ -8,7 +8,8 @@ answers with logits.  Here the one becomes the input of a dense layer and the ot
 * ``draw`` - an answer from logits and a uniform number of the caller's;
 * ``token_logprobs`` - log-probabilities and entropies of answers, what a policy gradient trains on.
 
-``embed``, ``adjust_logits`` and ``token_logprobs`` are differentiable, once.  Every call is enqueued on the current
+``embed``, ``adjust_logits`` and ``token_logprobs`` are differentiable, once and backwards: a tangent of forward-mode
+differentiation is refused (NotImplementedError).  Every call is enqueued on the current
 stream of its tensors' device, waits for nothing and may be captured into a HIP graph; tensors may have any strides, and a
 last dimension that is not adjacent in memory is copied.  What a backward pass reads again (``logits``, ``history``,
 ``lengths``, ``mask``, ``tokens``) must hold the same values until then; ``ids`` may change, a copy is kept (the

@@ -35,9 +35,14 @@ from typing import Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, envs, layouts, policy
 from .batched import BatchedMultiGrid
+
+
+def _primal(value):
+    return forward_ad.unpack_dual(value).primal if isinstance(value, torch.Tensor) else value
 
 
 class MultiGridVectorEnv:
@@ -167,9 +172,11 @@ class MultiGridVectorEnv:
         lead = (self.num_envs,) if self.single_agent else (self.num_envs, self.num_agents)
         if tuple(logits.shape) != lead + (self.num_actions,):
             raise ValueError(f"expected logits of shape {lead + (self.num_actions,)}, got {tuple(logits.shape)}")
+        # (actions have no derivative: neither a gradient nor a tangent is asked for)
+        logits, temperature = _primal(logits), _primal(temperature)
         with torch.no_grad():
             if adjust:
-                logits = policy.adjust_logits(logits, **adjust)
+                logits = policy.adjust_logits(logits, **{name: _primal(value) for name, value in adjust.items()})
             actions, logprobs = policy.draw(logits, uniforms, temperature=temperature, dtype=torch.uint8)
         obs, reward, terminated, truncated, infos = self.step(actions)
         infos["actions"] = actions.cpu().numpy() if self.numpy else actions

@@ -161,3 +161,62 @@ def test_out_counts_as_a_write(policy, k):
         policy.adjust_logits(kept, bias=torch.ones(k, device=DEV), out=kept)
     policy.adjust_logits(kept, bias=torch.ones(k, device=DEV), out=kept)
     assert (kept == 2).all()
+
+
+@pytest.mark.parametrize("k", [7, 40])
+def test_tangents_are_refused(policy, k):
+    """Forward-mode derivatives are not worked out: a tangent is refused, not lost (which would read as a derivative of 0)."""
+    import torch.autograd.forward_ad as forward
+    g = gen(k)
+    x, w, ones = randn(g, 4, k).to(DEV), randn(g, 24, 8).to(DEV), torch.ones(4, device=DEV)
+    ids, tokens, bias = torch.arange(4, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV), randn(g, k).to(DEV)
+    calls = [(lambda t: policy.embed(ids, t), w, "table"), (lambda t: policy.adjust_logits(t, presence=1.0), x, "logits"),
+             (lambda t: policy.adjust_logits(x, bias=t), bias, "bias"), (lambda t: policy.adjust_logits(x, repetition=t), ones, "repetition"),
+             (lambda t: policy.adjust_logits(x, presence=t), ones, "presence"), (lambda t: policy.adjust_logits(x, frequency=t), ones, "frequency"),
+             (lambda t: policy.adjust_logits(x, out=t), torch.empty_like(x), "out"), (lambda t: policy.token_logprobs(t, tokens), x, "logits"),
+             (lambda t: policy.token_logprobs(x, tokens, temperature=t), ones, "temperature"), (lambda t: policy.draw(x, temperature=t), ones, "temperature")]
+    for call, value, name in calls:
+        with forward.dual_level():
+            for watched in (value, value.clone().requires_grad_()) if name in ("table", "logits") else (value,):
+                dual = forward.make_dual(watched, torch.ones_like(value))
+                with pytest.raises(NotImplementedError, match=name):
+                    call(dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match=name):
+                    call(dual)
+                with pytest.raises(NotImplementedError, match=name):
+                    call(dual[:])  # a view of it
+            call(value)  # beside tangents, none of its own
+            call(forward.unpack_dual(dual).primal.detach())
+            tokens_of, _ = policy.draw(forward.make_dual(x, torch.ones_like(x)))  # whole numbers: nothing is lost
+            assert torch.equal(tokens_of, x.argmax(1))
+        call(value)
+    # a tangent that comes with the gradient
+    for call, value in ((lambda t: policy.embed(ids, t), w), (lambda t: policy.adjust_logits(t, presence=1.0), x), (lambda t: policy.token_logprobs(t, tokens)[0], x),
+                        (lambda t: policy.token_logprobs(t, tokens)[1], x)):
+        leaf = value.clone().requires_grad_()
+        y = call(leaf)
+        with forward.dual_level():
+            with pytest.raises(RuntimeError, match="once"):
+                torch.autograd.grad(y, leaf, forward.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
+        torch.autograd.grad(y, leaf, torch.ones_like(y))
+    for call, value in ((lambda t: policy.embed(ids, t), w), (lambda t: policy.token_logprobs(t, tokens)[0], x)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (value,), (torch.ones_like(value),))
+
+
+def test_step_logits_takes_logits_with_tangents(policy):
+    """Actions have no derivative: logits are taken with their tangents as they are taken while they require a gradient."""
+    import torch.autograd.forward_ad as forward
+    from multigrid_amd.vector import MultiGridVectorEnv
+    one, two = (MultiGridVectorEnv("MultiGrid-Empty-8x8-v0", 9, agents=2, num_layouts=8) for _ in range(2))
+    one.reset(seed=1), two.reset(seed=1)
+    g = gen(1)
+    logits, u, rep = randn(g, 9, 2, 7).to(DEV), torch.rand((9, 2), generator=g).to(DEV), 1 + torch.rand((9, 2), generator=g).to(DEV)
+    history = torch.randint(0, 7, (9, 2, 3), generator=g).to(DEV)
+    want = one.step_logits(logits, u, temperature=rep, repetition=rep, history=history)
+    with forward.dual_level():
+        dual = [forward.make_dual(t, torch.ones_like(t)) for t in (logits, rep)]
+        got = two.step_logits(dual[0], u, temperature=dual[1], repetition=dual[1], history=history)
+    assert torch.equal(got[4]["actions"], want[4]["actions"]) and torch.equal(got[4]["action_logprobs"], want[4]["action_logprobs"])
+    assert torch.equal(got[0]["image"], want[0]["image"])
+    one.close(), two.close()
