@@ -411,19 +411,25 @@ __global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedA
     }
     __syncthreads();
     for (int i = threadIdx.x; i < combined * vecs; i += COMBINED_THREADS) {
-        const int c = i / combined;
-        int rest = i - c * combined, base = a.rows;
-        const int at = rest;
-        float acc[V] = {};
-        for (int f = a.fields - 1; f >= 0; --f) {  // the last field varies first; the sum is over fields in any order
-            const int size = a.sizes[f], id = rest % (size + 1);
-            rest /= size + 1;
-            base -= size;
-            float x[V];
-            load<T, V>(table_s + (id < size ? base + id : a.rows) * pitch + c * V, x);
+        const int c = i / combined, at = i - c * combined;
+        int row[MG_MAX_FIELDS], rest = at, base = a.rows;
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[e] += x[e];
-        }
+        for (int f = MG_MAX_FIELDS - 1; f >= 0; --f)  // the last field varies first
+            if (f < a.fields) {
+                const int size = a.sizes[f], id = rest % (size + 1);
+                rest /= size + 1;
+                base -= size;
+                row[f] = id < size ? base + id : a.rows;
+            }
+        float acc[V] = {};
+#pragma unroll
+        for (int f = 0; f < MG_MAX_FIELDS; ++f)  // in the order of the other two kernels: a token's bits do not depend on how many there are
+            if (f < a.fields) {
+                float x[V];
+                load<T, V>(table_s + row[f] * pitch + c * V, x);
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] += x[e];
+            }
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] *= a.scale;
         store<T, V>(done_s + at * pitch + c * V, acc);

@@ -220,3 +220,19 @@ def test_step_logits_takes_logits_with_tangents(policy):
     assert torch.equal(got[4]["actions"], want[4]["actions"]) and torch.equal(got[4]["action_logprobs"], want[4]["action_logprobs"])
     assert torch.equal(got[0]["image"], want[0]["image"])
     one.close(), two.close()
+
+
+# ---- the same cell in another batch ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("sizes,dim,dtype", [((11, 6, 7), 16, torch.float32), ((11, 6, 7), 15, torch.float32), ((11, 6, 7), 32, torch.bfloat16), ((3, 2, 5, 2), 16, torch.float16)])
+def test_a_cell_has_the_same_bits_in_every_batch(policy, sizes, dim, dtype):
+    """Which kernel embeds a batch goes by its size; the order of a token's sum does not."""
+    combinations = math.prod(s + 1 for s in sizes)
+    n = 16 * 256 * combinations + 77
+    g = gen(dim)
+    ids = torch.stack([torch.randint(0, s + 1, (n,), generator=g, dtype=torch.uint8) for s in sizes], -1).to(DEV)
+    table = randn(g, sum(sizes), dim).to(dtype).to(DEV)
+    whole = policy.embed(ids, table, fields=sizes, scale=1.7)
+    for first, many in ((0, 1), (5, 98), (n - 4097, 4097), (1000, 131072 + 5), (0, n - 99)):
+        assert torch.equal(policy.embed(ids[first:first + many], table, fields=sizes, scale=1.7), whole[first:first + many]), many
