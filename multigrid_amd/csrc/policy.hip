@@ -1281,6 +1281,12 @@ constexpr float DEEP = -200.f;  // exp_twice of it is 0
 
 // ---- adjustment of logits ------------------------------------------------------------------------------------------
 
+// A repeated token's positive logit, or its gradient, is multiplied by 1 / repetition, rounded once for a row, instead of a division for
+// a token.  No float holds the reciprocal of a repetition below 2^-126 with all its bits, or at all (and infinity times a gradient of 0
+// would be NaN): they are multiplied by 2^24 first, and then by the reciprocal of 2^24 repetitions.
+__device__ __forceinline__ float before_reciprocal(float repetition) { return repetition < 0x1p-126f ? 0x1p24f : 1.f; }
+__device__ __forceinline__ float reciprocal(float repetition) { return 1.f / (repetition * before_reciprocal(repetition)); }
+
 // A block counts a stretch of tokens' occurrences in their rows' histories in LDS, then the stretch streams through once: of
 // `lanes` threads to a row (a power of two) each takes up to STRETCH 16-byte vectors, whose loads are under way while the
 // history is counted.  Short rows share a block, a row longer than a block's stretch is cut, and each piece looks through the
@@ -1310,7 +1316,7 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
         }
         float rep = 1.f, presence = 0.f, frequency = 0.f;
         if (live) {
-            rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;  // (its reciprocal below: a division for a row, not for a token)
+            rep = a.repetition_dev ? a.repetition_dev[row] : a.repetition;
             presence = a.presence_dev ? a.presence_dev[row] : a.presence;
             frequency = a.frequency_dev ? a.frequency_dev[row] : a.frequency;
         }
@@ -1347,7 +1353,8 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
             __syncthreads();
         }
         if (live) {
-            const float inverse = 1.f / rep;
+            const float inverse = reciprocal(rep);
+            const bool some_small = __any(before_reciprocal(rep) != 1.f);  // (asked once a wave: with a factor for every token one row of 32000 takes 6.2 us, not 5.9)
 #pragma unroll
             for (int j = 0; j < STRETCH; ++j) {
                 const int at = first + (j * lanes + lane) * V;
@@ -1378,12 +1385,17 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                     }
                 float y[V];
 #pragma unroll
+                for (int i = 0; i < V; ++i) y[i] = element<T>(GRAD ? g[j] : x[j], i);
+                if (some_small) {
+                    const float first = before_reciprocal(rep);
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (c[i] > 0 && element<T>(x[j], i) > 0.f) y[i] *= first;
+                }
+#pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    y[i] = element<T>(x[j], i);
                     if (GRAD) {
-                        const bool up = y[i] > 0.f;
-                        y[i] = element<T>(g[j], i);
-                        if (c[i] > 0) y[i] = y[i] * (up ? inverse : rep);
+                        if (c[i] > 0) y[i] = y[i] * (element<T>(x[j], i) > 0.f ? inverse : rep);
                     } else {
                         if (c[i] > 0) y[i] = y[i] * (y[i] > 0.f ? inverse : rep) - presence;
                         y[i] = y[i] - frequency * static_cast<float>(c[i]);
@@ -1489,7 +1501,7 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
         for (; i < len; ++i)
             if (h[i] >= 0 && h[i] < static_cast<H>(a.k)) atomicAdd(&counts[h[i]], 1u);
     }
-    const float inverse = 1.f / rep;
+    const float first = before_reciprocal(rep), inverse = reciprocal(rep);
 #pragma unroll
     for (int j = 0; j < K; ++j) {
         if (j >= a.k) continue;
@@ -1497,11 +1509,11 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
         const bool ok = (allow >> j) & 1;
         if (GRAD) {
             float v = g[j];
-            if (c > 0) v = v * (x[j] > 0.f ? inverse : rep);
+            if (c > 0) v = x[j] > 0.f ? v * first * inverse : v * rep;
             x[j] = ok ? v : 0.f;
         } else {
             float v = x[j];
-            if (c > 0) v = v * (v > 0.f ? inverse : rep) - presence;
+            if (c > 0) v = (v > 0.f ? v * first * inverse : v * rep) - presence;
             v = v - frequency * static_cast<float>(c);
             if (a.bias_dev) v = v + bias[j];
             x[j] = ok ? v : NEG_INF;

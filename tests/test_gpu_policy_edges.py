@@ -236,3 +236,32 @@ def test_a_cell_has_the_same_bits_in_every_batch(policy, sizes, dim, dtype):
     whole = policy.embed(ids, table, fields=sizes, scale=1.7)
     for first, many in ((0, 1), (5, 98), (n - 4097, 4097), (1000, 131072 + 5), (0, n - 99)):
         assert torch.equal(policy.embed(ids[first:first + many], table, fields=sizes, scale=1.7), whole[first:first + many]), many
+
+
+# ---- penalties at the ends of their ranges -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("k", [7, 32, 40, 9001])
+def test_repetitions_whose_reciprocal_no_float_holds(policy, k, dtype):
+    """A positive logit is divided by the repetition, however small that is, and a gradient of 0 stays 0."""
+    g = gen(k)
+    values = [2.0 ** -149, 2.0 ** -130, 1e-40, 2.0 ** -128, 2.0 ** -126, 1e-30, 1.0, 2.0 ** 127]
+    n = len(values)
+    rep = torch.tensor(values, dtype=torch.float64).float()
+    x = (randn(g, n, k) * 1e-8).to(dtype)
+    x[0] *= 0.5 ** 30  # (whose quotient by 2^-149 is finite)
+    history = torch.randint(0, k, (n, 5), generator=g)
+    history[:, 0] = x.float().argmax(1)
+    up = randn(g, n, k).to(dtype)
+    up[:, ::2] = 0.0
+    for repetition in (rep, *values[1:5]):
+        want, err, factor = ref.adjust(x, history, repetition=repetition)
+        leaf = x.to(DEV).requires_grad_()
+        y = policy.adjust_logits(leaf, history=history.to(DEV), repetition=to_gpu(repetition))
+        # (a product below 2^-126 is held in steps of 2^-149 before it is rounded to its type)
+        close_held(y, want, err + 2.0 ** -150, dtype)
+        dx, = torch.autograd.grad(y, leaf, up.to(DEV))
+        d = ref.np64(up) * factor
+        assert bool((dx[:, ::2] == 0).all())
+        close_held(dx, d, np.abs(d) * 2 * ref.U32 + 2.0 ** -150, dtype)
