@@ -353,8 +353,8 @@ int mg_embed_grad(const MgEmbed *e, const void *ids_dev, const void *grad_dev, v
 
 /* Adjustment of logits [n][k] before an answer is drawn.  With c = how often token j stands among the first
  * lengths[i] entries of history[i] (entries outside 0 .. k - 1 count for nothing):
- *     x = logit;  c > 0: x = x * (x > 0 ? 1 / repetition : repetition) - presence;
- *     x = x - frequency * c + bias[j];  x = -inf where the mask bars j.
+ *     x = logit;  c > 0: x = x * (x > 0 ? 1 / repetition : repetition) - presence - frequency * c;
+ *     x = x + bias[j];  x = -inf where the mask bars j.
  * Worked out in 32 bits, each operation rounded, and rounded to `dtype` once.  A row whose mask bars everything becomes
  * -inf throughout.  What a barred place held (NaN, infinities) does not matter. */
 #define MG_MASK_NONE 0

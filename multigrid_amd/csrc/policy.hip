@@ -1287,6 +1287,14 @@ constexpr float DEEP = -200.f;  // exp_twice of it is 0
 __device__ __forceinline__ float before_reciprocal(float repetition) { return repetition < 0x1p-126f ? 0x1p24f : 1.f; }
 __device__ __forceinline__ float reciprocal(float repetition) { return 1.f / (repetition * before_reciprocal(repetition)); }
 
+// frequency * c, and 0 for a token that is not there also if the frequency is infinite: this product is 0 where a factor is.  (With a test
+// instead, at a token or once a wave, 256 rows x 128000 take 36.6 us, not 36.0.)
+__device__ __forceinline__ float frequency_of(uint32_t c, float frequency) {
+    float product;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(product) : "v"(frequency), "v"(static_cast<float>(c)));
+    return product;
+}
+
 // A block counts a stretch of tokens' occurrences in their rows' histories in LDS, then the stretch streams through once: of
 // `lanes` threads to a row (a power of two) each takes up to STRETCH 16-byte vectors, whose loads are under way while the
 // history is counted.  Short rows share a block, a row longer than a block's stretch is cut, and each piece looks through the
@@ -1398,7 +1406,7 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(MgAdjust a, int lanes, 
                         if (c[i] > 0) y[i] = y[i] * (element<T>(x[j], i) > 0.f ? inverse : rep);
                     } else {
                         if (c[i] > 0) y[i] = y[i] * (y[i] > 0.f ? inverse : rep) - presence;
-                        y[i] = y[i] - frequency * static_cast<float>(c[i]);
+                        y[i] = y[i] - frequency_of(c[i], frequency);
                     }
                 }
                 if (!GRAD && a.bias_dev) {
@@ -1514,7 +1522,7 @@ __global__ __launch_bounds__(K <= 16 ? THREADS : 64) void adjust_short_kernel(Mg
         } else {
             float v = x[j];
             if (c > 0) v = (v > 0.f ? v * first * inverse : v * rep) - presence;
-            v = v - frequency * static_cast<float>(c);
+            v = v - frequency_of(c, frequency);
             if (a.bias_dev) v = v + bias[j];
             x[j] = ok ? v : NEG_INF;
         }

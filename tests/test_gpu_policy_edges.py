@@ -265,3 +265,27 @@ def test_repetitions_whose_reciprocal_no_float_holds(policy, k, dtype):
         d = ref.np64(up) * factor
         assert bool((dx[:, ::2] == 0).all())
         close_held(dx, d, np.abs(d) * 2 * ref.U32 + 2.0 ** -150, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [7, 32, 40, 9001])
+def test_infinite_penalties_reach_repeated_tokens_only(policy, k, dtype):
+    """A frequency or presence penalty of infinity bars what was answered before and leaves everything else as it was."""
+    g = gen(k)
+    x, history = randn(g, 6, k).to(dtype), torch.randint(0, k, (6, 4), generator=g)
+    seen = torch.from_numpy(ref.history_counts(history, None, 6, k) > 0)
+    bias = randn(g, k)
+    for much in (math.inf, torch.full((6,), math.inf)):
+        for name in ("frequency", "presence"):
+            y = policy.adjust_logits(x.to(DEV), history=history.to(DEV), bias=bias.to(DEV), **{name: to_gpu(much)})
+            plain = policy.adjust_logits(x.to(DEV), bias=bias.to(DEV))
+            assert torch.equal(y.cpu(), torch.where(seen, torch.tensor(-math.inf, dtype=dtype), plain.cpu()))
+        y = policy.adjust_logits(x.to(DEV), bias=bias.to(DEV), frequency=to_gpu(much))  # no history at all
+        assert torch.equal(y, plain)
+    y = policy.adjust_logits(x.to(DEV), history=history.to(DEV), frequency=math.nan)
+    assert torch.equal(torch.isnan(y).cpu(), seen)
+    # the smallest penalties are not lost
+    if dtype != torch.float16:
+        tiny = 2.0 ** -133
+        y = policy.adjust_logits(torch.zeros_like(x).to(DEV), history=history.to(DEV), frequency=tiny)
+        assert torch.equal(y.cpu().double(), torch.from_numpy(-tiny * ref.history_counts(history, None, 6, k)) + 0.0)
