@@ -410,9 +410,10 @@ int64_t mg_draw_workspace(const MgLogits *l);
 int mg_draw(const MgLogits *l, const void *logits_dev, const void *uniforms_dev, int32_t uniforms_type, void *tokens_dev,
             float *logprob_dev, void *workspace_dev, int64_t workspace_bytes, void *stream);
 
+#define MG_LOGPROB_NO_STATS 32
 /* Log-probability of a given token of every row and the row's entropy (either output may be NULL), and what the
- * gradient needs of the row: stats [n][4] floats, 16-byte aligned (may be NULL; up to 32 tokens a row the gradient works
- * them out again and needs none).  A token outside 0 .. k - 1 is ignored:
+ * gradient needs of the row: stats [n][4] floats, 16-byte aligned (may be NULL; up to MG_LOGPROB_NO_STATS tokens a row
+ * the gradient works them out again and needs none).  A token outside 0 .. k - 1 is ignored:
  * log-probability 0, and none of its gradient.  Rows that are all -inf: log-probability -inf, entropy 0, no gradient. */
 int64_t mg_token_logprobs_workspace(const MgLogits *l);
 int mg_token_logprobs(const MgLogits *l, const void *logits_dev, const void *tokens_dev, float *logprob_dev,

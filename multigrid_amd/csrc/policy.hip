@@ -1151,6 +1151,7 @@ __global__ __launch_bounds__(THREADS) void embed_span_kernel(EmbedArgs a, Sorted
 // gradient 22, adjustment with a history of 16 entries and a mask 26 (40 to 60 MB each); with eight threads to a row, as for
 // longer ones, draw 100, log-probabilities 48, adjustment 101, and of 32 tokens still 90 against 55, 47 against 42, 99 against 87.
 constexpr int SHORT = 32;
+static_assert(SHORT == MG_LOGPROB_NO_STATS, "the gradient of a short row reads no statistics");
 
 template <class T, int K>
 __device__ __forceinline__ void load_row(const T *p, int k, float (&x)[K], uint32_t fill) {

@@ -475,15 +475,13 @@ std::pair<Tensor, Tensor> draw(const Tensor &logits, const Maybe &uniforms, cons
     return {tokens, logprobs};
 }
 
-constexpr int64_t NO_STATS = 32;  // tokens of a row up to which the gradient needs nothing of the forward pass
-
 std::vector<Tensor> logprobs_forward(const Tensor &logits, const Tensor &given, const Number &temperature, bool stats) {
     Rows r = rows(logits, temperature, whole("tokens", beside("tokens", given, logits).scalar_type()));
     const auto lead = lead_of(logits);
     TORCH_CHECK_VALUE(given.sizes() == lead, "tokens must be of shape ", lead, ", got ", given.sizes());
     const Tensor tokens = given.contiguous();
     const auto floats = logits.options().dtype(at::kFloat);
-    const Tensor logprobs = at::empty(lead, floats), entropies = at::empty(lead, floats), kept = stats && r.l.k > NO_STATS ? at::empty({r.l.n, 4}, floats) : Tensor();
+    const Tensor logprobs = at::empty(lead, floats), entropies = at::empty(lead, floats), kept = stats && r.l.k > MG_LOGPROB_NO_STATS ? at::empty({r.l.n, 4}, floats) : Tensor();
     On on(logits);
     const Tensor ws = workspace(entry.logprobs_workspace(&r.l), logits);
     check(entry.logprobs(&r.l, address(r.x), address(tokens), static_cast<float *>(address(logprobs)), static_cast<float *>(address(entropies)),
