@@ -824,6 +824,9 @@ __device__ __forceinline__ void places(uint32_t *count, const uint32_t (&digit)[
     for (int j = 0; j < N; ++j) {
         at[j] = __builtin_amdgcn_mbcnt_hi(high[j], __builtin_amdgcn_mbcnt_lo(low[j], 0));
         before[j] = 0;
+        // An earlier digit's count comes first, also if it is another lane's: one wave's accesses to LDS are done in the order of its
+        // instructions, which the fence makes the compiler keep (it emits nothing).
+        if (j > 0) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (live[j] && at[j] == 0) before[j] = atomicAdd(&count[digit[j]], static_cast<uint32_t>(__popc(low[j]) + __popc(high[j])));
     }
 #pragma unroll
