@@ -392,8 +392,9 @@ __device__ __forceinline__ void copy_ids(const EmbedArgs &a, const I *ids, I *to
 }
 
 // The same where LDS holds the finished output of every combination of a token's ids, none included (cells: 12 x 7 x 8): worked
-// out once a block, then each 16 bytes of output are one read of LDS and one store.  6422528 cells x 32 bfloat16: 84 us (430 MB, 5.1
-// TB/s), 110 by embed_table_kernel, 185 by embed_kernel.
+// out once a block, then each 16 bytes of output are one read of LDS and one store.  For rows of whole vectors (`dim` a multiple of V):
+// storing other rows' ends element by element was slower than embed_table_kernel (4500000 cells x 31 bfloat16 174 us against 112).
+// 6422528 cells x 32 bfloat16: 90 us (430 MB, 4.8 TB/s), 109 by embed_table_kernel, 185 by embed_kernel; x 16 float32 92, 93 and 151.
 constexpr int COMBINED_BYTES = 53248, COMBINED_THREADS = 512, COMBINED_BLOCKS = 768;  // three blocks to a compute unit
 static_assert(FAR == COMBINED_THREADS, "a token's ids to each thread");
 
@@ -401,13 +402,13 @@ template <class T, class I>
 __global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedArgs a, int combined, const I *ids, const T *table, T *out, I *ids_copy) {
     constexpr int V = WIDE<T>, TOGETHER = 4;
     extern __shared__ __align__(16) char lds[];
-    const int vecs = (a.dim + V - 1) / V, pitch = vecs * V;
+    const int vecs = a.dim / V, pitch = a.dim;
     T *done_s = reinterpret_cast<T *>(lds), *table_s = done_s + combined * pitch;  // [combined][pitch], [rows + 1][pitch]
     if (ids_copy) copy_ids(a, ids, ids_copy);  // (a stream of its own, before the others: 4 us; a launch of its own 10, beside each token's output 17)
     uint16_t *which_s = reinterpret_cast<uint16_t *>(table_s + (a.rows + 1) * pitch);
     for (int i = threadIdx.x; i < (a.rows + 1) * pitch; i += COMBINED_THREADS) {
         const int r = i / pitch, d = i - r * pitch;
-        table_s[i] = r < a.rows && d < a.dim ? table[r * a.row_stride + d] : static_cast<T>(0.f);
+        table_s[i] = r < a.rows ? table[r * a.row_stride + d] : static_cast<T>(0.f);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < combined * vecs; i += COMBINED_THREADS) {
@@ -471,18 +472,10 @@ __global__ __launch_bounds__(COMBINED_THREADS) void embed_combined_kernel(EmbedA
                     for (int u = 0; u < TOGETHER; ++u) {
                         const int t = t0 + u * per_block;
                         if (t >= tokens) break;
-                        T *to = out + (n0 + t) * a.dim + c * V;
-                        if (c * V + V <= a.dim) {
-                            struct __attribute__((packed, aligned(sizeof(T)))) Words {
-                                uint32_t w[4];
-                            };
-                            *reinterpret_cast<Words *>(to) = Words{{q[u].x, q[u].y, q[u].z, q[u].w}};
-                        } else {
-                            const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-                            for (int e = 0; e < V; ++e)
-                                if (c * V + e < a.dim) to[e] = static_cast<T>(element<T>(w, e));
-                        }
+                        struct __attribute__((packed, aligned(sizeof(T)))) Words {
+                            uint32_t w[4];
+                        };
+                        *reinterpret_cast<Words *>(out + (n0 + t) * a.dim + c * V) = Words{{q[u].x, q[u].y, q[u].z, q[u].w}};
                     }
                 }
     }
@@ -2548,13 +2541,15 @@ int mg_embed(const MgEmbed *e, const void *ids_dev, const void *table_dev, void 
         const int vecs = (a.dim + WIDE<T> - 1) / WIDE<T>, per_block = THREADS / (vecs < THREADS ? vecs : THREADS);
         const int64_t held = static_cast<int64_t>(a.rows + 1) * vecs * 16;
         // What a block prepares has to be little beside the tokens that it then writes.  Combinations: sixteen tokens for each, at a
-        // block to a compute unit (401408 cells x 32, a tenth of that: 17.5 us by embed_combined_kernel, 11.1 by
-        // embed_table_kernel).  A table: a full share of tokens for every compute unit (100352 cells x 32: 6.3 us with it, 5.9 by
-        // embed_kernel; 401408: 11.1 and 12.6).
+        // block to a compute unit.  Microseconds by embed_combined_kernel and by embed_table_kernel where cells reach that, 2760000 of
+        // them, without the ids' copy and with it: x 32 bfloat16 44.6 and 48.3, 40.7 and 50.1, x 16 26.6 and 28.4, 23.6 and 32.6, x 16
+        // float32 46.8 and 41.2, 44.2 and 43.4, x 8 26.9 and 25.4, 23.2 and 29.5; half as many x 16 float32 27.9 and 21.2, 27.2 and 22.8.
+        // A table: a full share of tokens for every compute unit (131072 cells x 32 bfloat16, where they begin: 6.6 us with it, 5.9 by
+        // embed_kernel, x 64 float32 13.2 and 12.4; twice as many 8.7 and 9.5, 16.1 and 22.1).
         int64_t combined = 1;
         for (int f = 0; f < a.fields; ++f) combined = combined * (a.sizes[f] + 1) <= (1 << 15) ? combined * (a.sizes[f] + 1) : 1 << 15;
         const int64_t combined_bytes = (combined + a.rows + 1) * vecs * 16 + FAR * 2;
-        if (combined_bytes <= COMBINED_BYTES && a.n >= 16 * combined * UNITS) {
+        if (a.dim % WIDE<T> == 0 && combined_bytes <= COMBINED_BYTES && a.n >= 16 * combined * UNITS) {
             hipLaunchKernelGGL((embed_combined_kernel<T, I>), dim3(blocks_for((a.n + FAR - 1) / FAR, COMBINED_BLOCKS)), dim3(COMBINED_THREADS),
                                combined_bytes, static_cast<hipStream_t>(stream), a, static_cast<int>(combined),
                                static_cast<const I *>(ids_dev), static_cast<const T *>(table_dev), static_cast<T *>(out_dev), ids_copy);
