@@ -8,8 +8,9 @@
 // Sums, maxima and probabilities are held in 32 bits (64 in the draw, where a token's borders decide); a value is
 // rounded to its type once, when it is stored.
 //
-// All of it is bound by memory or by launches.  On this card a copy of 1 GiB moves 5.1 TB/s (read and written together), a fill
-// 6.9, a sum reads 3.7 to 4.0; the smallest launch takes 3.5 us.  The times beside the kernels are theirs alone, without the host.
+// On this card a copy of 1 GiB moves 5.1 TB/s (read and written together), a fill 6.9, torch's float32 sum reads 4.0; the smallest
+// launch takes 3.6 us.  The times beside the kernels are theirs, without the host.  A pass that reads much takes longer behind one that
+// has written much, while the caches still write that back: where two times are given, the first is of the pass by itself.
 
 #include <hip/hip_runtime.h>
 
@@ -514,14 +515,16 @@ __device__ __forceinline__ uint32_t row_of(Id id, uint32_t base, uint32_t size, 
 // permutation each.  The order of the tokens within 32 is free: a load takes four adjacent tokens, whole lines of memory.
 // Waves and blocks stride over the tokens, a block adds its four waves, embed_join_kernel the blocks, all in a fixed order.
 //
-// Bound by the reads: 6422528 cells x 32 bfloat16 122 us (430 MB with the ids, 3.5 TB/s), 401408 x 64 float32 36 us (104 MB, 2.9
-// TB/s: four or five turns of a wave, and their beginning and end).  By sorting the tokens these take 3250 and 172 us; with 64
+// Bound by the reads: with the join, 6422528 cells x 32 bfloat16 81 us (430 MB with the ids, 5.3 TB/s), 128 behind the lookup that
+// has written as much; 401408 x 64 float32 27 us (104 MB, 3.9 TB/s: four or five turns of a wave, and their beginning and end), 40
+// behind the lookup.  By sorting the tokens these take 3250 and 172 us; with 64
 // rows and 8190 tokens x 1024 the two are equal (28 and 26 us), with 2000 tokens x 64 it is 10 against 20.
 //
 // 0 times infinity or NaN is NaN: such a number would spoil a whole column.  A block whose sums are not all finite does its tokens
 // again, one after the other, each added to its own rows only.
-// Three blocks to a compute unit, two where a lane takes four columns and the registers allow no more (6422528 cells x 32 bfloat16:
-// 133 us with 640 of them, 122 with 768, 125 with 1024).
+// Three blocks to a compute unit, two where a lane takes four columns and the registers allow no more.  Against 512, 1024 and 1536 in
+// place of 768, over nine cases from 65536 x 64 float32 to 6422528 x 32 bfloat16: within 3 % for most; 512 gains 12 % with 401408 x 32
+// bfloat16 and loses 12 % with 1500000 x 100 float16, 1024 and more lose up to 8 and 24 %.
 constexpr int FEW = 64, FEW_BLOCKS = 768;
 constexpr int64_t FAR_ROWS = 1 << 24;  // a stride up to which 64 tokens lie within 32-bit offsets
 
@@ -961,6 +964,7 @@ __global__ __launch_bounds__(THREADS) void embed_count_kernel(EmbedArgs a, const
     for (int i = threadIdx.x; i < bins; i += THREADS) counts[static_cast<int64_t>(i) * blocks + blockIdx.x] = count_s[i];
 }
 
+// One workgroup: 3.4 us for the counts of 32768 entries, 60 for those of 1000000 (62720), three quarters of their sort.
 __global__ __launch_bounds__(SORT_THREADS) void embed_scan_kernel(uint32_t *counts, int n) {
     __shared__ uint32_t wave_sums[SORT_THREADS / 64];
     uint32_t done = 0;
@@ -1268,7 +1272,8 @@ template <class X>
 __device__ __forceinline__ X sum_of(X a, X b) { return a + b; }
 
 // exp(2 ln 2 * z) for z <= 0, NaN for NaN: the exponential instruction gives nothing below 2^-126, the square of half as much
-// goes down to the smallest float.
+// goes down to the smallest float.  For an exponent x it is off by up to 5 |x| + 5 half steps of float32, about twice as much as expf,
+// which rows of up to SHORT tokens take.
 __device__ __forceinline__ float exp_twice(float z) {
     const float h = __builtin_amdgcn_exp2f(z);
     return h * h;
@@ -1593,7 +1598,7 @@ __device__ __forceinline__ double uniform_at(const void *uniforms, int type, int
     return fmin(fmax(u, 0.0), 1.0);
 }
 
-// log p of a token from its logit; total - 1 is exact where little stands beside the maximum
+// log p of a token from its logit; total - 1 is exact where little stands beside the maximum.  The logarithm has 32 bits, as the result.
 __device__ __forceinline__ float drawn_logprob(float x, const Spread &s, double total) {
     return static_cast<float>((static_cast<double>(x) - s.m) * s.c * 0.6931471805599453 - log1pf(static_cast<float>(total - 1.0)));
 }
@@ -1604,8 +1609,9 @@ struct DrawShared {
     int token;
 };
 
-// Bound by the exponentials in 64 bits where there are many long rows (4095 x 30011 bfloat16: 136 us; reading them 60), by
-// latency where there are few: 64 rows x 128003 float16 in pieces 11 us and their join 7.5.
+// Many long rows: 4095 x 30011 bfloat16 141 us, the likeliest 130, where reading them takes 63 (log-probabilities); 53 are the issue of
+// the exponentials in 64 bits, and in a block loads, maximum, exponentials and sums stand one behind the other.  Few are bound by
+// latency: 64 rows x 128003 float16 in pieces 9.7 us and their join, which takes a piece's exponentials again, 7.1.
 //
 // The token of a row (or of a piece of one) at whose sum of probabilities the border lies, known to all of its threads, and
 // the total.  `share`: the border is that share of the total; otherwise `border` is it, `before` what stands before the row.
@@ -2069,7 +2075,7 @@ __global__ __launch_bounds__(BLOCK<LANES>) void logprob_kernel(MgLogits l, const
     }
 }
 
-// 4095 x 30011 bfloat16: 82 us (246 MB from memory, 3.0 TB/s; 55 us where the cache holds half of it).
+// 4095 x 30011 bfloat16: 63 us (246 MB, 3.9 TB/s; a float32 sum over them 69), 82 behind the gradient of another batch.
 //
 // A long row's pieces, and their join by one wave.
 template <class T>
@@ -2124,7 +2130,7 @@ __device__ __forceinline__ float logprob_slope(float x, bool is_token, float4 st
 }
 
 // One pass over the logits, `lanes` threads (a power of two) to a row or to a piece of one.  Bound by memory: 4095 x 30011 bfloat16
-// 87 us (492 MB, 5.6 TB/s: part of the logits is still in the cache).
+// 104 us (492 MB, 4.7 TB/s), 87 behind the forward pass (part of the logits is still in the cache).
 template <class T>
 __global__ __launch_bounds__(THREADS) void logprob_grad_kernel(MgLogits l, int lanes, const T *logits, const void *tokens, const float *stats,
                                                                const float *grad_lp, int64_t lp_stride, const float *grad_h, int64_t h_stride, T *out) {

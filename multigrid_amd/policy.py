@@ -9,12 +9,14 @@ answers with logits.  Here the one becomes the input of a dense layer and the ot
 * ``token_logprobs`` - log-probabilities and entropies of answers, what a policy gradient trains on.
 
 ``embed``, ``adjust_logits`` and ``token_logprobs`` are differentiable, once and backwards: a tangent of forward-mode
-differentiation is refused (NotImplementedError).  Every call is enqueued on the current
-stream of its tensors' device, waits for nothing and may be captured into a HIP graph; tensors may have any strides, and a
-last dimension that is not adjacent in memory is copied.  What a backward pass reads again (``logits``, ``history``,
-``lengths``, ``mask``, ``tokens``) must hold the same values until then; ``ids`` may change, a copy is kept (the
-simulator writes its images in place).  float32, bfloat16 and float16; sums are held in 32 bits or more and rounded
-once.
+differentiation is refused (NotImplementedError).  Every call is enqueued on the current stream of its tensors' device,
+waits for nothing and may be captured into a HIP graph; tensors may have any strides, and a last dimension that is not
+adjacent in memory is copied.  What a backward pass reads again (``logits``, ``history``, ``lengths``, ``mask``, ``tokens``)
+must hold the same values until then; ``ids`` may change, a copy is kept (the simulator writes its images in place).
+float32, bfloat16 and float16; sums are held in 32 bits or more and rounded once.
+
+Arguments that do not fit raise ValueError, what the library itself refuses ``_lib.MgError`` (a RuntimeError; out of a backward
+pass it comes as a plain RuntimeError with the same text).
 
 A backward pass that is captured must not meet a leaf that an eager graph of the default stream still holds: the leaf's
 gradient would be accumulated on that stream, which ends the process.  A differentiable call under capture looks for such
@@ -64,7 +66,7 @@ def embed(ids: torch.Tensor, table: torch.Tensor, *, fields: Optional[Sequence[i
 def embed_grad(grad: torch.Tensor, ids: torch.Tensor, rows: int, *, fields: Optional[Sequence[int]] = None,
                scale: float = 1.0) -> torch.Tensor:
     """The gradient ``[rows, dim]`` of ``embed``'s table for the gradient ``grad`` ``[..., dim]`` of its output, summed by
-    token in an order that depends on the shapes and ids alone, in ``grad``'s type."""
+    token in an order that depends on the shapes and ids alone, in ``grad``'s type.  Not differentiable."""
     return (_bound or _native()).embed_grad(grad, ids, rows, fields, scale)
 
 
@@ -76,7 +78,7 @@ def adjust_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = Non
     ``history`` ``[..., t]`` (or ``[t]`` for all rows): what was answered before, whole numbers; of row i the first
     ``lengths[i]`` count (all without ``lengths``), entries outside 0 .. k - 1 do not.  A token that stands there c > 0 times
     has its logit x made ``x * (1 / repetition)`` where positive and ``x * repetition`` elsewhere, less ``presence``, less
-    ``frequency * c``; each of the three is a number or a tensor of one per row.  ``bias`` ``[k]`` or ``[..., k]`` is added.
+    ``frequency * c``; each of the three is a number or a tensor of one per row, ``repetition`` positive.  ``bias`` ``[k]`` or ``[..., k]`` is added.
     ``mask`` says what may be answered - ``bool`` / ``uint8`` ``[k]`` or ``[..., k]``, or one bit per token in ``int32``
     ``[ceil(k / 32)]`` or ``[..., ceil(k / 32)]``, lowest bit first; everything else becomes -inf, also all of a row.
 
@@ -99,9 +101,10 @@ def draw(logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None, *, tempe
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature=1.0):
-    """Log-probability of ``tokens`` ``[...]`` (whole numbers) under ``logits`` ``[..., k]``, and the entropy of every row:
-    two float32 tensors ``[...]``, both differentiable with respect to the logits.  A token outside 0 .. k - 1 is ignored: its
-    log-probability is 0 and passes no gradient.  -inf logits (what ``adjust_logits`` bars) have probability 0 and
+    """Log-probability of ``tokens`` ``[...]`` (int64, int32, or uint8 for up to 255 tokens) under ``logits`` ``[..., k]``, and
+    the entropy of every row: two float32 tensors ``[...]``, both differentiable with respect to the logits.  A token outside
+    0 .. k - 1 is ignored: its log-probability is 0 and passes no gradient.  -inf logits (what ``adjust_logits`` bars) have probability 0 and
     gradient 0; a row of nothing else has log-probability -inf, entropy 0 and no gradient.  ``temperature`` is a number
-    or a tensor of one per row; it passes no gradient."""
+    or a tensor of one per row (a row whose number is no temperature - below 2^-126, infinite or NaN - gives NaN); it passes
+    no gradient."""
     return (_bound or _native()).token_logprobs(logits, tokens, temperature)
