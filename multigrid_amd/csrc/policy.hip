@@ -506,7 +506,8 @@ __device__ __forceinline__ uint32_t row_of(Id id, uint32_t base, uint32_t size, 
 
 // Few rows (up to FEW): the gradient is the product of the rows' indicator [rows][n] (1 where token n reads the row) and the
 // incoming gradient [n][dim], which is what matrix instructions are for: 1 is exact in every type, so every product is, and
-// the sums are held in float32.  16-bit gradients go in as they are, float32 ones as three bfloat16 parts of eight bits each.
+// the sums are held in float32.  16-bit gradients go in as they are, float32 ones as three bfloat16 parts of eight bits each (of 2^16
+// times the number: bfloat16 ends at 2^-133, float32 at 2^-149).
 //
 // A wave takes 64 tokens at a time: lane n puts its token's rows into LDS, then two 16 x 16 x 32 products per 16 rows and 16
 // columns.  The indicator's fragment (row l % 16, tokens 8 (l / 16) ...) is made from eight row numbers by three packed 16-bit
@@ -557,6 +558,9 @@ union Fragment {
 template <class T, int W, int TILES, int FIELDS>
 __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 || FIELDS > 3 ? 2 : 3) void embed_grad_few_kernel(EmbedArgs a, const void *ids, int ids_type, const T *grad, T *out, float *parts) {
     constexpr int COLS = 16 * W, WORDS = (W * sizeof(T) + 3) / 4;
+    // float32 numbers times this are three bfloat16 parts to the last bit, 2^-149 as well: bfloat16 ends at 2^-133.  All sums are whole
+    // multiples of 2^-149 too, so dividing by it loses nothing; where it overflows, a sum is not finite (see above).
+    constexpr float UP = 0x1p16f;
     __shared__ __align__(16) uint16_t rows_s[THREADS / 64][FIELDS][64];  // 0xFFFF: none
     __shared__ float sum_s[TILES * 16][COLS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, l16 = lane % 16, quad = lane / 16;
@@ -660,6 +664,8 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 || FIELDS > 3 ? 2 : 3) 
                     for (int m = 0; m < TILES; ++m) acc[m][i] = Operand<T>::multiply(hot[m].template get<T>(), g.template get<T>(), acc[m][i]);
                 } else {
 #pragma unroll
+                    for (int j = 0; j < 8; ++j) x[s][j][i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, x[s][j][i]) * UP);
+#pragma unroll
                     for (int part = 0; part < 3; ++part) {
 #pragma unroll
                         for (int p = 0; p < 4; ++p) {
@@ -715,7 +721,8 @@ __global__ __launch_bounds__(THREADS, TILES > 2 || W > 2 || FIELDS > 3 ? 2 : 3) 
                         for (int q = 0; q < 4; ++q)
                             if (from_col + i >= col) {
                                 float &s = sum_s[m * 16 + quad * 4 + q][from_col + i];
-                                s = w ? s + acc[m][i][q] : acc[m][i][q];
+                                const float own_sum = sizeof(T) == 4 ? acc[m][i][q] * (1.f / UP) : acc[m][i][q];
+                                s = w ? s + own_sum : own_sum;
                             }
             }
             __syncthreads();

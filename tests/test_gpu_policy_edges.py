@@ -289,3 +289,22 @@ def test_infinite_penalties_reach_repeated_tokens_only(policy, k, dtype):
         tiny = 2.0 ** -133
         y = policy.adjust_logits(torch.zeros_like(x).to(DEV), history=history.to(DEV), frequency=tiny)
         assert torch.equal(y.cpu().double(), torch.from_numpy(-tiny * ref.history_counts(history, None, 6, k)) + 0.0)
+
+
+# ---- the smallest and the largest gradients ----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,exponent", [(torch.float32, e) for e in (-112, -120, -126, -132, -140, 110, 120)] +
+                         [(torch.bfloat16, e) for e in (-120, -126, -131, 120)] + [(torch.float16, e) for e in (-14, -20, 9)])
+@pytest.mark.parametrize("n,sizes", [(64, (24,)), (300, (60,)), (5000, (24,)), (20000, (11, 6, 7)), (5000, (700,))])
+def test_embed_grad_at_the_ends_of_the_types(policy, n, sizes, dtype, exponent):
+    """Every number of a type counts with all its bits, the subnormal ones too, and a sum overflows only where it passes the
+    largest float."""
+    g = gen(n + exponent)
+    ids = torch.stack([torch.randint(0, s, (n,), generator=g) for s in sizes], -1)
+    if exponent > 100:  # a few tokens hold them, so that their sums are finite
+        ids[64:] = -1
+    grad = (randn(g, n, 24) * 2.0 ** exponent).to(dtype)
+    dw = policy.embed_grad(grad.to(DEV), ids.to(DEV), sum(sizes), fields=sizes)
+    # (sums of float16 numbers of 2^9 pass its largest, 65504, from which half a step on a rounding gives infinity)
+    close_held(dw, *ref.embed_grad(ids, grad, sizes, 1.0), dtype)
